@@ -16,6 +16,7 @@ from __future__ import annotations
 import argparse
 import concurrent.futures as cf
 import os
+import re
 import subprocess
 import sys
 from pathlib import Path
@@ -31,8 +32,8 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [*ARCH, "-O3", "-std=c++17", "--fmad=false", "-lineinfo", "-Xcompiler", "-fPIC",
               "-Xptxas", "-warn-spills", f"-I{INCLUDE}"]
 CUDA_SOURCES = ["es_abi.cu", "es_rows_f32.cu", "es_rows_f64.cu", "es_rows_f16.cu", "es_rows_bf16.cu",
-                "es_rows_full_f32.cu", "es_rows_full_f64.cu", "es_rows_full_f16.cu", "es_rows_full_bf16.cu"]
-HEADERS = sorted(CSRC.glob("*.cuh")) + [INCLUDE / "exactsample_b200.h"]
+                "es_rows_full_f32.cu", "es_rows_full_f64.cu", "es_rows_full_f16.cu", "es_rows_full_bf16.cu",
+                "es_score_abi.cu", "es_score_f32.cu", "es_score_f16.cu", "es_score_bf16.cu"]
 
 CORE_LIB = PACKAGE / "libexactsample_b200.so"
 TORCH_LIB = PACKAGE / "exactsample_cuda.so"
@@ -49,6 +50,18 @@ def _stale(target: Path, deps) -> bool:
     return any(Path(d).stat().st_mtime > t for d in deps)
 
 
+def _sources(src: Path, seen: set | None = None) -> set:
+    """A source and every header of this repository that it includes, directly or not."""
+    seen = set() if seen is None else seen
+    if src not in seen:
+        seen.add(src)
+        for name in re.findall(r'^#include "([^"]+)"', src.read_text(), flags=re.M):
+            for folder in (CSRC, INCLUDE):
+                if (folder / name).is_file():
+                    _sources(folder / name, seen)
+    return seen
+
+
 def _run(cmd):
     result = subprocess.run(cmd, capture_output=True, text=True)
     if result.returncode != 0:
@@ -63,7 +76,7 @@ def build_core(force: bool = False, verbose: bool = False) -> Path:
         src = CSRC / name
         obj = BUILD / (name + ".o")
         objects.append(obj)
-        if force or _stale(obj, [src, *HEADERS]):
+        if force or _stale(obj, _sources(src)):
             jobs.append([NVCC, *NVCC_FLAGS, "-c", str(src), "-o", str(obj)])
     if jobs:
         with cf.ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 4)) as pool:
@@ -85,7 +98,7 @@ def build_checked(force: bool = False) -> Path:
         src = CSRC / name
         obj = CHECKED_BUILD / (name + ".o")
         objects.append(obj)
-        if force or _stale(obj, [src, *HEADERS]):
+        if force or _stale(obj, _sources(src)):
             jobs.append([NVCC, *NVCC_FLAGS, "-DES_CHECKS", "-c", str(src), "-o", str(obj)])
     if jobs:
         with cf.ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 4)) as pool:

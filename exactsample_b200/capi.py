@@ -21,9 +21,11 @@ ERRORS = {0: "ES_SUCCESS", -1: "ES_ERR_ARGUMENT", -2: "ES_ERR_CAPACITY", -3: "ES
 # Every function the header declares.
 EXPORTS = ["es_workspace_bytes", "es_verify", "es_verify_timed", "es_verify_static", "es_verify_sharded",
            "es_shard_exchange_bytes", "es_shard_signal", "es_shard_wait", "es_shard_finish", "es_ipc_alloc", "es_ipc_open", "es_ipc_close", "es_ipc_free",
+           "es_token_logprobs", "es_top_logits", "es_policy_loss", "es_distill_loss",
            "es_last_error", "es_abi_version"]
 MAX_SHARDS = 8  # ES_MAX_SHARDS
 STATIC_MAX_ROWS = 4096  # ES_STATIC_MAX_ROWS
+MAX_TOP = 256  # ES_MAX_TOP
 
 
 class Tensor(ctypes.Structure):
@@ -51,6 +53,28 @@ class Shards(ctypes.Structure):
         for name in ["target", "draft", "tokens", "accepted", "status", "path", "ready"]] + [
         ("phases", ctypes.c_int32), ("pad", ctypes.c_int32), ("exchange", ctypes.c_void_p * MAX_SHARDS),
         ("scratch", ctypes.c_void_p)]
+
+
+class Rows(ctypes.Structure):
+    """es_rows: the logits a row operator works on."""
+    _fields_ = [("logits", Tensor), ("mask", Tensor), ("temperature", Tensor), ("temperature_all", ctypes.c_double)]
+
+
+def _row_args(name, doc, *fields):
+    kinds = [(f, ctypes.c_double) if f in ("clip_low", "clip_high", "kl_coef", "entropy_coef") else (f, Tensor)
+             for f in fields]
+    return type(name, (ctypes.Structure,), {"__doc__": doc, "_fields_": [("rows", Rows), *kinds]})
+
+
+LogprobArgs = _row_args("LogprobArgs", "es_logprob_args", "tokens", "logprobs", "entropy", "status", "grad",
+                        "grad_logprobs", "grad_entropy")
+TopArgs = _row_args("TopArgs", "es_top_args", "values", "ids", "rest", "status")
+PolicyArgs = _row_args("PolicyArgs", "es_policy_args", "tokens", "old_logprobs", "advantages", "ref_logprobs",
+                       "weights", "clip_low", "clip_high", "kl_coef", "entropy_coef", "loss", "logprobs", "kl",
+                       "entropy", "status", "grad")
+DistillArgs = _row_args("DistillArgs", "es_distill_args", "values", "ids", "rest", "weights", "loss", "status", "grad")
+ROW_OPERATORS = {"es_token_logprobs": LogprobArgs, "es_top_logits": TopArgs, "es_policy_loss": PolicyArgs,
+                 "es_distill_loss": DistillArgs}
 
 
 _lib = None
@@ -93,6 +117,9 @@ def load(path: str | Path | None = None) -> ctypes.CDLL:
         lib.es_ipc_close.restype = ctypes.c_int
         lib.es_ipc_free.argtypes = [ctypes.c_void_p]
         lib.es_ipc_free.restype = ctypes.c_int
+        for name, args in ROW_OPERATORS.items():
+            getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+            getattr(lib, name).restype = ctypes.c_int
         lib.es_last_error.argtypes = []
         lib.es_last_error.restype = ctypes.c_char_p
         lib.es_abi_version.argtypes = []
@@ -186,3 +213,26 @@ def args_of(tensors: dict, *, mode: int = 0, dispatch: int = 0, max_draft: int =
         setattr(args, name, describe(tensors.get(name)))
     args.mode, args.dispatch, args.max_draft, args.list_max = mode, dispatch, max_draft, list_max
     return args
+
+
+def row_operator(name: str, tensors: dict, *, stream=None, temperature_all: float = 1.0, **scalars) -> None:
+    """One of the row operators (ROW_OPERATORS) on torch tensors.
+
+    ``tensors`` maps the operator's field names, and ``logits``, ``mask`` and
+    ``temperature``, to tensors (optional ones may be absent or None);
+    ``scalars`` are es_policy_args' coefficients. ``stream`` is a
+    torch.cuda.Stream (default: current).
+    """
+    import torch
+
+    args = ROW_OPERATORS[name]()
+    for field, kind in args._fields_[1:]:
+        if kind is Tensor:
+            setattr(args, field, describe(tensors.get(field)))
+        else:
+            setattr(args, field, scalars.get(field, 0.0))
+    for field in ("logits", "mask", "temperature"):
+        setattr(args.rows, field, describe(tensors.get(field)))
+    args.rows.temperature_all = temperature_all
+    s = (stream or torch.cuda.current_stream()).cuda_stream
+    check(getattr(load(), name)(ctypes.byref(args), ctypes.c_void_p(s)))

@@ -8,9 +8,9 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
-#include <numeric>
 #include <string>
 
+#include "es_host.h"
 #include "es_kernel.cuh"
 
 namespace es {
@@ -146,64 +146,15 @@ extern template cudaError_t launch_rows<ES_BF16>(const Params&, int, cudaStream_
 namespace {
 using es::Params;
 
-thread_local std::string g_error;
+using es::host::check;
+using es::host::device_check;
+using es::host::disjoint;
+using es::host::element_size;
+using es::host::fail;
+using es::host::g_error;
+using es::host::no_internal_overlap;
+using es::host::numel;
 
-int fail(int code, const std::string& message) {
-  g_error = message;
-  return code;
-}
-
-size_t element_size(int32_t dtype) {
-  switch (dtype) {
-    case ES_F32: case ES_I32: return 4;
-    case ES_F64: case ES_I64: return 8;
-    case ES_F16: case ES_BF16: return 2;
-    case ES_U8: return 1;
-    default: return 0;
-  }
-}
-int64_t numel(const es_tensor& t) {
-  int64_t n = 1;
-  for (int d = 0; d < t.ndim; ++d) n *= t.size[d];
-  return n;
-}
-// [first byte, one past the last byte] of a strided view.
-bool extent(const es_tensor& t, uintptr_t* begin, uintptr_t* end) {
-  if (numel(t) == 0) return false;
-  const size_t e = element_size(t.dtype);
-  uintptr_t span = e;
-  for (int d = 0; d < t.ndim; ++d) span += uintptr_t(t.size[d] - 1) * uintptr_t(t.stride[d]) * e;
-  *begin = reinterpret_cast<uintptr_t>(t.data);
-  *end = *begin + span;
-  return true;
-}
-// Address intervals prove disjointness (bindings.cpp:25-37).
-bool disjoint(const es_tensor& a, const es_tensor& b) {
-  uintptr_t a0, a1, b0, b1;
-  if (!extent(a, &a0, &a1) || !extent(b, &b0, &b1)) return true;
-  return a1 <= b0 || b1 <= a0;
-}
-// A view whose elements never share an address (bindings.cpp:38-44).
-bool no_internal_overlap(const es_tensor& t) {
-  if (numel(t) <= 1) return true;
-  for (int d = 0; d < t.ndim; ++d)
-    if (t.size[d] > 1 && t.stride[d] == 0) return false;
-  if (t.ndim == 1 || t.size[0] <= 1 || t.size[1] <= 1) return true;
-  const int64_t divisor = std::gcd(t.stride[0], t.stride[1]);
-  return t.size[0] <= t.stride[1] / divisor || t.size[1] <= t.stride[0] / divisor;
-}
-bool check(const es_tensor& t, int32_t dtype, int ndim, const char* name) {
-  if (t.dtype != dtype || t.ndim != ndim || (t.data == nullptr && numel(t) != 0)) {
-    g_error = std::string(name) + " has wrong device, dtype or rank";
-    return false;
-  }
-  for (int d = 0; d < ndim; ++d)
-    if (t.stride[d] < 0 || t.size[d] < 0) {
-      g_error = std::string(name) + " has a negative stride";
-      return false;
-    }
-  return true;
-}
 bool is_logit_dtype(int32_t d) { return d == ES_F32 || d == ES_F64 || d == ES_F16 || d == ES_BF16; }
 
 // Ranks per row and the row mode.
@@ -288,18 +239,6 @@ int choose_cluster(int64_t rows, int64_t vocab, int dtype, bool full_rows, int* 
       return used;
     }
   }
-}
-
-int device_check() {
-  static thread_local int checked_device = -1;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return fail(ES_ERR_DEVICE, "no CUDA device is available");
-  if (dev == checked_device) return ES_SUCCESS;
-  int major = 0;
-  if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess || major != 10)
-    return fail(ES_ERR_DEVICE, "exactsample_b200 requires an sm_100 (B200) GPU");
-  checked_device = dev;
-  return ES_SUCCESS;
 }
 
 // `own_scratch`: 0 when the caller provides the workspace (sized by the

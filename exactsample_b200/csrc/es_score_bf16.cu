@@ -1,0 +1,9 @@
+// The row operators for bf16 logits.
+#include "es_top.cuh"
+
+namespace es {
+namespace score {
+template cudaError_t launch_loss<ES_BF16>(const LossParams&, int, int64_t, cudaStream_t);
+template cudaError_t launch_top<ES_BF16>(const TopParams&, int64_t, cudaStream_t);
+}  // namespace score
+}  // namespace es

@@ -3,8 +3,12 @@
 // every tensor is on the logits' CUDA device, describes each tensor as an
 // es_tensor, and calls es_verify on the current stream. Every other check
 // (dtype, rank, shape, capacity, alignment, aliasing) is the C ABI's, and its
-// message becomes the RuntimeError.
+// message becomes the RuntimeError. The row operators (token_logprobs,
+// top_logits, policy_loss, distill_loss) are shims of the same kind, which
+// also allocate their per-row outputs.
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -91,6 +95,135 @@ void verify_out(const Tensor& logits, const Tensor& cu_rows, const Tensor& draft
   const int result = es_verify(&a, c10::cuda::getCurrentCUDAStream(device.index()).stream());
   TORCH_CHECK(result == ES_SUCCESS, es_last_error());
 }
+
+// ---- row operators on logits ----
+// The call's device and stream, and its inputs: each is checked to be on the
+// device and tied to the stream, so that the allocator does not hand its
+// memory on while the call may still read it.
+struct RowCall {
+  const Tensor& logits;
+  c10::cuda::CUDAGuard guard;
+  c10::cuda::CUDAStream stream;
+  bool capturing;
+
+  static c10::Device device_of(const Tensor& logits) {
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, "logits must be a 2D CUDA tensor");
+    return logits.device();
+  }
+  explicit RowCall(const Tensor& l)
+      : logits(l), guard(device_of(l)), stream(c10::cuda::getCurrentCUDAStream(l.device().index())),
+        capturing(c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {}
+
+  es_tensor use(const Tensor& t, const char* name) const {
+    TORCH_CHECK(t.device() == logits.device(), name, " has wrong device, dtype or rank");
+    if (!capturing) c10::cuda::CUDACachingAllocator::recordStream(t.storage().data_ptr(), stream);
+    return describe(t);
+  }
+  es_tensor use(const OptionalTensor& t, const char* name) const {
+    return t.has_value() ? use(*t, name) : es_tensor{};
+  }
+  // A gradient tensor is written: whoever saved it for a backward pass must be able to tell.
+  es_tensor write(const OptionalTensor& t, const char* name) const {
+    if (t.has_value() && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    return use(t, name);
+  }
+  es_rows rows(const OptionalTensor& temperature, double temperature_all, const OptionalTensor& mask) const {
+    es_rows r{};
+    r.logits = use(logits, "logits");
+    r.mask = use(mask, "mask");
+    r.temperature = use(temperature, "temperature");
+    r.temperature_all = temperature_all;
+    return r;
+  }
+  Tensor floats() const { return at::empty({logits.size(0)}, logits.options().dtype(at::kFloat)); }
+  Tensor statuses() const { return at::empty({logits.size(0)}, logits.options().dtype(at::kInt)); }
+  static void done(int result) { TORCH_CHECK(result == ES_SUCCESS, es_last_error()); }
+};
+
+std::tuple<Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& tokens,
+                                                  const OptionalTensor& temperature, double temperature_all,
+                                                  const OptionalTensor& mask, const OptionalTensor& grad,
+                                                  const OptionalTensor& grad_logprobs,
+                                                  const OptionalTensor& grad_entropy) {
+  const RowCall call(logits);
+  Tensor logprobs = call.floats(), entropy = call.floats(), status = call.statuses();
+  es_logprob_args a{};
+  a.in = call.rows(temperature, temperature_all, mask);
+  a.tokens = call.use(tokens, "tokens");
+  a.logprobs = describe(logprobs);
+  a.entropy = describe(entropy);
+  a.status = describe(status);
+  a.grad = call.write(grad, "grad");
+  a.grad_logprobs = call.use(grad_logprobs, "grad_logprobs");
+  a.grad_entropy = call.use(grad_entropy, "grad_entropy");
+  call.done(es_token_logprobs(&a, call.stream.stream()));
+  return {logprobs, entropy, status};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> top_logits(const Tensor& logits, int64_t k, const OptionalTensor& temperature,
+                                                      double temperature_all, const OptionalTensor& mask) {
+  const RowCall call(logits);
+  TORCH_CHECK(k >= 1 && k <= ES_MAX_TOP, "k must be in [1, 256]");
+  Tensor values = at::empty({logits.size(0), k}, logits.options().dtype(at::kFloat));
+  Tensor ids = at::empty({logits.size(0), k}, logits.options().dtype(at::kLong));
+  Tensor rest = call.floats(), status = call.statuses();
+  es_top_args a{};
+  a.in = call.rows(temperature, temperature_all, mask);
+  a.values = describe(values);
+  a.ids = describe(ids);
+  a.rest = describe(rest);
+  a.status = describe(status);
+  call.done(es_top_logits(&a, call.stream.stream()));
+  return {values, ids, rest, status};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> policy_loss(
+    const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs, const Tensor& advantages,
+    const OptionalTensor& ref_logprobs, const OptionalTensor& weights, const OptionalTensor& temperature,
+    double temperature_all, const OptionalTensor& mask, double clip_low, double clip_high, double kl_coef,
+    double entropy_coef, const OptionalTensor& grad) {
+  const RowCall call(logits);
+  Tensor loss = call.floats(), logprobs = call.floats(), kl = call.floats(), entropy = call.floats();
+  Tensor status = call.statuses();
+  es_policy_args a{};
+  a.in = call.rows(temperature, temperature_all, mask);
+  a.tokens = call.use(tokens, "tokens");
+  a.old_logprobs = call.use(old_logprobs, "old_logprobs");
+  a.advantages = call.use(advantages, "advantages");
+  a.ref_logprobs = call.use(ref_logprobs, "ref_logprobs");
+  a.weights = call.use(weights, "weights");
+  a.clip_low = clip_low;
+  a.clip_high = clip_high;
+  a.kl_coef = kl_coef;
+  a.entropy_coef = entropy_coef;
+  a.loss = describe(loss);
+  a.logprobs = describe(logprobs);
+  a.kl = describe(kl);
+  a.entropy = describe(entropy);
+  a.status = describe(status);
+  a.grad = call.write(grad, "grad");
+  call.done(es_policy_loss(&a, call.stream.stream()));
+  return {loss, logprobs, kl, entropy, status};
+}
+
+std::tuple<Tensor, Tensor> distill_loss(const Tensor& logits, const Tensor& values, const Tensor& ids,
+                                        const OptionalTensor& rest, const OptionalTensor& weights,
+                                        const OptionalTensor& temperature, double temperature_all,
+                                        const OptionalTensor& mask, const OptionalTensor& grad) {
+  const RowCall call(logits);
+  Tensor loss = call.floats(), status = call.statuses();
+  es_distill_args a{};
+  a.in = call.rows(temperature, temperature_all, mask);
+  a.values = call.use(values, "values");
+  a.ids = call.use(ids, "ids");
+  a.rest = call.use(rest, "rest");
+  a.weights = call.use(weights, "weights");
+  a.loss = describe(loss);
+  a.status = describe(status);
+  a.grad = call.write(grad, "grad");
+  call.done(es_distill_loss(&a, call.stream.stream()));
+  return {loss, status};
+}
 }  // namespace
 
 TORCH_LIBRARY(exactsample, m) {
@@ -100,5 +233,24 @@ TORCH_LIBRARY(exactsample, m) {
       "Tensor seeds, Tensor stream_ids, Tensor positions, Tensor? mask, "
       "Tensor(a!) workspace, Tensor(b!) tokens, Tensor(c!) accepted_len, Tensor(d!) status, "
       "Tensor(e!) path_used, int mode, int dispatch, int max_draft, int list_max) -> ()");
+  m.def(
+      "token_logprobs(Tensor logits, Tensor tokens, Tensor? temperature, float temperature_all, Tensor? mask, "
+      "Tensor(a!)? grad, Tensor? grad_logprobs, Tensor? grad_entropy) -> (Tensor, Tensor, Tensor)");
+  m.def(
+      "top_logits(Tensor logits, int k, Tensor? temperature, float temperature_all, Tensor? mask) "
+      "-> (Tensor, Tensor, Tensor, Tensor)");
+  m.def(
+      "policy_loss(Tensor logits, Tensor tokens, Tensor old_logprobs, Tensor advantages, Tensor? ref_logprobs, "
+      "Tensor? weights, Tensor? temperature, float temperature_all, Tensor? mask, float clip_low, float clip_high, "
+      "float kl_coef, float entropy_coef, Tensor(a!)? grad) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def(
+      "distill_loss(Tensor logits, Tensor values, Tensor ids, Tensor? rest, Tensor? weights, Tensor? temperature, "
+      "float temperature_all, Tensor? mask, Tensor(a!)? grad) -> (Tensor, Tensor)");
 }
-TORCH_LIBRARY_IMPL(exactsample, CUDA, m) { m.impl("verify_out", &verify_out); }
+TORCH_LIBRARY_IMPL(exactsample, CUDA, m) {
+  m.impl("verify_out", &verify_out);
+  m.impl("token_logprobs", &token_logprobs);
+  m.impl("top_logits", &top_logits);
+  m.impl("policy_loss", &policy_loss);
+  m.impl("distill_loss", &distill_loss);
+}

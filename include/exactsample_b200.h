@@ -236,6 +236,120 @@ int es_ipc_open(const void* handle, void** ptr);
 int es_ipc_close(void* ptr);
 int es_ipc_free(void* ptr);
 
+/* ---- Row operators on logits (no counterpart in the reference) ----
+ *
+ * What a model's user does with the same logits besides sampling from them:
+ * the log-probabilities of tokens (es_token_logprobs), the largest logits of
+ * each row (es_top_logits), and two training losses with their gradients
+ * (es_policy_loss, es_distill_loss). Every row is its own problem, and its
+ * results do not depend on the other rows, on their number or on where the
+ * row lies in memory. The calls need no workspace, so any number of them may
+ * run at once, on any streams and in any captured graphs.
+ *
+ * Of one row, with x[j] = logits[j] / temperature over the allowed tokens
+ * (mask bit set; all without a mask):
+ *   log p[j] = x[j] - log(sum_i exp(x[i])),  entropy H = -sum_j p[j] log p[j].
+ *
+ * Statuses are per row and follow es_verify's: ES_INVALID_INPUT for a NaN or
+ * +inf logit anywhere in the row (behind the mask too), for a temperature
+ * that is not positive and finite (or beyond float32's range) and for any
+ * other per-row input that is not finite or out of range, except weights and
+ * incoming gradients, which multiply as they are; ES_NO_VALID_TOKEN
+ * when no token is allowed or every allowed one is -inf; ES_DRAFT_ZERO_PROB
+ * when a token that the operator needs has probability zero. A row whose
+ * status is not ES_OK has log-probability -inf, loss, KL and entropy 0, and
+ * a gradient of zeros.
+ *
+ * A gradient has the logits' type and shape. It may be the logits tensor
+ * itself (same address and strides): the row is then replaced by its
+ * gradient. */
+typedef struct es_rows {
+  es_tensor logits;       /* f32/f16/bf16 [rows, vocab] */
+  es_tensor mask;         /* optional i32 [rows, ceil(vocab / 32)], as in es_args */
+  es_tensor temperature;  /* optional f64 [rows] */
+  double temperature_all; /* every row's temperature when the tensor is absent */
+} es_rows;
+
+/* log p[token] and the entropy of each row. A negative token marks a row
+ * without one (padding): its logits are not read, its results are 0 and its
+ * status is ES_OK. With `grad`: the gradient of
+ *   sum over rows of grad_logprobs * log p[token] + grad_entropy * H. */
+typedef struct es_logprob_args {
+  es_rows in;
+  es_tensor tokens;         /* i64 [rows] */
+  es_tensor logprobs;       /* out f32 [rows] */
+  es_tensor entropy;        /* out f32 [rows] */
+  es_tensor status;         /* out i32 [rows] */
+  es_tensor grad;           /* optional out, the logits' type, [rows, vocab] */
+  es_tensor grad_logprobs;  /* optional f32 [rows]; only with grad; absent: zeros */
+  es_tensor grad_entropy;   /* optional f32 [rows]; only with grad; absent: zeros */
+} es_logprob_args;
+int es_token_logprobs(const es_logprob_args* args, void* stream);
+
+/* The k largest logits of each row, in descending order and the lowest id
+ * first among equal ones, and the rest's log-sum:
+ *   rest = log(sum over the other tokens of exp(x[j])), -inf if there is none.
+ * Entries beyond the row's allowed tokens have id -1 and value -inf. So does
+ * every entry of a row whose status is not ES_OK; its rest is -inf. */
+#define ES_MAX_TOP 256
+typedef struct es_top_args {
+  es_rows in;
+  es_tensor values;  /* out f32 [rows, k], 1 <= k <= ES_MAX_TOP: logits, not divided by the temperature */
+  es_tensor ids;     /* out i64 [rows, k] */
+  es_tensor rest;    /* out f32 [rows] */
+  es_tensor status;  /* out i32 [rows] */
+} es_top_args;
+int es_top_logits(const es_top_args* args, void* stream);
+
+/* The clipped policy-ratio loss of each row's token, with r = exp(log p[token]
+ * - old_logprobs), A = advantages, d = ref_logprobs - log p[token]:
+ *   kl   = exp(d) - d - 1 (0 without ref_logprobs)
+ *   loss = weights * (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ *                     + kl_coef * kl - entropy_coef * H).
+ * Where r A equals the clipped product the gradient goes through r. Negative
+ * tokens as in es_token_logprobs. With `grad`: the gradient of the losses' sum. */
+typedef struct es_policy_args {
+  es_rows in;
+  es_tensor tokens;        /* i64 [rows] */
+  es_tensor old_logprobs;  /* f32 [rows] */
+  es_tensor advantages;    /* f32 [rows] */
+  es_tensor ref_logprobs;  /* optional f32 [rows] */
+  es_tensor weights;       /* optional f32 [rows]; absent: ones */
+  double clip_low;         /* in [0, 1] */
+  double clip_high;        /* >= 0 */
+  double kl_coef;          /* finite; needs ref_logprobs unless 0 */
+  double entropy_coef;     /* finite */
+  es_tensor loss;          /* out f32 [rows] */
+  es_tensor logprobs;      /* out f32 [rows] */
+  es_tensor kl;            /* out f32 [rows] */
+  es_tensor entropy;       /* out f32 [rows] */
+  es_tensor status;        /* out i32 [rows] */
+  es_tensor grad;          /* optional out, the logits' type, [rows, vocab] */
+} es_policy_args;
+int es_policy_loss(const es_policy_args* args, void* stream);
+
+/* KL(teacher || student) of each row against a record of es_top_logits made
+ * at the same temperature. With `rest` the teacher's distribution is over
+ * its kept tokens and one bucket for all others; without it the teacher is
+ * renormalised over the kept tokens. With q the student's distribution, t the
+ * teacher's, and for the bucket q_rest = sum of q over the tokens not kept:
+ *   loss = weights * (sum_k t[k] (log t[k] - log q[k])
+ *                     + t_rest (log t_rest - log q_rest)).
+ * Entries with a negative id are unused; a row with no other entries is
+ * padding, as a negative token is for es_token_logprobs. An id given twice
+ * is ES_INVALID_INPUT. With `grad`: the gradient of the losses' sum. */
+typedef struct es_distill_args {
+  es_rows in;
+  es_tensor values;   /* f32 [rows, k], 1 <= k <= ES_MAX_TOP: the teacher's logits */
+  es_tensor ids;      /* i64 [rows, k] */
+  es_tensor rest;     /* optional f32 [rows] */
+  es_tensor weights;  /* optional f32 [rows]; absent: ones */
+  es_tensor loss;     /* out f32 [rows] */
+  es_tensor status;   /* out i32 [rows] */
+  es_tensor grad;     /* optional out, the logits' type, [rows, vocab] */
+} es_distill_args;
+int es_distill_loss(const es_distill_args* args, void* stream);
+
 /* The message of the last error returned on this thread ("" after success). */
 const char* es_last_error(void);
 
