@@ -18,13 +18,20 @@
 
 #include "es_device.cuh"
 
+#ifndef ES_SCORE_THREADS
+#define ES_SCORE_THREADS 128
+#endif
+#ifndef ES_SCORE_BLOCKS
+#define ES_SCORE_BLOCKS 5
+#endif
+
 namespace es {
 namespace score {
 
 enum Op { LOGPROB = 0, POLICY = 1, DISTILL = 2 };
+constexpr int THREADS = ES_SCORE_THREADS, WARPS = THREADS / 32;
 constexpr int MAX_RANKS = 16;   // cluster size (beyond 8: non-portable, as for the row kernels)
 constexpr int MAX_TOP = ES_MAX_TOP;
-constexpr int PIECES = 4;       // bulk copies of a slice, each with its own barrier
 constexpr int SLICE_STEP = 128; // slices are a multiple of this many tokens: whole mask words and 16-byte chunks
 constexpr float LOWEST = -3.402823466e38f;
 // Exponents (base 2) are held at or above this: 2^FAR is 0, and a product of
@@ -48,7 +55,7 @@ struct Rows {
   int64_t l_s0, l_s1;
   Grid2<const int32_t> mask;
   Column<const double> temperature;
-  double temperature_all;
+  double inv_all;  // 1 / temperature where it is one number
   int32_t vocab, ranks, slice;
 };
 
@@ -173,58 +180,139 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // ---------------------------------------------------------------------------
-// The running maximum m of the logits seen, s = sum 2^((z - m) scale) and
-// u = sum 2^d d with d = (z - m) scale: everything a row's log-sum and entropy
-// need. scale = log2(e) / temperature. The difference is taken before the
-// scaling, so that a row of the type's lowest values, or of huge ones, does
-// not overflow. s and u are held as two partial sums.
+// The running maximum m of the logits seen, s = sum 2^d and u = sum 2^d d with
+// d = (z - m) scale: everything a row's log-sum and entropy need. scale =
+// log2(e) / temperature. s and u are held as two partial sums.
+//
+// The fast form takes d = z scale - r in one instruction, with r = m scale
+// rounded to 32 bits; acc_exact afterwards makes s and u those of m itself. It
+// leaves three kinds of rows wrong, and acc_failed tells: a -inf beside an
+// entropy (0 * -inf), an r that overflows, and an r so large that its rounding
+// moves the exponents. The careful form, which subtracts first and holds
+// exponents at FAR, is right for those.
 struct Acc {
-  float m;
+  float m, r;
   float2 s, u;
 };
-__device__ __forceinline__ Acc acc_none() { return {LOWEST, {0.f, 0.f}, {0.f, 0.f}}; }
+__device__ __forceinline__ Acc acc_none() { return {-INFINITY, 0.f, {0.f, 0.f}, {0.f, 0.f}}; }
 __device__ __forceinline__ float exponent(float z, float m, float scale) {
   return max_nan(__fmul_rn(__fsub_rn(z, m), scale), FAR);
 }
-template <bool ENTROPY> __device__ __forceinline__ void acc_raise(Acc& a, float m, float scale) {
-  const float d = exponent(a.m, m, scale), f = ex2(d);
-  if (ENTROPY) a.u = mul2(both(f), fma2(both(d), a.s, a.u));
-  a.s = mul2(both(f), a.s);
-  a.m = m;
+// The largest of two chunks; a NaN may drop out here, and shows up in s.
+template <int DT> __device__ __forceinline__ float chunk_max(const uint4& p, const uint4& q) {
+  if constexpr (DT == ES_F32) {
+    const float* a = reinterpret_cast<const float*>(&p);
+    const float* b = reinterpret_cast<const float*>(&q);
+    return fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), fmaxf(fmaxf(b[0], b[1]), fmaxf(b[2], b[3])));
+  } else if constexpr (DT == ES_F16) {
+    const __half2* a = reinterpret_cast<const __half2*>(&p);
+    const __half2* b = reinterpret_cast<const __half2*>(&q);
+    const float2 m = __half22float2(__hmax2(__hmax2(__hmax2(a[0], a[1]), __hmax2(a[2], a[3])),
+                                            __hmax2(__hmax2(b[0], b[1]), __hmax2(b[2], b[3]))));
+    return fmaxf(m.x, m.y);
+  } else {
+    const __nv_bfloat162* a = reinterpret_cast<const __nv_bfloat162*>(&p);
+    const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&q);
+    const float2 m = __bfloat1622float2(__hmax2(__hmax2(__hmax2(a[0], a[1]), __hmax2(a[2], a[3])),
+                                                __hmax2(__hmax2(b[0], b[1]), __hmax2(b[2], b[3]))));
+    return fmaxf(m.x, m.y);
+  }
 }
-template <int N, bool ENTROPY> __device__ __forceinline__ void acc_chunk(Acc& a, const float2* v, float scale) {
-  float top = fmaxf(v[0].x, v[0].y);  // a NaN drops out here and shows up in s
-#pragma unroll
-  for (int i = 1; i < N / 2; ++i) top = fmaxf(top, fmaxf(v[i].x, v[i].y));
-  if (top > a.m) acc_raise<ENTROPY>(a, top, scale);
-  const float2 nm = both(-a.m), sc = both(scale);
+// The same, and NaN if there is one.
+template <int DT> __device__ __forceinline__ float chunk_max_nan(const uint4& q) {
+  if constexpr (DT == ES_F32) {
+    return max_nan(max_nan(__uint_as_float(q.x), __uint_as_float(q.y)), max_nan(__uint_as_float(q.z), __uint_as_float(q.w)));
+  } else if constexpr (DT == ES_F16) {
+    const __half2* h = reinterpret_cast<const __half2*>(&q);
+    const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return __half2float(__hmax_nan(__low2half(m), __high2half(m)));
+  } else {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return __bfloat162float(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m)));
+  }
+}
+template <int N, bool ENTROPY>
+__device__ __forceinline__ void acc_fast(Acc& a, const float2* v, float top, float scale) {
+  if (top > a.m) {
+    const float r = __fmul_rn(top, scale), d = __fsub_rn(a.r, r), f = a.m == -INFINITY ? 0.f : ex2(d);
+    if (ENTROPY) a.u = mul2(both(f), fma2(both(fmaxf(d, FAR)), a.s, a.u));
+    a.s = mul2(both(f), a.s);
+    a.m = top;
+    a.r = r;
+  }
+  const float2 nr = both(-a.r), sc = both(scale);
 #pragma unroll
   for (int i = 0; i < N / 2; ++i) {
-    float2 d = mul2(add2(v[i], nm), sc);
-    if (ENTROPY) d = make_float2(max_nan(d.x, FAR), max_nan(d.y, FAR));
+    const float2 d = fma2(v[i], sc, nr);
     const float2 e = make_float2(ex2(d.x), ex2(d.y));
     a.s = add2(a.s, e);
     if (ENTROPY) a.u = fma2(e, d, a.u);
   }
 }
+template <int N, bool ENTROPY>
+__device__ __forceinline__ void acc_careful(Acc& a, const float2* v, float top, float scale) {
+  top = fmaxf(top, LOWEST);
+  if (top > a.m) {
+    const float d = a.m == -INFINITY ? FAR : exponent(a.m, top, scale), f = ex2(d);
+    if (ENTROPY) a.u = mul2(both(f), fma2(both(d), a.s, a.u));
+    a.s = mul2(both(f), a.s);
+    a.m = top;
+  }
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    const float2 d = make_float2(exponent(v[i].x, a.m, scale), exponent(v[i].y, a.m, scale));
+    const float2 e = make_float2(ex2(d.x), ex2(d.y));
+    a.s = add2(a.s, e);
+    if (ENTROPY) a.u = fma2(e, d, a.u);
+  }
+}
+constexpr float LARGE_R = 65536.f;  // its rounding is 2^-8 at most, which acc_exact takes back
+template <bool ENTROPY> __device__ __forceinline__ bool acc_failed(const Acc& a) {
+  const float s = a.s.x + a.s.y, u = a.u.x + a.u.y;
+  return !(fabsf(a.r) <= LARGE_R) || !(s < INFINITY) || (ENTROPY && !(fabsf(u) < INFINITY));
+}
 
-// What one rank knows of its slice.
+// What one rank knows of its slice: s and u against the maximum m.
 struct Record {
   float m, s, u;
-  uint32_t bad;  // a NaN or +inf behind the mask, a repeated id, a copy that did not arrive
+  uint32_t flags;
 };
-__device__ __forceinline__ Record merge(Record a, Record b, float scale) {
-  Record r;
-  r.m = fmaxf(a.m, b.m);
-  const float da = exponent(a.m, r.m, scale), db = exponent(b.m, r.m, scale);
-  const float fa = ex2(da), fb = ex2(db);
-  r.s = __fadd_rn(__fmul_rn(fa, a.s), __fmul_rn(fb, b.s));
-  r.u = __fadd_rn(__fmul_rn(fa, __fadd_rn(a.u, __fmul_rn(da, a.s))), __fmul_rn(fb, __fadd_rn(b.u, __fmul_rn(db, b.s))));
-  r.bad = a.bad | b.bad;
+// BAD: an invalid row (a NaN or +inf, a repeated id, a copy that did not
+// arrive). CAREFUL: the gradient needs the careful form too. FULL: top_rows'
+// lists did not fit.
+constexpr uint32_t BAD = 1, CAREFUL = 2, FULL = 4;
+
+// s and u against m itself: with m scale = r + rest, 2^(z scale - r) is 2^rest
+// times too large and its exponent off by rest (at most 2^-8).
+template <bool ENTROPY> __device__ __forceinline__ Record acc_exact(const Acc& a, float scale, bool careful) {
+  const float rest = careful || a.m == -INFINITY ? 0.f : __fmaf_rn(a.m, scale, -a.r), f = ex2(-rest);
+  const float s = __fadd_rn(a.s.x, a.s.y), u = __fadd_rn(a.u.x, a.u.y);
+  return {fmaxf(a.m, LOWEST), __fmul_rn(f, s), ENTROPY ? __fmul_rn(f, __fmaf_rn(-rest, s, u)) : 0.f, careful ? CAREFUL : 0u};
+}
+// The records of a warp's lanes as one. Every warp of a block takes it, not in
+// a branch: where the compiler cannot tell that a whole warp is there, a
+// shuffle costs about 240 cycles instead of 25 (3,600 for these 16, measured).
+template <bool ENTROPY> __device__ __forceinline__ Record warp_record(Record r, float scale) {
+  const float m = warp_all(r.m, [](float a, float b) { return fmaxf(a, b); });
+  const float d = exponent(r.m, m, scale), f = ex2(d);
+  const auto sum = [](float a, float b) { return __fadd_rn(a, b); };
+  if (ENTROPY) r.u = warp_all(__fmul_rn(f, __fmaf_rn(d, r.s, r.u)), sum);
+  r.s = warp_all(__fmul_rn(f, r.s), sum);
+  r.m = m;
+  r.flags = __reduce_or_sync(0xffffffffu, r.flags);
   return r;
 }
-__device__ __forceinline__ Record shfl_record(Record r, int o) {
-  return {shfl_xor(r.m, o), shfl_xor(r.s, o), shfl_xor(r.u, o), shfl_xor(r.bad, o)};
+
+// This lane's of `count` records, empty beyond them.
+__device__ __forceinline__ Record lane_record(const Record* records, int count) {
+  const bool mine = lane_id() < count;
+  Record r = records[mine ? lane_id() : 0];
+  r.m = mine ? r.m : LOWEST;
+  r.s = mine ? r.s : 0.f;
+  r.u = mine ? r.u : 0.f;
+  r.flags = mine ? r.flags : 0u;
+  return r;
 }
 
 // ---------------------------------------------------------------------------
@@ -233,161 +321,300 @@ __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------
-// A rank's slice of the row in shared memory. Element i lies at
-// base + shift + i * sizeof(T), where shift is the row's misalignment against
-// 16 bytes, so that the aligned middle of the slice comes by bulk copies and
-// only the ragged ends by plain loads. Rows without unit stride are gathered.
+// 1 / temperature in two floats, and log2(e) / temperature.
+struct Scale {
+  float log2;      // of the exponents
+  float hi, lo;    // 1 / temperature
+  bool bad;        // not positive and finite, or beyond float32's range
+};
+__device__ __forceinline__ Scale row_scale(const Rows& in, int64_t row) {
+  const double inv = in.temperature.p ? 1. / in.temperature[row] : in.inv_all;
+  Scale s;
+  s.log2 = float(LOG2E * inv);
+  s.bad = !(s.log2 >= 1.17549435e-38f && s.log2 <= 3.402823466e38f);
+  s.hi = float(inv);
+  s.lo = float(inv - double(s.hi));
+  if (s.bad) s = {float(LOG2E), 1.f, 0.f, true};
+  return s;
+}
+
+// ---------------------------------------------------------------------------
+// 16 bytes at `shift` bytes past p, from two aligned pieces.
+template <int SIZE> __device__ __forceinline__ uint4 shifted_chunk(const uint4* p, uint32_t shift) {
+  const uint4 a = p[0], b = p[1];
+  uint32_t w[7] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z};
+  if (shift & 8) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 2];
+    w[5] = b.w;
+  }
+  if (shift & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  if (SIZE == 2 && (shift & 2)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A rank's slice of the row in shared memory, element i at base + i sizeof(T).
+// The aligned middle of the slice comes by one bulk copy and only the ragged
+// ends by plain loads: a row that does not start on 16 bytes lands as far off
+// them and is then moved into place. Rows without unit stride are gathered.
 template <int DT> struct Slice {
   using T = typename Elem<DT>::T;
   static constexpr int N = Elem<DT>::N;
   uint8_t* base;
   uint64_t* bar;
-  uint32_t shift, at, piece;  // the bulk part starts at byte `at`, in pieces of `piece` bytes
-  int n, chunks, pieces, ready;
-  bool late;  // a copy did not arrive in time
+  uint32_t shift;
+  int n, chunks;
+  bool bulk;
 
-  __device__ __forceinline__ T& operator[](int i) const { return reinterpret_cast<T*>(base + shift)[i]; }
+  __device__ __forceinline__ T& operator[](int i) const { return reinterpret_cast<T*>(base)[i]; }
+  __device__ __forceinline__ uint4& chunk(int c) const { return reinterpret_cast<uint4*>(base)[c]; }
 
   // All threads; ends with a block barrier.
-  __device__ __forceinline__ void load(const Rows& in, int64_t row, int begin, int count, uint8_t* buffer, uint64_t* bars) {
+  __device__ __forceinline__ void load(const Rows& in, int64_t row, int begin, int count, uint8_t* buffer, uint64_t* barrier) {
     base = buffer;
-    bar = bars;
+    bar = barrier;
     n = count;
     chunks = (n + N - 1) / N;
-    ready = 0;
-    late = false;
     const T* src = static_cast<const T*>(in.logits) + row * in.l_s0 + int64_t(begin) * in.l_s1;
     const int tid = threadIdx.x;
-    pieces = 0;
-    at = 0;
-    piece = 4096;
+    bulk = false;
+    shift = 0;
     if (in.l_s1 == 1) {
       const uint32_t bytes = uint32_t(n) * sizeof(T);
       shift = uint32_t(reinterpret_cast<uintptr_t>(src)) & 15;
-      const uint32_t lead = min((16 - shift) & 15, bytes), bulk = (bytes - lead) & ~15u;
-      at = shift + lead;
-      piece = max(4096u, (bulk / PIECES + 4095) & ~4095u);
-      pieces = int((bulk + piece - 1) / piece);
-      if (tid == 0) {
-        for (int i = 0; i < pieces; ++i) mbar_init(bar + i, 1);
-        mbar_init_fence();
-        const uint8_t* g = reinterpret_cast<const uint8_t*>(src) + lead;
-        for (int i = 0; i < pieces; ++i) {
-          const uint32_t size = min(piece, bulk - i * piece);
-          mbar_arrive_expect_tx(bar + i, size);
-          bulk_load(base + at + i * piece, g + i * piece, size, bar + i);
-        }
+      const uint32_t lead = min((16 - shift) & 15, bytes), middle = (bytes - lead) & ~15u;
+      bulk = middle > 0;
+      if (tid == 0 && bulk) {
+        mbar_init(bar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        mbar_arrive_expect_tx(bar, middle);
+        bulk_load(base + shift + lead, reinterpret_cast<const uint8_t*>(src) + lead, middle, bar);
       }
-      const int head = int(lead / sizeof(T)), tail = int((lead + bulk) / sizeof(T));
-      if (tid < head) (*this)[tid] = src[tid];
-      if (tid >= 32 && tail + tid - 32 < n) (*this)[tail + tid - 32] = src[tail + tid - 32];
+      T* landed = reinterpret_cast<T*>(base + shift);
+      const int head = int(lead / sizeof(T)), tail = int((lead + middle) / sizeof(T));
+      if (tid < head) landed[tid] = src[tid];
+      if (tid >= 32 && tail + tid - 32 < n) landed[tail + tid - 32] = src[tail + tid - 32];
     } else {
-      shift = 0;
       for (int i = tid; i < n; i += THREADS) (*this)[i] = src[i * in.l_s1];
     }
-    if (tid < chunks * N - n) (*this)[n + tid] = Elem<DT>::put(-INFINITY);  // the last chunk's unused places
+    if (tid < chunks * N - n)  // the last chunk's unused places
+      reinterpret_cast<T*>(base + shift)[n + tid] = Elem<DT>::put(-INFINITY);
     __syncthreads();
   }
-  // Until the first `end` bytes of the buffer are there.
-  __device__ __forceinline__ void wait(uint32_t end) {
-    while (ready < pieces && at + ready * piece < end) {
+  // All threads: the slice is there and in place. False if it did not come in time.
+  __device__ __forceinline__ bool wait() const {
+    bool came = true;
+    if (bulk) {
       uint32_t spins = 0;
-      while (!mbar_try_wait(bar + ready, 0))
+      while (!mbar_try_wait(bar, 0))
         if (++spins >= WAIT_LIMIT) {
-          late = true;
+          came = false;
           break;
         }
-      ++ready;
     }
-  }
-  __device__ __forceinline__ void wait_all() { wait(0xffffffffu); }
-  // Chunk c (elements [c N, c N + N)). A shifted chunk is cut out of two aligned ones.
-  __device__ __forceinline__ uint4 chunk(int c) const {
-    const uint4* p = reinterpret_cast<const uint4*>(base) + c;
-    uint4 a = p[0];
     if (shift) {
-      const uint4 b = p[1];
-      uint32_t w[7] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z};
-      uint32_t last = b.w;
-      if (shift & 8) {
-#pragma unroll
-        for (int i = 0; i < 5; ++i) w[i] = w[i + 2];
-        w[5] = last;
+      // Chunks move down by less than one chunk, THREADS at a time: a round
+      // reads only what no earlier round wrote.
+      for (int first = 0; first < chunks; first += THREADS) {
+        const int c = first + int(threadIdx.x);
+        uint4 q;
+        if (c < chunks) q = shifted_chunk<sizeof(T)>(&chunk(c), shift);
+        __syncthreads();
+        if (c < chunks) chunk(c) = q;
       }
-      if (shift & 4) {
-#pragma unroll
-        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-      }
-      if (sizeof(T) == 2 && (shift & 2)) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
-      }
-      a = make_uint4(w[0], w[1], w[2], w[3]);
+      __syncthreads();
     }
-    return a;
-  }
-  __device__ __forceinline__ void set_chunk(int c, const uint4& q) const {
-    if (shift == 0) {
-      reinterpret_cast<uint4*>(base)[c] = q;
-    } else {
-      const T* v = reinterpret_cast<const T*>(&q);
-#pragma unroll
-      for (int i = 0; i < N; ++i) (*this)[c * N + i] = v[i];
-    }
+    return came;
   }
 };
 
-// Masked tokens of a chunk become -inf; returns whether one of them is NaN or +inf.
-template <int DT> __device__ __forceinline__ bool mask_chunk(const int32_t* words, int64_t stride, int first, float2* v) {
-  constexpr int N = Elem<DT>::N;
-  const uint32_t bits = uint32_t(words[(first >> 5) * stride]) >> (first & 31);
-  bool bad = false;
+// Masked rows hold the logits in the sums at or above this, where 2^d is 0 but
+// 0 times d is too. Rows with a real logit near it, or a scale that brings it
+// near 0, take the careful form (SMALL_SCALE, LARGE_R).
+constexpr float MASKED = -1e30f;
+constexpr float SMALL_SCALE = 1e-20f;
+// The N mask bits of a chunk.
+template <int DT> __device__ __forceinline__ uint32_t mask_bits(const int32_t* words, int64_t stride, int first) {
+  return uint32_t(words[(first >> 5) * stride]) >> (first & 31);
+}
+template <int DT> __device__ __forceinline__ void mask_chunk(uint32_t bits, float value, float2* v) {
 #pragma unroll
-  for (int i = 0; i < N / 2; ++i) {
-    if (!(bits >> (2 * i) & 1)) {
-      bad |= !(v[i].x < INFINITY);
-      v[i].x = -INFINITY;
+  for (int i = 0; i < Elem<DT>::N / 2; ++i) {
+    if (!(bits >> (2 * i) & 1)) v[i].x = value;
+    if (!(bits >> (2 * i + 1) & 1)) v[i].y = value;
+  }
+}
+// Whether a chunk holds a NaN or +inf.
+template <int DT> __device__ __forceinline__ bool chunk_bad(const float2* v) {
+  float top = max_nan(v[0].x, v[0].y);
+#pragma unroll
+  for (int i = 1; i < Elem<DT>::N / 2; ++i) top = max_nan(top, max_nan(v[i].x, v[i].y));
+  return !(top < INFINITY);
+}
+template <int N> __device__ __forceinline__ float max_of(const float2* v) {
+  float top = fmaxf(v[0].x, v[0].y);
+#pragma unroll
+  for (int i = 1; i < N / 2; ++i) top = fmaxf(top, fmaxf(v[i].x, v[i].y));
+  return top;
+}
+
+// This thread's share of a slice as a Record: the fast form, or where that
+// fails the careful one. `mask` is the slice's first word, or null.
+template <int DT, bool ENTROPY, bool HAS_MASK>
+__device__ __forceinline__ Record sum_slice(const Slice<DT>& slice, const int32_t* mask, int64_t stride, float scale) {
+  constexpr int N = Elem<DT>::N;
+  const int tid = threadIdx.x;
+  bool bad = false;
+  Acc a = acc_none();
+  if (HAS_MASK) {
+    for (int c = tid; c < slice.chunks; c += THREADS) {
+      float2 v[N / 2];
+      unpack<DT>(slice.chunk(c), v);
+      bad |= chunk_bad<DT>(v);
+      mask_chunk<DT>(mask_bits<DT>(mask, stride, c * N), -INFINITY, v);
+      const float top = max_of<N>(v);
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) v[i] = make_float2(fmaxf(v[i].x, MASKED), fmaxf(v[i].y, MASKED));
+      acc_fast<N, ENTROPY>(a, v, top, scale);
     }
-    if (!(bits >> (2 * i + 1) & 1)) {
-      bad |= !(v[i].y < INFINITY);
-      v[i].y = -INFINITY;
+  } else {
+    // Two chunks a step: one look at the maximum for both, and independent
+    // loads and exponentials.
+    int c = tid;
+    for (; c + THREADS < slice.chunks; c += 2 * THREADS) {
+      const uint4 q0 = slice.chunk(c), q1 = slice.chunk(c + THREADS);
+      float2 v[N];
+      unpack<DT>(q0, v);
+      unpack<DT>(q1, v + N / 2);
+      acc_fast<2 * N, ENTROPY>(a, v, chunk_max<DT>(q0, q1), scale);
+    }
+    if (c < slice.chunks) {
+      const uint4 q = slice.chunk(c);
+      float2 v[N / 2];
+      unpack<DT>(q, v);
+      acc_fast<N, ENTROPY>(a, v, chunk_max<DT>(q, q), scale);
     }
   }
-  return bad;
+  const bool failed = acc_failed<ENTROPY>(a) || scale < SMALL_SCALE;
+  if (failed) {
+    a = acc_none();
+    for (int c = tid; c < slice.chunks; c += THREADS) {
+      float2 v[N / 2];
+      unpack<DT>(slice.chunk(c), v);
+      if (HAS_MASK) mask_chunk<DT>(mask_bits<DT>(mask, stride, c * N), -INFINITY, v);
+      acc_careful<N, ENTROPY>(a, v, max_of<N>(v), scale);
+    }
+  }
+  Record r = acc_exact<ENTROPY>(a, scale, failed);
+  if (bad) r.flags |= BAD;
+  return r;
 }
 
 // ---------------------------------------------------------------------------
-// One row's scalars for the gradient: every token's is e (a + b d) with
-// d = (z - m) scale and e = 2^d; the row's token has its own.
+// Row scalars. They sit between the row's two passes on one thread, and FP64
+// there costs about 4 us a row (FP64 operations are several times slower to
+// follow one another than FP32's). Logarithms are held as a float and the
+// float it is off by instead, so that differences of them lose no digits.
+struct Pair {
+  float hi, lo;
+};
+__device__ __forceinline__ Pair pair_sum(Pair a, Pair b) {
+  const float hi = __fadd_rn(a.hi, b.hi), t = __fsub_rn(hi, a.hi);  // hi + rest is a.hi + b.hi exactly
+  const float rest = __fadd_rn(__fsub_rn(a.hi, __fsub_rn(hi, t)), __fsub_rn(b.hi, t));
+  return {hi, __fadd_rn(rest, __fadd_rn(a.lo, b.lo))};
+}
+__device__ __forceinline__ Pair negated(Pair a) { return {-a.hi, -a.lo}; }
+__device__ __forceinline__ float value_of(Pair a) { return __fadd_rn(a.hi, a.lo); }
+// (a - b) / temperature.
+__device__ __forceinline__ Pair scaled_gap(float a, float b, const Scale& s) {
+  const float hi = __fsub_rn(a, b), t = __fadd_rn(hi, b);
+  const float rest = __fsub_rn(__fsub_rn(a, t), __fsub_rn(b, __fsub_rn(t, hi)));  // a - b = hi + rest
+  const float p = __fmul_rn(hi, s.hi);
+  return {p, __fmaf_rn(hi, s.hi, -p) + (hi * s.lo + rest * s.hi)};
+}
+// log(s) for a positive, normal s, to about 2^-32: with s = 2^k f, f in
+// [3/4, 3/2), log f = 2 artanh(q) = 2 (q + q^3 / 3 + q^5 / 5 + ...) at
+// q = (f - 1) / (f + 1), |q| <= 1/5.
+__device__ __forceinline__ Pair log_pair(float s) {
+  const int bits = __float_as_int(s), k = (bits - 0x3f400000) >> 23;
+  const float f = __int_as_float(bits - (k << 23));
+  const float num = f - 1.f, den = f + 1.f, den_lo = f - (den - 1.f), inv = __frcp_rn(den);
+  const float q = __fmul_rn(num, inv), q_lo = (__fmaf_rn(-q, den, num) - q * den_lo) * inv;
+  const float u = q * q;
+  const float series = q * u * __fmaf_rn(u, __fmaf_rn(u, __fmaf_rn(u, __fmaf_rn(u, 2.f / 11.f, 2.f / 9.f), 2.f / 7.f), 2.f / 5.f), 2.f / 3.f);
+  constexpr float LN2_HI = 0.693145751953125f;  // 16 bits: its products with k are exact
+  constexpr float LN2_LO = float(LN2 - double(LN2_HI));
+  return pair_sum({float(k) * LN2_HI, 0.f}, {2.f * q, __fmaf_rn(2.f, q_lo, __fmaf_rn(float(k), LN2_LO, series))});
+}
+// exp(x) - 1 - x, from its series where the difference would lose digits.
+__device__ __forceinline__ float exp_beyond_first_order(float x, float exp_less_one) {
+  if (fabsf(x) >= 1.f) return exp_less_one - x;
+  float sum = 1.f / 3628800.f / 132.f;
+  constexpr float C[10] = {1.f / 39916800.f, 1.f / 3628800.f, 1.f / 362880.f, 1.f / 40320.f, 1.f / 5040.f,
+                           1.f / 720.f, 1.f / 120.f, 1.f / 24.f, 1.f / 6.f, 1.f / 2.f};
+#pragma unroll
+  for (int i = 0; i < 10; ++i) sum = __fmaf_rn(sum, x, C[i]);
+  return sum * x * x;
+}
+
+// One row's scalars for the gradient: every token's is 2^d (a + b d), in the
+// fast form with d = z scale - r, in the careful form with d = (z - m) scale;
+// the row's token has its own.
 struct RowScalars {
-  float m, a, b, token_grad;
-  int32_t zero;  // a row without a gradient
-  // Distillation: the kept tokens' gradients are w (q - t).
-  double top, log_total, teacher, w;
+  float m, r, a, b, token_grad;
+  int32_t zero, careful;   // a row without a gradient; the form
+  float w, inv_q, inv_t;   // distillation: the kept tokens' gradients are w (q inv_q - t inv_t)
 };
 
 struct Shared {
-  uint64_t bar[PIECES];
+  uint64_t bar;
   Record inbox[MAX_RANKS];
   Record warps[WARPS];
   RowScalars row;
+  float sums[WARPS][3];  // distillation: kept_sums by warp
 };
-// Distillation: the teacher's entries and, a bit per token of the slice, which ids were seen.
+
+// Distillation: the teacher's entries, k of each (rounded up to whole warps):
+// their ids (-1: unused) and logits, the row's own logits at them, and the
+// exponentials of both; then a bit per token of the slice, which ids were seen.
 struct Kept {
-  float value[MAX_TOP], x[MAX_TOP];
-  int32_t id[MAX_TOP];  // -1: unused
+  int32_t* id;
+  float *value, *x, *t, *q;
+  uint32_t* seen;
+  static constexpr __host__ __device__ size_t bytes(int k, int slice) {
+    return size_t((k + 31) / 32 * 32) * 20 + size_t(slice) / 8;
+  }
+  __device__ Kept(uint8_t* p, int k) {
+    const int width = (k + 31) / 32 * 32;
+    id = reinterpret_cast<int32_t*>(p);
+    value = reinterpret_cast<float*>(id + width);
+    x = value + width;
+    t = x + width;
+    q = t + width;
+    seen = reinterpret_cast<uint32_t*>(q + width);
+  }
 };
 
-template <int DT> __host__ __device__ constexpr size_t loss_smem(int slice, int op) {
-  return sizeof(Shared) + (op == DISTILL ? sizeof(Kept) + size_t(slice) / 8 : 0) + 16 +
-         size_t(slice) * sizeof(typename Elem<DT>::T) + 32;
+constexpr size_t SHARED_BYTES = (sizeof(Shared) + 15) / 16 * 16;
+// The buffer of a slice and what a shifted one reaches beyond it.
+template <int DT> __host__ __device__ constexpr size_t slice_bytes(int slice) {
+  return size_t(slice) * sizeof(typename Elem<DT>::T) + 32;
+}
+template <int DT> __host__ __device__ constexpr size_t loss_smem(int slice, int k) {
+  return SHARED_BYTES + slice_bytes<DT>(slice) + (k > 0 ? Kept::bytes(k, slice) : 0);
 }
 
-__device__ __forceinline__ double warp_sum(double v) {
-  return warp_all(v, [](double a, double b) { return a + b; });
+__device__ __forceinline__ float warp_sum(float v) {
+  return warp_all(v, [](float a, float b) { return __fadd_rn(a, b); });
 }
-__device__ __forceinline__ double warp_max(double v) {
-  return warp_all(v, [](double a, double b) { return fmax(a, b); });
+__device__ __forceinline__ float warp_top(float v) {
+  return warp_all(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
 template <int DT, int OP, bool GRAD> struct LossRow {
@@ -434,284 +661,362 @@ template <int DT, int OP, bool GRAD> struct LossRow {
     if (OP == POLICY) p.kl[row] = kl;
   }
 
-  // Warp 0, from the merged records: the token's log-probability and what
-  // hangs on it. The row's scalars are in FP64: they cost one warp a few
-  // hundred instructions, and differences of logarithms lose no digits.
-  __device__ __forceinline__ void token_scalars(Shared& sh, float m, double s, double u, bool bad, double temperature,
-                                                int64_t token, float z, bool token_allowed) {
-    double log_s = log(s), lp = (double(z) - m) / temperature - log_s, h = log_s - u / s * LN2;
-    int status = ES_OK;
-    bad |= !(s < double(INFINITY)) || m == INFINITY || token >= p.in.vocab;  // a NaN logit makes s NaN
-    double slope = 0, on_entropy = 0, loss = 0, kl = 0;  // of lp and of h
+  // What the row's scalars need besides the sums, fetched while the row is on its way.
+  struct Inputs {
+    int64_t token;
+    float z;        // the token's logit
+    bool allowed;
+    float first, second, ref, w;  // logprob: the two incoming gradients; policy: old log-probability
+                                  // and advantage; distillation: the teacher's rest
+  };
+
+  // a and b as 2^d (a + b d) needs them: with m scale = r + rest, 2^d of the
+  // fast form is 2^rest times 2^((z - m) scale), and its d is off by rest.
+  __device__ __forceinline__ void set_scalars(RowScalars& r, float m, float scale, float a, float b, bool careful) const {
+    r.m = m;
+    r.r = __fmul_rn(m, scale);
+    r.careful = careful || !(fabsf(r.r) <= LARGE_R);
+    const float rest = r.careful ? 0.f : __fmaf_rn(m, scale, -r.r), x = rest * float(LN2);
+    const float f = 1.f - x * (1.f - 0.5f * x);
+    r.a = f * (a - b * rest);
+    r.b = f * b;
+  }
+
+  // One thread, from the merged records: the token's log-probability and what
+  // hangs on it.
+  __device__ __forceinline__ void token_scalars(Shared& sh, float m, float s, float u, uint32_t flags, const Scale& scale,
+                                                const Inputs& in) {
+    const Pair log_s = log_pair(s), lp = pair_sum(scaled_gap(in.z, m, scale), negated(log_s));
+    const float inv_s = __frcp_rn(s), gap = u * inv_s * float(LN2);  // log(s) - h
+    const float h = value_of({log_s.hi, log_s.lo - gap});
+    // A NaN logit makes s NaN, +inf the maximum.
+    bool bad = (flags & BAD) || !(s < INFINITY) || m == INFINITY || in.token >= p.in.vocab;
+    float slope = 0.f, on_entropy = 0.f, loss = 0.f, kl = 0.f;  // gradients of lp and of h
     if (OP == LOGPROB) {
-      if (GRAD) {
-        slope = p.grad_logprobs.p ? p.grad_logprobs[row] : 0.f;
-        on_entropy = p.grad_entropy.p ? p.grad_entropy[row] : 0.f;
-      }
+      slope = in.first;
+      on_entropy = in.second;
     } else {
-      const double old = p.old_logprobs[row], adv = p.advantages[row], w = p.weights.p ? p.weights[row] : 1.f;
-      const double r = exp(lp - old), plain = r * adv, clipped = fmin(fmax(r, p.ratio_low), p.ratio_high) * adv;
-      loss = -fmin(plain, clipped);
-      slope = plain <= clipped ? -plain : 0.;
-      bad |= !isfinite(old) || !isfinite(adv);
+      const float ratio = expf((lp.hi - in.first) + lp.lo);
+      // In 64 bits: where the ratio meets a border.
+      const double r = ratio, clipped = fmin(fmax(r, p.ratio_low), p.ratio_high);
+      const bool through = r * in.second <= clipped * in.second;
+      loss = through ? -ratio * in.second : float(-clipped * in.second);
+      slope = through ? -ratio * in.second : 0.f;
+      bad |= !isfinite(in.first) || !isfinite(in.second);
       if (p.ref_logprobs.p) {
-        const double ref = p.ref_logprobs[row], d = ref - lp, rise = expm1(d);
-        kl = rise - d;
-        loss += p.kl_coef * kl;
-        slope -= p.kl_coef * rise;
-        bad |= !isfinite(ref);
+        const float x = (in.ref - lp.hi) - lp.lo, rise = expm1f(x);
+        kl = exp_beyond_first_order(x, rise);
+        loss += float(p.kl_coef) * kl;
+        slope -= float(p.kl_coef) * rise;
+        bad |= !isfinite(in.ref);
       }
-      loss -= p.entropy_coef * h;
-      bad |= s > 0 && isfinite(lp) && !(isfinite(float(loss)) && isfinite(float(slope)) && isfinite(float(kl)));
+      loss -= float(p.entropy_coef) * h;
+      bad |= s > 0.f && isfinite(lp.hi) && !(isfinite(loss) && isfinite(slope) && isfinite(kl));
       // Weights multiply as they are: an infinite or NaN one (an overflowed
       // loss scale) shows in the loss and the gradient.
-      loss *= w;
-      slope *= w;
-      on_entropy = -p.entropy_coef * w;
+      loss *= in.w;
+      slope *= in.w;
+      on_entropy = -float(p.entropy_coef) * in.w;
     }
+    int status = ES_OK;
     if (bad) status = ES_INVALID_INPUT;
-    else if (s == 0) status = ES_NO_VALID_TOKEN;
-    else if (z == -INFINITY || !token_allowed) status = ES_DRAFT_ZERO_PROB;
-    if (lane_id() != 0) return;
+    else if (s == 0.f) status = ES_NO_VALID_TOKEN;
+    else if (in.z == -INFINITY || !in.allowed) status = ES_DRAFT_ZERO_PROB;
     const bool ok = status == ES_OK;
-    if (rank == 0) outputs(status, ok ? float(loss) : 0.f, ok ? float(lp) : -INFINITY, ok ? float(kl) : 0.f, ok ? float(h) : 0.f);
+    if (rank == 0)
+      outputs(status, ok ? loss : 0.f, ok ? value_of(lp) : -INFINITY, ok ? kl : 0.f, ok ? h : 0.f);
     if (GRAD) {
-      slope /= temperature;
-      on_entropy /= temperature;
+      slope *= scale.hi;
+      on_entropy *= scale.hi;
       RowScalars& r = sh.row;
       r.zero = !ok;
-      r.m = m;
-      // slope (1[j = t] - p_j) - on_entropy p_j (log p_j + h), with p_j = e / s
-      // and log p_j = d ln 2 - log s.
-      r.a = float(-(slope + on_entropy * (h - log_s)) / s);
-      r.b = float(-on_entropy * LN2 / s);
-      r.token_grad = float(-slope * expm1(lp) - on_entropy * exp(lp) * (lp + h));
+      // slope (1[j = t] - p_j) - on_entropy p_j (log p_j + h), with p_j = 2^d / s,
+      // log p_j = d ln 2 - log s and h = log s - gap.
+      set_scalars(r, m, scale.log2, -(slope - on_entropy * gap) * inv_s, -on_entropy * float(LN2) * inv_s,
+                  flags & CAREFUL || scale.log2 < SMALL_SCALE);
+      r.token_grad = -slope * expm1f(value_of(lp)) - on_entropy * expf(value_of(lp)) * (value_of(lp) + h);
     }
   }
 
-  // Warp 0, from the merged records of the tokens not kept (m, s): the two
-  // distributions over the kept tokens and the bucket.
-  __device__ __forceinline__ void distill_scalars(Shared& sh, const Kept& kept, float m, double s, bool bad,
-                                                  double temperature) {
-    const bool tail = p.rest.p != nullptr;
-    const double t_rest = tail ? double(p.rest[row]) : -INFINITY;
-    double t_top = t_rest, x_top = s > 0 ? double(m) : -INFINITY;
+  // Distillation, every thread: the exponentials t and q of both models'
+  // logits at the kept tokens, against the maxima over them, and the sums
+  //   sum t, sum q, sum t (log t - log q).
+  __device__ __forceinline__ void kept_sums(Shared& sh, const Kept& kept, const Scale& scale, float& value_top, float& x_top) const {
+    value_top = x_top = -INFINITY;
     for (int k = lane_id(); k < p.k; k += 32)
       if (kept.id[k] >= 0) {
-        t_top = fmax(t_top, kept.value[k] / temperature);
-        x_top = fmax(x_top, double(kept.x[k]));
+        value_top = fmaxf(value_top, kept.value[k]);
+        x_top = fmaxf(x_top, kept.x[k]);
       }
-    t_top = warp_max(t_top);
-    x_top = warp_max(x_top);
-    double t_sum = 0, x_sum = 0;
-    for (int k = lane_id(); k < p.k; k += 32)
+    value_top = warp_top(value_top);
+    x_top = warp_top(x_top);
+    float t_sum = 0.f, q_sum = 0.f, cross = 0.f;
+    for (int k = tid; k < p.k; k += THREADS) {
+      float t = 0.f, q = 0.f;
       if (kept.id[k] >= 0) {
-        t_sum += exp(kept.value[k] / temperature - t_top);
-        x_sum += exp((kept.x[k] - x_top) / temperature);
+        const Pair lt = scaled_gap(kept.value[k], value_top, scale), lq = scaled_gap(kept.x[k], x_top, scale);
+        t = kept.value[k] == -INFINITY ? 0.f : expf(lt.hi) * (1.f + lt.lo);
+        q = kept.x[k] == -INFINITY ? 0.f : expf(lq.hi) * (1.f + lq.lo);
+        if (t > 0.f) cross += kept.x[k] == -INFINITY ? INFINITY : t * ((lt.hi - lq.hi) + (lt.lo - lq.lo));
+        t_sum += t;
+        q_sum += q;
       }
-    const double rest_factor = s > 0 ? exp((m - x_top) / temperature) : 0.;
-    t_sum = warp_sum(t_sum) + (tail ? exp(t_rest - t_top) : 0.);
-    x_sum = warp_sum(x_sum) + s * rest_factor;
-    const double log_t = t_top + log(t_sum), log_x = log(x_sum);
-    const double w = p.weights.p ? p.weights[row] : 1.f;
-    bad |= !(s < double(INFINITY)) || !isfinite(log_t) || (tail && !(t_rest < INFINITY));
-    double loss = 0;
-    bool lost = false;  // the student has no mass where the teacher has some
-    for (int k = lane_id(); k < p.k; k += 32)
-      if (kept.id[k] >= 0) {
-        const double lt = kept.value[k] / temperature - log_t, lq = (kept.x[k] - x_top) / temperature - log_x;
-        const double t = exp(lt);
-        if (t > 0) {
-          loss += t * (lt - lq);
-          lost |= kept.x[k] == -INFINITY;
-        }
-      }
-    loss = warp_sum(loss);
-    lost = __any_sync(0xffffffffu, lost);
-    double pull = 1;  // of the tokens not kept: 1 - t_rest / q_rest
-    const double lt_rest = t_rest - log_t;
-    if (tail && exp(lt_rest) > 0) {
-      const double off = lt_rest - (log(s) + (m - x_top) / temperature - log_x);
-      loss += exp(lt_rest) * off;
-      pull = -expm1(off);
-      lost |= !(s > 0);
+      kept.t[k] = t;
+      kept.q[k] = q;
     }
+    t_sum = warp_sum(t_sum);
+    q_sum = warp_sum(q_sum);
+    cross = warp_sum(cross);
+    if (lane_id() == 0) {
+      sh.sums[warp_id()][0] = t_sum;
+      sh.sums[warp_id()][1] = q_sum;
+      sh.sums[warp_id()][2] = cross;
+    }
+  }
+
+  // A model's total over its entries (their sum `entries`, relative to their
+  // maximum) and the others (`others`, relative to theirs, which lies `over`
+  // above the entries'): its logarithm relative to both, and the shares that
+  // an entry's and another token's relative exponentials are multiplied with.
+  struct Total {
+    Pair to_entries, to_others;
+    float entry_share, other_share, total;
+  };
+  static __device__ __forceinline__ Total total_of(float entries, float others, Pair over) {
+    if (!(others > 0.f)) over = {-INFINITY, 0.f};
+    if (!(entries > 0.f)) over = {INFINITY, 0.f};
+    const bool above = over.hi > 0.f;  // the others are the reference
+    const float f = isfinite(over.hi) ? expf(above ? -over.hi : over.hi) * (1.f + (above ? -over.lo : over.lo)) : 0.f;
+    const float f_entries = entries > 0.f ? (above ? f : 1.f) : 0.f, f_others = others > 0.f ? (above ? 1.f : f) : 0.f;
+    Total r;
+    r.total = entries * f_entries + others * f_others;
+    const float inv = __frcp_rn(r.total);
+    const Pair log_total = log_pair(r.total);
+    r.to_entries = above ? pair_sum(log_total, over) : log_total;
+    r.to_others = above ? log_total : pair_sum(log_total, negated(over));
+    r.entry_share = f_entries * inv;
+    r.other_share = f_others * inv;
+    return r;
+  }
+
+  // One thread, from the merged records of the tokens not kept (m, s). With T
+  // and Q the logs of both totals, relative to the maxima over the entries,
+  //   loss = sum_k t (lt - lq) / e^T + (Q - T) sum_k t / e^T + the bucket's term.
+  __device__ __forceinline__ void distill_scalars(Shared& sh, float m, float s, uint32_t flags, const Scale& scale,
+                                                  const Inputs& in, float value_top, float x_top) {
+    const bool tail = p.rest.p != nullptr;
+    float t_sum = 0.f, q_sum = 0.f, cross = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      t_sum += sh.sums[w][0];
+      q_sum += sh.sums[w][1];
+      cross += sh.sums[w][2];
+    }
+    const Total t = total_of(t_sum, tail && in.first > -INFINITY ? 1.f : 0.f,
+                             pair_sum({in.first, 0.f}, negated(scaled_gap(value_top, 0.f, scale))));
+    const Total q = total_of(q_sum, s, scaled_gap(m, x_top, scale));
+    float loss = 0.f, pull = 1.f;   // pull, of the tokens not kept: 1 - t_rest / q_rest
+    bool lost = cross == INFINITY;  // the student has no mass where the teacher has some
+    if (t_sum > 0.f) loss = (cross + t_sum * value_of(pair_sum(q.to_entries, negated(t.to_entries)))) * t.entry_share;
+    if (t.other_share > 0.f) {
+      // log t_rest - log q_rest
+      const float off = value_of(pair_sum(pair_sum(q.to_others, negated(t.to_others)), negated(log_pair(s))));
+      loss += t.other_share * off;
+      pull = -expm1f(off);
+      lost |= !(s > 0.f);
+    }
+    const bool bad = (flags & BAD) || !(s < INFINITY) || !(t.total > 0.f && t.total < INFINITY) || (tail && !(in.first < INFINITY));
     int status = ES_OK;
     if (bad) status = ES_INVALID_INPUT;
-    else if (x_top == -INFINITY) status = ES_NO_VALID_TOKEN;
+    else if (!(q_sum > 0.f) && !(s > 0.f)) status = ES_NO_VALID_TOKEN;
     else if (lost) status = ES_DRAFT_ZERO_PROB;
-    else if (!isfinite(float(loss))) status = ES_INVALID_INPUT;
-    if (lane_id() != 0) return;
+    else if (!isfinite(loss)) status = ES_INVALID_INPUT;
     const bool ok = status == ES_OK;
-    if (rank == 0) outputs(status, ok ? float(w * loss) : 0.f, 0.f, 0.f, 0.f);
+    if (rank == 0) outputs(status, ok ? in.w * loss : 0.f, 0.f, 0.f, 0.f);
     if (GRAD) {
       RowScalars& r = sh.row;
       r.zero = !ok;
-      r.m = m;
-      r.a = s > 0 ? float(w / temperature * pull * rest_factor / x_sum) : 0.f;
-      r.b = 0.f;
-      r.top = x_top;
-      r.log_total = log_x;
-      r.teacher = log_t;
-      r.w = w / temperature;
+      r.w = in.w * scale.hi;
+      r.inv_q = q.entry_share;
+      r.inv_t = t.entry_share;
+      set_scalars(r, m, scale.log2, s > 0.f ? r.w * pull * q.other_share : 0.f, 0.f, flags & CAREFUL || scale.log2 < SMALL_SCALE);
     }
+  }
+
+  // The gradient of chunk c from its logits. FORM 0: 2^d a; 1: 2^d (a + b d);
+  // 2: the careful form of the latter.
+  template <int FORM, bool HAS_MASK>
+  __device__ __forceinline__ uint4 grad_chunk(const uint4& q, int c, const int32_t* mask, const RowScalars& r, float scale,
+                                              int token) const {
+    float2 v[N / 2];
+    unpack<DT>(q, v);
+    if (HAS_MASK) {
+      mask_chunk<DT>(mask_bits<DT>(mask, p.in.mask.s1, c * N), -INFINITY, v);
+      if (FORM == 1) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) v[i] = make_float2(fmaxf(v[i].x, MASKED), fmaxf(v[i].y, MASKED));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      float2 d;
+      if (FORM == 2) d = make_float2(exponent(v[i].x, r.m, scale), exponent(v[i].y, r.m, scale));
+      else d = fma2(v[i], both(scale), both(-r.r));
+      const float2 e = make_float2(ex2(d.x), ex2(d.y));
+      v[i] = mul2(e, FORM == 0 ? both(r.a) : fma2(both(r.b), d, both(r.a)));
+    }
+    if (OP != DISTILL && token / N == c) {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        if (token % N == 2 * i) v[i].x = r.token_grad;
+        if (token % N == 2 * i + 1) v[i].y = r.token_grad;
+      }
+    }
+    return pack<DT>(v);
   }
 
   // The gradient of this rank's slice from its shared copy.
-  template <bool TWO> __device__ __forceinline__ void write_grad(const Slice<DT>& slice, const RowScalars& r, float scale,
-                                                                 int token) const {
-    const float2 nm = both(-r.m), sc = both(scale), a = both(r.a), b = both(r.b);
-    const bool vector = grad_vector();
-    for (int c = tid; c < slice.chunks; c += THREADS) {
-      float2 v[N / 2];
-      unpack<DT>(slice.chunk(c), v);
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        float2 d = mul2(add2(v[i], nm), sc);
-        if (TWO) d = make_float2(fmaxf(d.x, FAR), fmaxf(d.y, FAR));
-        const float2 e = make_float2(ex2(d.x), ex2(d.y));
-        v[i] = mul2(e, TWO ? fma2(b, d, a) : a);
+  template <int FORM, bool HAS_MASK>
+  __device__ __forceinline__ void write_grad(const Slice<DT>& slice, const RowScalars& scalars, float scale, int token) const {
+    const RowScalars r = scalars;
+    const int32_t* mask = HAS_MASK ? p.in.mask.p + row * p.in.mask.s0 + (begin >> 5) * p.in.mask.s1 : nullptr;
+    if (grad_vector()) {
+      uint4* out = reinterpret_cast<uint4*>(grad_at(begin));
+      const int whole = n / N;
+      int c = tid;
+      for (; c + THREADS < whole; c += 2 * THREADS) {
+        const uint4 q0 = slice.chunk(c), q1 = slice.chunk(c + THREADS);
+        out[c] = grad_chunk<FORM, HAS_MASK>(q0, c, mask, r, scale, token);
+        out[c + THREADS] = grad_chunk<FORM, HAS_MASK>(q1, c + THREADS, mask, r, scale, token);
       }
-      if (OP != DISTILL && token / N == c) {
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-          if (token % N == 2 * i) v[i].x = r.token_grad;
-          if (token % N == 2 * i + 1) v[i].y = r.token_grad;
+      for (; c < slice.chunks; c += THREADS) {
+        const uint4 q = grad_chunk<FORM, HAS_MASK>(slice.chunk(c), c, mask, r, scale, token);
+        if (c < whole) {
+          out[c] = q;
+        } else {
+          const T* v = reinterpret_cast<const T*>(&q);
+          for (int i = 0; i < n - c * N; ++i) *grad_at(begin + c * N + i) = v[i];
         }
       }
-      const uint4 q = pack<DT>(v);
-      if (vector && (c + 1) * N <= n) {
-        *reinterpret_cast<uint4*>(grad_at(begin + c * N)) = q;
-      } else if (vector) {
-        const T* t = reinterpret_cast<const T*>(&q);
-        for (int i = 0; i < n - c * N; ++i) *grad_at(begin + c * N + i) = t[i];
-      } else {
-        slice.set_chunk(c, q);
-      }
+      return;
     }
-    if (vector) return;
-    // Gradient rows that do not start on 16 bytes, or have a stride: from
-    // shared memory, in whole 16-byte pieces where both sides are aligned alike.
+    // Gradient rows that do not start on 16 bytes, or have a stride: by way of
+    // shared memory, in 16-byte pieces from the first aligned address on.
+    for (int c = tid; c < slice.chunks; c += THREADS)
+      slice.chunk(c) = grad_chunk<FORM, HAS_MASK>(slice.chunk(c), c, mask, r, scale, token);
     __syncthreads();
-    const bool alike = p.g_s1 == 1 && (reinterpret_cast<uintptr_t>(grad_at(begin)) & 15) == slice.shift;
-    if (alike) {
-      const int head = min(int((16 - slice.shift) & 15) / int(sizeof(T)), n), whole = (n - head) / N;
-      const uint4* s = reinterpret_cast<const uint4*>(&slice[head]);
-      uint4* g = reinterpret_cast<uint4*>(grad_at(begin + head));
-      for (int c = tid; c < whole; c += THREADS) g[c] = s[c];
+    int done = 0;
+    if (p.g_s1 == 1) {
+      const int head = min(int(uint32_t(16 - (reinterpret_cast<uintptr_t>(grad_at(begin)) & 15)) / sizeof(T)), n);
+      const int pieces = (n - head) / N;
+      uint4* out = reinterpret_cast<uint4*>(grad_at(begin + head));
+      for (int i = tid; i < pieces; i += THREADS) out[i] = shifted_chunk<sizeof(T)>(&slice.chunk(i), head * sizeof(T));
       if (tid < head) *grad_at(begin + tid) = slice[tid];
-      const int i = head + whole * N + tid;
-      if (i < n) *grad_at(begin + i) = slice[i];
-    } else {
-      for (int i = tid; i < n; i += THREADS) *grad_at(begin + i) = slice[i];
+      done = head + pieces * N;
     }
+    for (int i = done + tid; i < n; i += THREADS) *grad_at(begin + i) = slice[i];
+  }
+  template <bool HAS_MASK>
+  __device__ __forceinline__ void write_form(const Slice<DT>& slice, const RowScalars& r, float scale, int token) const {
+    if (r.careful) write_grad<2, HAS_MASK>(slice, r, scale, token);
+    else if (ENTROPY && r.b != 0.f) write_grad<1, HAS_MASK>(slice, r, scale, token);
+    else write_grad<0, HAS_MASK>(slice, r, scale, token);
   }
 
   __device__ __forceinline__ void run(uint8_t* smem) {
     Shared& sh = *reinterpret_cast<Shared*>(smem);
-    Kept& kept = *reinterpret_cast<Kept*>(smem + sizeof(Shared));
-    uint32_t* seen = reinterpret_cast<uint32_t*>(smem + sizeof(Shared) + sizeof(Kept));
-    uint8_t* buffer = smem + ((sizeof(Shared) + (OP == DISTILL ? sizeof(Kept) + size_t(p.in.slice) / 8 : 0) + 15) & ~size_t(15));
+    uint8_t* buffer = smem + SHARED_BYTES;
+    const Kept kept(buffer + slice_bytes<DT>(p.in.slice), p.k);
 
     // The row's token, or the teacher's entries; rows without are not read.
-    int64_t token = -1;
-    float z = 0.f, x = 0.f;
-    bool token_allowed = true, bad = false;
-    int id = -1;
+    Inputs in{};
+    bool bad = false;
     if (OP != DISTILL) {
-      token = p.tokens[row];
+      in.token = p.tokens[row];
     } else {
-      float value = 0.f;
-      int64_t wide = -1;
-      if (tid < p.k) {
-        wide = p.ids.p[row * p.ids.s0 + tid * p.ids.s1];
-        value = p.values.p[row * p.values.s0 + tid * p.values.s1];
+      bool any = false;
+      for (int k = tid; k < p.k; k += THREADS) {
+        const int64_t id = p.ids.p[row * p.ids.s0 + k * p.ids.s1];
+        const float value = p.values.p[row * p.values.s0 + k * p.values.s1];
+        any |= id >= 0;
+        bad |= id >= p.in.vocab || (id >= 0 && !(value < INFINITY));
+        kept.id[k] = id >= 0 && id < p.in.vocab ? int(id) : -1;
+        kept.value[k] = value;
       }
-      if (__syncthreads_or(wide >= 0)) token = 0;
-      if (wide >= 0) {
-        bad |= wide >= p.in.vocab || !(value < INFINITY);
-        id = wide < p.in.vocab ? int(wide) : -1;
-      }
-      if (tid < p.k) {
-        kept.id[tid] = id;
-        kept.value[tid] = value;
-      }
-      for (int i = tid; i < p.in.slice / 32; i += THREADS) seen[i] = 0;
+      for (int i = tid; i < p.in.slice / 32; i += THREADS) kept.seen[i] = 0;
+      in.token = __syncthreads_or(any) ? 0 : -1;
     }
-    if (token < 0) {
+    if (in.token < 0) {
       if (GRAD) zero_grad();
       if (rank == 0 && tid == 0) outputs(ES_OK, 0.f, 0.f, 0.f, 0.f);
       return;
     }
     cluster_arrive();  // this rank's shared memory may be written from now on
-    double temperature = p.in.temperature.p ? p.in.temperature[row] : p.in.temperature_all;
-    float scale = float(LOG2E / temperature);
-    if (!(temperature > 0 && scale >= 1.17549435e-38f && scale <= 3.402823466e38f)) {
-      bad = true;
-      temperature = 1;
-      scale = float(LOG2E);
-    }
     Slice<DT> slice;
-    slice.load(p.in, row, begin, n, buffer, sh.bar);
-    if (OP != DISTILL) {
-      if (warp_id() == 0 && token < p.in.vocab) {
-        z = E::get(logit(token));
-        token_allowed = allowed(token);
+    slice.load(p.in, row, begin, n, buffer, &sh.bar);
+    const Scale scale = row_scale(p.in, row);
+    bad |= scale.bad;
+    if (tid == 0) {
+      if (OP != DISTILL && in.token < p.in.vocab) {
+        in.z = E::get(logit(in.token));
+        in.allowed = allowed(in.token);
       }
-    } else {
-      if (id >= 0) {
-        x = E::get(logit(id));
-        bad |= !(x < INFINITY);
-        if (!allowed(id)) x = -INFINITY;
+      if (OP == LOGPROB && GRAD) {
+        if (p.grad_logprobs.p) in.first = p.grad_logprobs[row];
+        if (p.grad_entropy.p) in.second = p.grad_entropy[row];
       }
-      if (tid < p.k) kept.x[tid] = x;
-      slice.wait_all();
+      if (OP == POLICY) {
+        in.first = p.old_logprobs[row];
+        in.second = p.advantages[row];
+        if (p.ref_logprobs.p) in.ref = p.ref_logprobs[row];
+      }
+      if (OP == DISTILL && p.rest.p) in.first = p.rest[row];
+      if (OP != LOGPROB) in.w = p.weights.p ? p.weights[row] : 1.f;
+    }
+    float value_top = 0.f, x_top = 0.f;
+    if (OP == DISTILL) {
+      for (int k = tid; k < p.k; k += THREADS) {
+        float x = -INFINITY;
+        if (kept.id[k] >= 0) {
+          x = E::get(logit(kept.id[k]));
+          bad |= !(x < INFINITY);
+          if (!allowed(kept.id[k])) x = -INFINITY;
+        }
+        kept.x[k] = x;
+      }
+      __syncthreads();
+      kept_sums(sh, kept, scale, value_top, x_top);
+    }
+    bad |= !slice.wait();
+    if (OP == DISTILL) {
       // The kept tokens leave the slice, so that what is summed is the others.
-      const int local = id - begin;
-      if (id >= 0 && local >= 0 && local < n) {
-        bad |= (atomicOr(&seen[local >> 5], 1u << (local & 31)) >> (local & 31)) & 1;
-        slice[local] = E::put(-INFINITY);
+      for (int k = tid; k < p.k; k += THREADS) {
+        const int local = kept.id[k] - begin;
+        if (kept.id[k] >= 0 && local >= 0 && local < n) {
+          bad |= (atomicOr(&kept.seen[local >> 5], 1u << (local & 31)) >> (local & 31)) & 1;
+          slice[local] = E::put(-INFINITY);
+        }
       }
       __syncthreads();
     }
 
-    Acc acc = acc_none();
-    const int32_t* mask = p.in.mask.p ? p.in.mask.p + row * p.in.mask.s0 : nullptr;
-    for (int c = tid; c < slice.chunks; c += THREADS) {
-      slice.wait(uint32_t(c - tid + THREADS + 1) * 16);
-      float2 v[N / 2];
-      unpack<DT>(slice.chunk(c), v);
-      if (mask) {
-        bad |= mask_chunk<DT>(mask, p.in.mask.s1, begin + c * N, v);
-        if (GRAD) slice.set_chunk(c, pack<DT>(v));
-      }
-      acc_chunk<N, ENTROPY>(acc, v, scale);
-    }
-    slice.wait_all();
-    Record rec = {acc.m, __fadd_rn(acc.s.x, acc.s.y), __fadd_rn(acc.u.x, acc.u.y), uint32_t(bad || slice.late)};
-#pragma unroll
-    for (int o = 16; o; o >>= 1) rec = merge(rec, shfl_record(rec, o), scale);
+    const int32_t* mask = p.in.mask.p ? p.in.mask.p + row * p.in.mask.s0 + (begin >> 5) * p.in.mask.s1 : nullptr;
+    Record rec = mask ? sum_slice<DT, ENTROPY, true>(slice, mask, p.in.mask.s1, scale.log2)
+                      : sum_slice<DT, ENTROPY, false>(slice, nullptr, 0, scale.log2);
+    if (bad) rec.flags |= BAD;
+    rec = warp_record<ENTROPY>(rec, scale.log2);
     if (lane_id() == 0) sh.warps[warp_id()] = rec;
     cluster_wait();  // every rank has started
     __syncthreads();
-    if (warp_id() == 0) {
-      rec = sh.warps[lane_id() & (WARPS - 1)];
-#pragma unroll
-      for (int o = WARPS / 2; o; o >>= 1) rec = merge(rec, shfl_record(rec, o), scale);
-      if (lane_id() < ranks) cg::this_cluster().map_shared_rank(sh.inbox, lane_id())[rank] = rec;
-    }
+    rec = warp_record<ENTROPY>(lane_record(sh.warps, WARPS), scale.log2);
+    if (tid < ranks) cg::this_cluster().map_shared_rank(sh.inbox, tid)[rank] = rec;
     cluster_arrive();
     cluster_wait();
     if (!GRAD && rank != 0) return;
-    if (warp_id() == 0) {
-      const bool mine = lane_id() < ranks;
-      rec = mine ? sh.inbox[lane_id()] : Record{LOWEST, 0.f, 0.f, 0u};
-      const float m = warp_all(rec.m, [](float a, float b) { return fmaxf(a, b); });
-      const float d = exponent(rec.m, m, scale);
-      const double f = exp2f(d), s = warp_sum(f * rec.s), u = warp_sum(f * (double(rec.u) + double(d) * rec.s));
-      bad = __any_sync(0xffffffffu, rec.bad != 0);
-      if (OP == DISTILL) distill_scalars(sh, kept, m, s, bad, temperature);
-      else token_scalars(sh, m, s, u, bad, temperature, token, z, token_allowed);
+    rec = warp_record<ENTROPY>(lane_record(sh.inbox, ranks), scale.log2);
+    if (tid == 0) {
+      if (OP == DISTILL) distill_scalars(sh, rec.m, rec.s, rec.flags, scale, in, value_top, x_top);
+      else token_scalars(sh, rec.m, rec.s, rec.u, rec.flags, scale, in);
     }
     if (!GRAD) return;
     __syncthreads();
@@ -720,24 +1025,23 @@ template <int DT, int OP, bool GRAD> struct LossRow {
       zero_grad();
       return;
     }
-    const int64_t local = token - begin;
+    const int64_t local = in.token - begin;
     const int at = OP != DISTILL && local >= 0 && local < n ? int(local) : -N;
-    if (r.b != 0.f) write_grad<true>(slice, r, scale, at);
-    else write_grad<false>(slice, r, scale, at);
+    if (mask) write_form<true>(slice, r, scale.log2, at);
+    else write_form<false>(slice, r, scale.log2, at);
     if (OP == DISTILL) {
       __syncthreads();  // after the slice's zeros at these places
-      const int at_id = id - begin;
-      if (id >= 0 && at_id >= 0 && at_id < n) {
-        const double q = exp((x - r.top) / temperature - r.log_total), t = exp(kept.value[tid] / temperature - r.teacher);
-        *grad_at(id) = E::put(float(r.w * (q - t)));
+      for (int k = tid; k < p.k; k += THREADS) {
+        const int local_id = kept.id[k] - begin;
+        if (kept.id[k] >= 0 && local_id >= 0 && local_id < n)
+          *grad_at(kept.id[k]) = E::put(r.w * (kept.q[k] * r.inv_q - kept.t[k] * r.inv_t));
       }
     }
   }
 };
 
-// Five blocks to an SM, so that some load while others exchange or write.
 template <int DT, int OP, bool GRAD>
-__global__ void __launch_bounds__(THREADS, 4) loss_rows(const __grid_constant__ LossParams p) {
+__global__ void __launch_bounds__(THREADS, ES_SCORE_BLOCKS) loss_rows(const __grid_constant__ LossParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   const int ranks = p.in.ranks, rank = int(blockIdx.x % unsigned(ranks));
   const int begin = rank * p.in.slice, n = min(p.in.slice, p.in.vocab - begin);
@@ -777,7 +1081,7 @@ cudaError_t launch_clusters(void (*kernel)(P), const P& p, int64_t rows, int ran
 
 template <int DT, int OP, bool GRAD> cudaError_t launch_one(const LossParams& p, int64_t rows, cudaStream_t stream) {
   static std::atomic<uint64_t> configured{0};
-  return launch_clusters(loss_rows<DT, OP, GRAD>, p, rows, p.in.ranks, loss_smem<DT>(p.in.slice, OP), stream, configured);
+  return launch_clusters(loss_rows<DT, OP, GRAD>, p, rows, p.in.ranks, loss_smem<DT>(p.in.slice, p.k), stream, configured);
 }
 template <int DT> cudaError_t launch_loss(const LossParams& p, int op, int64_t rows, cudaStream_t stream) {
   const bool grad = p.grad != nullptr;

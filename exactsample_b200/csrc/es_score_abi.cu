@@ -123,21 +123,21 @@ constexpr size_t MAX_SMEM = 227 * 1024;
 // Ranks of a row's cluster: slices of about SLICE_BYTES, the fewest ranks
 // that allow them, at most 16. The rule sees only the vocabulary and the type, so that a
 // row's results do not depend on the batch.
-int split(Rows& r, const es_rows& in, size_t slice_bytes, size_t (*smem)(int, int32_t, int), int op, size_t* bytes) {
+int split(Rows& r, const es_rows& in, size_t slice_bytes, size_t (*smem)(int, int32_t, int), int k, size_t* bytes) {
   const int64_t vocab = in.logits.size[1];
   const int64_t steps = (vocab + SLICE_STEP - 1) / SLICE_STEP;
   const int64_t row_bytes = vocab * int64_t(element_size(in.logits.dtype));
   const int64_t want = std::clamp<int64_t>((row_bytes + int64_t(slice_bytes) - 1) / int64_t(slice_bytes), 1, MAX_RANKS);
   const int64_t slice = (steps + want - 1) / want * SLICE_STEP;
   if (slice > int64_t(MAX_SMEM)) return fail(ES_ERR_UNSUPPORTED, "vocabulary too large for one 16-block cluster's shared memory");
-  *bytes = smem(int(slice), in.logits.dtype, op);
+  *bytes = smem(int(slice), in.logits.dtype, k);
   if (*bytes > MAX_SMEM) return fail(ES_ERR_UNSUPPORTED, "vocabulary too large for one 16-block cluster's shared memory");
   r.logits = in.logits.data;
   r.l_s0 = in.logits.stride[0];
   r.l_s1 = in.logits.stride[1];
   r.mask = grid2<const int32_t>(in.mask);
   r.temperature = col<const double>(in.temperature);
-  r.temperature_all = in.temperature_all;
+  r.inv_all = 1. / in.temperature_all;
   r.vocab = int32_t(vocab);
   r.slice = int32_t(slice);
   r.ranks = int32_t((vocab + slice - 1) / slice);
@@ -145,8 +145,8 @@ int split(Rows& r, const es_rows& in, size_t slice_bytes, size_t (*smem)(int, in
   return ES_SUCCESS;
 }
 
-size_t loss_bytes(int slice, int32_t dtype, int op) {
-  return dtype == ES_F32 ? loss_smem<ES_F32>(slice, op) : loss_smem<ES_F16>(slice, op);
+size_t loss_bytes(int slice, int32_t dtype, int k) {
+  return dtype == ES_F32 ? loss_smem<ES_F32>(slice, k) : loss_smem<ES_F16>(slice, k);
 }
 constexpr size_t LOSS_SLICE_BYTES = 38 * 1024;
 
@@ -159,7 +159,7 @@ int run_loss(Call& call, LossParams& p, const es_tensor& grad, int op, cudaStrea
   if (const int e = call.gradient(grad); e != ES_SUCCESS) return e;
   if (const int e = call.finish(); e != ES_SUCCESS) return e;
   size_t smem = 0;
-  if (const int e = split(p.in, call.in, LOSS_SLICE_BYTES, loss_bytes, op, &smem); e != ES_SUCCESS) return e;
+  if (const int e = split(p.in, call.in, LOSS_SLICE_BYTES, loss_bytes, p.k, &smem); e != ES_SUCCESS) return e;
   if (call.rows == 0) return ES_SUCCESS;
   if (const int e = device_check(); e != ES_SUCCESS) return e;
   p.grad = present(grad) ? grad.data : nullptr;

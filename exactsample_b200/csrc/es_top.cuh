@@ -3,11 +3,11 @@
 //
 // A row is split over a cluster and kept in shared memory as in es_score.cuh.
 // Selection needs no sort of the row:
-//   1. the load pass takes the maximum of every tile of 32 tokens;
-//   2. each rank finds the ceil(k / ranks)-th largest of its tile maxima (to
-//      18 bits of its key). At least that many of its tokens reach it, so the
-//      smallest of the ranks' values is a bound that at least k tokens of the
-//      row reach, and few more (a tile rarely holds two of the largest);
+//   1. each thread takes the maximum of its tokens as they arrive;
+//   2. each rank finds the ceil(k / ranks)-th largest of its threads' maxima
+//      (to 16 bits of its key). At least that many of its tokens reach it, so
+//      the smallest of the ranks' values is a bound that at least k tokens of
+//      the row reach, and few more (a thread rarely holds two of the largest);
 //   3. tokens at or above the bound are listed and leave the slice; the pass
 //      over what is left sums the rest without them, so that a rest far below
 //      the largest logits loses no digits to a subtraction;
@@ -35,15 +35,14 @@ struct TopParams {
 constexpr uint32_t KEY_NONE = 0x007fffffu;  // the key of -inf: not a token of the row
 constexpr int LISTED = 512;                 // entries a rank lists
 constexpr int COLLECTED = 1024;             // entries rank 0 takes
-constexpr int TILE = 32;
-constexpr uint32_t BAD = 1, FULL = 2;       // Record::bad: an invalid row, a list that did not fit
+
+static_assert(THREADS >= 8 * MAX_RANKS, "exact_threshold's exchange has a thread per digit and rank");
 
 struct TopShared {
-  uint64_t bar[PIECES];
+  uint64_t bar;
   Record inbox[MAX_RANKS];
   Record warps[WARPS];
   uint32_t bound[MAX_RANKS];
-  uint32_t tiles_above[2][8];
   uint32_t digits[2][MAX_RANKS][8];
   uint32_t warp_digits[WARPS][8];
   uint32_t listed, total, place;
@@ -52,7 +51,7 @@ struct TopShared {
 };
 
 template <int DT> __host__ __device__ constexpr size_t top_smem(int slice) {
-  return sizeof(TopShared) + size_t(slice) / TILE * 4 + 16 + size_t(slice) * sizeof(typename Elem<DT>::T) + 32;
+  return (sizeof(TopShared) + 15) / 16 * 16 + slice_bytes<DT>(slice);
 }
 
 __device__ __forceinline__ uint64_t entry_of(uint32_t key, int id) { return (uint64_t(key) << 32) | (0xffffffffu - uint32_t(id)); }
@@ -66,25 +65,13 @@ template <int DT> struct TopRow {
   int64_t row;
   int rank, ranks, begin, n, tid;
 
-  // Warps 1..7 count the tiles at or above seven thresholds at once, three
-  // bits of the key a step, 18 bits in all. 0: fewer than `need` tiles.
-  __device__ __forceinline__ uint32_t tile_bound(TopShared& sh, const uint32_t* tiles, int count, int need) const {
+  // A bound with 16 zero bits below that at least `need` of the threads' keys
+  // reach; 0 if fewer threads than that have any token.
+  __device__ __forceinline__ uint32_t thread_bound(uint32_t key, int need) const {
     uint32_t found = 0;
-    int turn = 0;
-    for (int shift = 29; shift >= 14; shift -= 3, turn ^= 1) {
-      if (warp_id() > 0) {
-        const uint32_t least = found | (uint32_t(warp_id()) << shift);
-        int above = 0;
-        for (int t = lane_id(); t < count; t += 32) above += tiles[t] >= least;
-        above = __reduce_add_sync(0xffffffffu, above);
-        if (lane_id() == 0) sh.tiles_above[turn][warp_id()] = above;
-      }
-      __syncthreads();
-      int digit = 0;
-#pragma unroll
-      for (int w = 1; w < 8; ++w) digit += sh.tiles_above[turn][w] >= uint32_t(need);
-      found |= uint32_t(digit) << shift;
-    }
+#pragma unroll 1
+    for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
+      if (__syncthreads_count(key >= (found | bit)) >= need) found |= bit;
     return found;
   }
 
@@ -134,24 +121,20 @@ template <int DT> struct TopRow {
     return found;
   }
 
-  // Lists the tokens at or above `least` and takes them out of the slice.
-  __device__ __forceinline__ void list_entries(TopShared& sh, const uint32_t* tiles, int count, const Slice<DT>& slice,
-                                               uint64_t least) const {
-    const uint32_t least_key = uint32_t(least >> 32);
-    for (int base = warp_id() * 32; base < count; base += THREADS) {
-      const int t = base + lane_id();
-      uint32_t hot = __ballot_sync(0xffffffffu, t < count && tiles[t] >= least_key);
-      while (hot) {
-        const int i = (base + __ffs(hot) - 1) * TILE + lane_id();
-        hot &= hot - 1;
-        uint64_t entry = 0;
-        if (i < n) entry = entry_of(order_key(E::get(slice[i])), begin + i);
-        const bool take = i < n && entry >= least;
-        const uint32_t takers = __ballot_sync(0xffffffffu, take);
-        uint32_t at = 0;
-        if (lane_id() == 0) at = atomicAdd(&sh.listed, uint32_t(__popc(takers)));
-        at = __shfl_sync(0xffffffffu, at, 0) + __popc(takers & ((1u << lane_id()) - 1));
-        if (take && at < LISTED) {
+  // Lists the tokens at or above `least` and takes them out of the slice. A
+  // warp goes through the tokens of each of its threads whose maximum reaches it.
+  __device__ __forceinline__ void list_entries(TopShared& sh, uint32_t key, const Slice<DT>& slice, uint64_t least) const {
+    uint32_t hot = __ballot_sync(0xffffffffu, key >= uint32_t(least >> 32));
+    while (hot) {
+      const int owner = warp_id() * 32 + __ffs(hot) - 1;
+      hot &= hot - 1;
+      for (int first = owner; first < slice.chunks; first += THREADS * (32 / N)) {
+        const int i = (first + lane_id() / N * THREADS) * N + lane_id() % N;
+        if (i >= n) continue;
+        const uint64_t entry = entry_of(order_key(E::get(slice[i])), begin + i);
+        if (entry < least) continue;
+        const uint32_t at = atomicAdd(&sh.listed, 1u);
+        if (at < LISTED) {
           sh.list[at] = entry;
           slice[i] = E::put(-INFINITY);
         }
@@ -165,62 +148,47 @@ template <int DT> struct TopRow {
   }
 
   __device__ __forceinline__ Record block_record(TopShared& sh, Record rec, float scale) const {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) rec = merge(rec, shfl_record(rec, o), scale);
+    rec = warp_record<false>(rec, scale);
     __syncthreads();
     if (lane_id() == 0) sh.warps[warp_id()] = rec;
     __syncthreads();
-    rec = sh.warps[lane_id() & (WARPS - 1)];
-#pragma unroll
-    for (int o = WARPS / 2; o; o >>= 1) rec = merge(rec, shfl_record(rec, o), scale);
-    return rec;
+    return warp_record<false>(lane_record(sh.warps, WARPS), scale);
   }
 
   __device__ __forceinline__ void run(uint8_t* smem) {
     TopShared& sh = *reinterpret_cast<TopShared*>(smem);
-    uint32_t* tiles = reinterpret_cast<uint32_t*>(smem + sizeof(TopShared));
-    uint8_t* buffer = smem + ((sizeof(TopShared) + size_t(p.in.slice) / TILE * 4 + 15) & ~size_t(15));
-    const int count = (n + TILE - 1) / TILE;
+    uint8_t* buffer = smem + (sizeof(TopShared) + 15) / 16 * 16;
     bool bad = false;
-    double temperature = p.in.temperature.p ? p.in.temperature[row] : p.in.temperature_all;
-    float scale = float(LOG2E / temperature);
-    if (!(temperature > 0 && scale >= 1.17549435e-38f && scale <= 3.402823466e38f)) {
-      bad = true;
-      temperature = 1;
-      scale = float(LOG2E);
-    }
     if (tid == 0) sh.listed = sh.total = 0;
     cluster_arrive();  // this rank's shared memory may be written from now on
     Slice<DT> slice;
-    slice.load(p.in, row, begin, n, buffer, sh.bar);
+    slice.load(p.in, row, begin, n, buffer, &sh.bar);
+    const Scale temperature = row_scale(p.in, row);
+    const float scale = temperature.log2;
+    bad |= temperature.bad;
+    bad |= !slice.wait();
 
-    // Tile maxima: 32 / N neighbouring lanes hold a tile's chunks.
-    const int32_t* mask = p.in.mask.p ? p.in.mask.p + row * p.in.mask.s0 : nullptr;
-    for (int first = 0; first < slice.chunks; first += THREADS) {
-      slice.wait(uint32_t(first + THREADS + 1) * 16);
-      const int c = first + tid;
-      float top = -INFINITY;
-      if (c < slice.chunks) {
+    // This thread's maximum; masked tokens leave the slice.
+    const int32_t* mask = p.in.mask.p ? p.in.mask.p + row * p.in.mask.s0 + (begin >> 5) * p.in.mask.s1 : nullptr;
+    float top = -INFINITY;
+    if (mask) {
+      for (int c = tid; c < slice.chunks; c += THREADS) {
         float2 v[N / 2];
         unpack<DT>(slice.chunk(c), v);
-        if (mask) {
-          bad |= mask_chunk<DT>(mask, p.in.mask.s1, begin + c * N, v);
-          slice.set_chunk(c, pack<DT>(v));
-        }
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) top = max_nan(top, max_nan(v[i].x, v[i].y));
-        bad |= !(top < INFINITY);
+        bad |= chunk_bad<DT>(v);
+        mask_chunk<DT>(mask_bits<DT>(mask, p.in.mask.s1, c * N), -INFINITY, v);
+        slice.chunk(c) = pack<DT>(v);
+        top = fmaxf(top, max_of<N>(v));
       }
-#pragma unroll
-      for (int o = 1; o < TILE / N; o <<= 1) top = fmaxf(top, shfl_xor(top, o));
-      if (c < slice.chunks && c % (TILE / N) == 0) tiles[c / (TILE / N)] = order_key(top);
+    } else {
+#pragma unroll 4
+      for (int c = tid; c < slice.chunks; c += THREADS) top = max_nan(top, chunk_max_nan<DT>(slice.chunk(c)));
     }
-    slice.wait_all();
-    bad |= slice.late;
+    bad |= !(top < INFINITY);
+    const uint32_t key = order_key(top);
     cluster_wait();  // every rank has started
-    __syncthreads();
 
-    const uint32_t own = max(tile_bound(sh, tiles, count, (p.k + ranks - 1) / ranks), KEY_NONE + 1);
+    const uint32_t own = max(thread_bound(key, (p.k + ranks - 1) / ranks), KEY_NONE + 1);
     if (tid < ranks) cg::this_cluster().map_shared_rank(sh.bound, tid)[rank] = own;
     cluster_arrive();
     cluster_wait();
@@ -229,23 +197,18 @@ template <int DT> struct TopRow {
     uint64_t least = uint64_t(bound) << 32;
 
     for (bool exact = false;; exact = true) {
-      list_entries(sh, tiles, count, slice, least);
+      list_entries(sh, key, slice, least);
       __syncthreads();
       const uint32_t listed = sh.listed;
       const bool fits = listed <= LISTED;
       // Rank 0's places for this rank's entries: asked for now, used after the sums.
       if (tid == 0) sh.place = fits ? atomicAdd(cg::this_cluster().map_shared_rank(&sh.total, 0), listed) : COLLECTED;
-      Acc acc = acc_none();
-      if (fits)
-        for (int c = tid; c < slice.chunks; c += THREADS) {
-          float2 v[N / 2];
-          unpack<DT>(slice.chunk(c), v);
-          acc_chunk<N, false>(acc, v, scale);
-        }
-      Record rec = {acc.m, __fadd_rn(acc.s.x, acc.s.y), 0.f, bad ? BAD : 0u};
+      Record rec = {LOWEST, 0.f, 0.f, 0u};
+      if (fits) rec = sum_slice<DT, false, false>(slice, nullptr, 0, scale);
+      if (bad) rec.flags |= BAD;
       rec = block_record(sh, rec, scale);
       const bool room = sh.place + listed <= COLLECTED;
-      rec.bad |= room ? 0 : FULL;
+      rec.flags |= room ? 0 : FULL;
       if (room) {
         uint64_t* to = cg::this_cluster().map_shared_rank(sh.collected, 0) + sh.place;
         for (uint32_t i = tid; i < listed; i += THREADS) to[i] = sh.list[i];
@@ -254,7 +217,7 @@ template <int DT> struct TopRow {
       cluster_arrive();
       cluster_wait();
       uint32_t flags = 0;
-      for (int r = 0; r < ranks; ++r) flags |= sh.inbox[r].bad;
+      for (int r = 0; r < ranks; ++r) flags |= sh.inbox[r].flags;
       bad = flags & BAD;
       if (!(flags & FULL) || bad || exact) break;
       // Too many entries: put the listed ones back and take the exact threshold.
@@ -271,26 +234,32 @@ template <int DT> struct TopRow {
     for (int i = tid; i < entries; i += THREADS) {
       const uint64_t mine = sh.collected[i];
       int place = 0;
+#pragma unroll 4
       for (int j = 0; j < entries; ++j) place += sh.collected[j] > mine;
       const float value = key_value(uint32_t(mine >> 32));
-      if (place < p.k) write(place, value, int64_t(0xffffffffu - uint32_t(mine)));
-      else rec = merge(rec, Record{value, 1.f, 0.f, 0u}, scale);
+      if (place < p.k) {
+        write(place, value, int64_t(0xffffffffu - uint32_t(mine)));
+      } else {
+        const float m = fmaxf(rec.m, value);
+        rec.s = __fadd_rn(__fmul_rn(ex2(exponent(rec.m, m, scale)), rec.s), ex2(exponent(value, m, scale)));
+        rec.m = m;
+      }
     }
     for (int i = entries + tid; i < p.k; i += THREADS) write(i, -INFINITY, -1);
     rec = block_record(sh, rec, scale);
     if (tid == 0) {
       float m = rec.m;
       for (int r = 0; r < ranks; ++r) m = fmaxf(m, sh.inbox[r].m);
-      double s = rec.s * exp2(double(exponent(rec.m, m, scale)));
-      for (int r = 0; r < ranks; ++r) s += sh.inbox[r].s * exp2(double(exponent(sh.inbox[r].m, m, scale)));
+      float s = rec.s * ex2(exponent(rec.m, m, scale));
+      for (int r = 0; r < ranks; ++r) s += sh.inbox[r].s * ex2(exponent(sh.inbox[r].m, m, scale));
       const bool ok = !bad && entries > 0;
-      p.rest[row] = ok && s > 0 ? float(double(m) / temperature + log(s)) : -INFINITY;
+      p.rest[row] = ok && s > 0 ? value_of(pair_sum(scaled_gap(m, 0.f, temperature), log_pair(s))) : -INFINITY;
       p.status[row] = bad ? ES_INVALID_INPUT : ok ? ES_OK : ES_NO_VALID_TOKEN;
     }
   }
 };
 
-template <int DT> __global__ void __launch_bounds__(THREADS, 4) top_rows(const __grid_constant__ TopParams p) {
+template <int DT> __global__ void __launch_bounds__(THREADS, ES_SCORE_BLOCKS) top_rows(const __grid_constant__ TopParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   const int ranks = p.in.ranks, rank = int(blockIdx.x % unsigned(ranks));
   const int begin = rank * p.in.slice, n = min(p.in.slice, p.in.vocab - begin);

@@ -116,19 +116,29 @@ class RowBounds:
         return self.sum * (2 + 2 * self.m1) + 3 * 2.0**-24 * self.m2 + 2.0**-23 * abs(float(h))
 
     def probability(self, logp):
-        """Relative, of each token's probability."""
+        """Relative, of each token's probability times the row's coefficient.
+
+        The coefficient's way in 32 bits: 1 / temperature, its product with
+        the slope, the entropy's part (a product, a difference), 1 / sum, the
+        product with it, the correction of the exponent's reference (three),
+        and the last product: ten roundings."""
         d = (logp - logp.max()).clamp(min=-200).abs()
-        return 2.0**-22 + 3 * 2.0**-24 * d + self.sum + 4 * 2.0**-24
+        return 2.0**-22 + 3 * 2.0**-24 * d + self.sum + 10 * 2.0**-24
 
 
-def token_grad_bound(bounds, logp, grad, on_lp, on_h, h, temperature, dtype):
-    """Per token, for the gradient of on_lp * lp + on_h * H."""
+def token_grad_bound(bounds, logp, grad, token, on_lp, on_h, h, temperature, dtype):
+    """Per token, for the gradient of on_lp * lp + on_h * H at `token`."""
     p = logp.exp()
     # The kernel's sum has h, log(sum) and d in it, and log(sum) = d - log p.
     d = (logp - logp.max()).clamp(min=-1e4).abs()
     size = abs(on_lp) + abs(on_h) * (logp.clamp(min=-1e4).abs() + abs(h) + 2 * d)
     absolute = p * (size * bounds.probability(logp) + abs(on_h) * bounds.entropy(h)) / temperature
-    # The token's own entry is formed in 64 bits from p: the same bound holds.
+    # The token's own entry, (1 - p) on_lp / temperature and the entropy's
+    # part, moves with p by as much, and is a product of its own: 1 /
+    # temperature and two products are rounded once each (2^-24), and expm1
+    # is within one unit in the last place (2^-23).
+    absolute[token] += 5 * 2.0**-24 * (abs(on_lp) * float(-torch.expm1(logp[token])) +
+                                       abs(on_h) * float(p[token]) * (abs(float(logp[token])) + abs(h))) / temperature
     # An exponential below 2^-126 (of the maximum's, at most the sum) is
     # flushed to zero: p is then off by at most 2^-126, and the gradient by
     # that times size / temperature, which exceeds the type's smallest number

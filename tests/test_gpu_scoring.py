@@ -85,7 +85,7 @@ def check_logprobs(x, tokens, temperatures, allowed, out, grad=None, on_lp=None,
             leaf = z[r].clone().requires_grad_()
             f(leaf).backward()
             want = torch.where(allowed[r] & (z[r] > -math.inf), leaf.grad, 0.0)
-            limit = ref.token_grad_bound(bounds, logp, want, a, b, h, temperature, x.dtype)
+            limit = ref.token_grad_bound(bounds, logp, want, t, a, b, h, temperature, x.dtype)
             off = (grad[r].cpu().double() - want).abs()
             assert bool((off <= limit).all()), (r, float((off / limit).max()))
 
@@ -336,7 +336,7 @@ def check_policy(x, temperatures, allowed, inputs, out, grad, kl_coef, entropy_c
         want = torch.where(allowed[r], leaf.grad, 0.0)
         # The slope itself moves with lp: ratio and the KL term's exponential, relatively by bounds.sum.
         size = w * (slope + kl_coef * (rise + 1) * with_ref)
-        limit = ref.token_grad_bound(bounds, logp, want, size, w * entropy_coef, float(h), temperature, x.dtype)
+        limit = ref.token_grad_bound(bounds, logp, want, t, size, w * entropy_coef, float(h), temperature, x.dtype)
         limit[t] += size * bounds.sum / temperature
         off = (grad[r].cpu().double() - want).abs()
         assert bool((off <= limit).all()), (r, float((off / limit).max()))
@@ -435,14 +435,30 @@ def check_distill(x, values, ids, rest, weights, temperatures, allowed, out, gra
         if lost:
             assert float(out.loss[r]) == 0 and (grad is None or bool((grad[r] == 0).all()))
             continue
-        # The others' sum has 32-bit terms; the kept tokens' are 64-bit, and
-        # so is everything after. log q moves by at most the sum's error, and
-        # the loss with it, t being a distribution.
+        # All in 32 bits. The others' sum is off by `error`. The kept tokens'
+        # exponentials t and q are off by an expf (2^-23) and two products;
+        # sums of them add at most K / 128 + 10 joins (12 here), and shares of
+        # the totals a reciprocal and three products: 20 roundings at most,
+        # `part`. In the loss, a term t (lt - lq) has the error of t and three
+        # roundings of its own, 24 with the sum's joins; the logs of the
+        # totals move by the totals' relative errors, and their difference is
+        # rounded with what multiplies it.
         others = (z / temperature).masked_fill(~allowed[r], -math.inf)
         others[i[i >= 0]] = -math.inf
-        error = ref.RowBounds(torch.log_softmax(others, 0), vocab).sum if bool((others > -math.inf).any()) else 2.0**-40
-        # The record's rest and the kept values are inputs; nothing else is rounded.
-        assert abs(float(out.loss[r]) - w * float(want)) <= w * 2 * error + 2.0**-24 * abs(w * float(want)), r
+        error = ref.RowBounds(torch.log_softmax(others, 0), vocab).sum if bool((others > -math.inf).any()) else 0.0
+        part = 20 * 2.0**-24
+        kept = i >= 0
+        scale = 1 / temperature
+        x_kept = (z / temperature).masked_fill(~allowed[r], -math.inf)[i[kept]]
+        lt, lq = v[kept] * scale, x_kept
+        t = torch.log_softmax(torch.cat([lt, rr[None]]) if rr is not None else lt, 0).exp()
+        live = t[:lt.numel()] > 0
+        gaps = ((lt - lt.max()) - (lq - lq.max()))[live].abs()
+        gap_of_totals = abs(float(torch.logsumexp(lt - lt.max(), 0) - torch.logsumexp(lq - lq.max(), 0)))
+        gap_of_totals += abs(float(rr - lt.max())) if rr is not None and float(rr) > -math.inf else 0.0
+        limit = 24 * 2.0**-24 * float((t[:lt.numel()][live] * gaps).sum()) + (part + 2.0**-23) * (1 + gap_of_totals) + 2 * part
+        limit = w * (limit + 2 * error) + 3 * 2.0**-24 * abs(w * float(want))
+        assert abs(float(out.loss[r]) - w * float(want)) <= limit, r
         if grad is None:
             continue
         leaf = z.clone().requires_grad_()
@@ -451,13 +467,17 @@ def check_distill(x, values, ids, rest, weights, temperatures, allowed, out, gra
         q = logp.exp()
         pull = torch.ones(())
         if rr is not None:
-            t = torch.log_softmax(torch.cat([v[i >= 0] / temperature, rr[None]]), 0)[-1]
-            q_rest = torch.logsumexp(logp.masked_fill(torch.zeros(vocab).index_fill(0, i[i >= 0], 1).bool(), -math.inf), 0)
-            pull = 1 + (t - q_rest).exp() if q_rest > -math.inf else pull
+            q_rest = torch.logsumexp(others, 0) - torch.logsumexp((z / temperature).masked_fill(~allowed[r], -math.inf), 0)
+            pull = 1 + (t[-1].log() - q_rest).exp() if q_rest > -math.inf else pull
         d = (others - others.max()).clamp(min=-200).abs() if bool((others > -math.inf).any()) else torch.zeros(vocab)
-        relative = 2 * error + 2.0**-22 + 3 * 2.0**-24 * d + 4 * 2.0**-24
+        # 1 - t_rest / q_rest moves with both logs (part and error each), and
+        # the coefficient has six roundings more. A kept token's w (q - t) has
+        # both shares' errors and three roundings.
         # (2^-126: exponentials below it are flushed to zero.)
-        limit = w / temperature * (q * relative + 2.0**-126) * pull + g.abs() * ref.HALF_STEP[x.dtype] * 1.01 + ref.SMALLEST[x.dtype]
+        relative = 2 * error + 2.0**-22 + 3 * 2.0**-24 * d + 2 * part + 6 * 2.0**-24
+        size = (q * relative + 2.0**-126) * pull
+        size[i[kept]] += t[:lt.numel()] * (part + 3 * 2.0**-24) + 2.0**-126
+        limit = w / temperature * size + g.abs() * ref.HALF_STEP[x.dtype] * 1.01 + ref.SMALLEST[x.dtype]
         off = (grad[r].cpu().double() - g).abs()
         assert bool((off <= limit).all()), (r, float((off / limit).max()))
 
@@ -796,7 +816,8 @@ def test_a_decode_step_then_training_on_it():
     step = scoring.policy_loss(logits, tokens, old.logprobs, adv, ref_logprobs=old.logprobs, kl_coef=0.1, grad=grad, **common)
     assert torch.equal(step.logprobs, old.logprobs)
     want = torch.where(tokens >= 0, -adv, 0.0)
-    torch.testing.assert_close(step.loss, want, rtol=2.0**-22, atol=0)  # log p is rounded to float32 once
+    # log p was rounded to float32 (half a step, 2^-24 of it), the ratio is an expf (2^-23) and the loss a product.
+    torch.testing.assert_close(step.loss, want, rtol=2.0**-24 * float(old.logprobs.abs().max()) + 2.0**-22, atol=0)
     assert bool((grad[7] == 0).all()) and bool((grad[~allowed] == 0).all())
     # A student equal to its teacher: no loss and, but for rounding, no gradient.
     out = scoring.distill_loss(logits, top, grad=grad, **common)
