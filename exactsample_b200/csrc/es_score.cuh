@@ -14,6 +14,7 @@
 // takes the same elements whatever the row's address, so a row's results are
 // the same bits in any batch and at any alignment.
 #pragma once
+#include <algorithm>
 #include <atomic>
 
 #include "es_device.cuh"
@@ -22,7 +23,7 @@
 #define ES_SCORE_THREADS 128
 #endif
 #ifndef ES_SCORE_BLOCKS
-#define ES_SCORE_BLOCKS 5
+#define ES_SCORE_BLOCKS 6
 #endif
 
 namespace es {
@@ -32,6 +33,7 @@ enum Op { LOGPROB = 0, POLICY = 1, DISTILL = 2 };
 constexpr int THREADS = ES_SCORE_THREADS, WARPS = THREADS / 32;
 constexpr int MAX_RANKS = 16;   // cluster size (beyond 8: non-portable, as for the row kernels)
 constexpr int MAX_TOP = ES_MAX_TOP;
+constexpr int STEP = 4 * THREADS;  // chunks that the block takes at a time, four a thread
 constexpr int SLICE_STEP = 128; // slices are a multiple of this many tokens: whole mask words and 16-byte chunks
 constexpr float LOWEST = -3.402823466e38f;
 // Exponents (base 2) are held at or above this: 2^FAR is 0, and a product of
@@ -56,6 +58,7 @@ struct Rows {
   Grid2<const int32_t> mask;
   Column<const double> temperature;
   double inv_all;  // 1 / temperature where it is one number
+  int64_t rows;
   int32_t vocab, ranks, slice;
 };
 
@@ -274,7 +277,7 @@ template <bool ENTROPY> __device__ __forceinline__ bool acc_failed(const Acc& a)
 }
 
 // What one rank knows of its slice: s and u against the maximum m.
-struct Record {
+struct alignas(16) Record {
   float m, s, u;
   uint32_t flags;
 };
@@ -290,34 +293,74 @@ template <bool ENTROPY> __device__ __forceinline__ Record acc_exact(const Acc& a
   const float s = __fadd_rn(a.s.x, a.s.y), u = __fadd_rn(a.u.x, a.u.y);
   return {fmaxf(a.m, LOWEST), __fmul_rn(f, s), ENTROPY ? __fmul_rn(f, __fmaf_rn(-rest, s, u)) : 0.f, careful ? CAREFUL : 0u};
 }
-// The records of a warp's lanes as one. Every warp of a block takes it, not in
-// a branch: where the compiler cannot tell that a whole warp is there, a
-// shuffle costs about 240 cycles instead of 25 (3,600 for these 16, measured).
-template <bool ENTROPY> __device__ __forceinline__ Record warp_record(Record r, float scale) {
-  const float m = warp_all(r.m, [](float a, float b) { return fmaxf(a, b); });
+// The records of LANES neighbouring lanes as one, in every lane. Every warp of
+// a block takes it, not in a branch: where the compiler cannot tell that a
+// whole warp is there, a shuffle costs about 240 cycles instead of 25 (3,600
+// for the 16 of a whole warp's record, measured).
+template <bool ENTROPY, int LANES> __device__ __forceinline__ Record lanes_record(Record r, float scale) {
+  float m = r.m;
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) m = fmaxf(m, shfl_xor(m, o));
   const float d = exponent(r.m, m, scale), f = ex2(d);
-  const auto sum = [](float a, float b) { return __fadd_rn(a, b); };
-  if (ENTROPY) r.u = warp_all(__fmul_rn(f, __fmaf_rn(d, r.s, r.u)), sum);
-  r.s = warp_all(__fmul_rn(f, r.s), sum);
+  if (ENTROPY) r.u = __fmul_rn(f, __fmaf_rn(d, r.s, r.u));
+  r.s = __fmul_rn(f, r.s);
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) {
+    r.s = __fadd_rn(r.s, shfl_xor(r.s, o));
+    if (ENTROPY) r.u = __fadd_rn(r.u, shfl_xor(r.u, o));
+    if (LANES < 32) r.flags |= shfl_xor(r.flags, o);
+  }
+  if (LANES == 32) r.flags = __reduce_or_sync(0xffffffffu, r.flags);
   r.m = m;
-  r.flags = __reduce_or_sync(0xffffffffu, r.flags);
   return r;
 }
-
-// This lane's of `count` records, empty beyond them.
-__device__ __forceinline__ Record lane_record(const Record* records, int count) {
-  const bool mine = lane_id() < count;
-  Record r = records[mine ? lane_id() : 0];
+// `count` records of at most LANES as one, in every lane.
+template <bool ENTROPY, int LANES>
+__device__ __forceinline__ Record join_records(const Record* records, int count, float scale) {
+  const int lane = lane_id() & (LANES - 1);
+  const bool mine = lane < count;
+  Record r = records[mine ? lane : 0];
   r.m = mine ? r.m : LOWEST;
   r.s = mine ? r.s : 0.f;
   r.u = mine ? r.u : 0.f;
   r.flags = mine ? r.flags : 0u;
-  return r;
+  return lanes_record<ENTROPY, LANES>(r, scale);
 }
 
 // ---------------------------------------------------------------------------
 // Cluster barrier halves: between them a rank does work of its own.
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+// Before any access to another rank's memory there is nothing to release but
+// the initialisation of barriers, which has its own fence.
+__device__ __forceinline__ void cluster_started() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+
+// A record into another rank's shared memory, counted by that rank's barrier:
+// the receiver waits on its own barrier alone, and the sender for nothing.
+__device__ __forceinline__ void send_record(Record* to, uint64_t* bar, int rank, const Record& r) {
+  uint32_t address, barrier;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(address) : "r"(smem_addr(to)), "r"(rank));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(barrier) : "r"(smem_addr(bar)), "r"(rank));
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(address),
+               "r"(__float_as_uint(r.m)), "r"(__float_as_uint(r.s)), "r"(__float_as_uint(r.u)), "r"(r.flags), "r"(barrier)
+               : "memory");
+}
+// Whether a barrier's phase completed in time.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
+  uint32_t spins = 0;
+  while (!mbar_try_wait(bar, parity))
+    if (++spins >= WAIT_LIMIT) return false;
+  return true;
+}
+
+// 16 bytes from global to shared memory, without passing through registers;
+// a thread's own copies are there after its copies_done.
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int GROUPS> __device__ __forceinline__ void copies_done() {  // all but the last GROUPS groups
+  asm volatile("cp.async.wait_group %0;" ::"n"(GROUPS) : "memory");
+}
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------
@@ -360,64 +403,85 @@ template <int SIZE> __device__ __forceinline__ uint4 shifted_chunk(const uint4* 
 }
 
 // A rank's slice of the row in shared memory, element i at base + i sizeof(T).
-// The aligned middle of the slice comes by one bulk copy and only the ragged
-// ends by plain loads: a row that does not start on 16 bytes lands as far off
-// them and is then moved into place. Rows without unit stride are gathered.
+// Chunk c is copied, read and written by thread c mod THREADS alone, so that
+// an aligned row needs no barrier between its copy and its sums. Of a row
+// that does not start on 16 bytes the aligned middle is copied and only the
+// ragged ends come by plain loads; it lands as far off 16 bytes and is then
+// moved into place. Rows without unit stride are gathered.
 template <int DT> struct Slice {
   using T = typename Elem<DT>::T;
   static constexpr int N = Elem<DT>::N;
   uint8_t* base;
-  uint64_t* bar;
   uint32_t shift;
-  int n, chunks;
-  bool bulk;
+  int n, chunks, half;  // half: chunks of the first of two groups of copies, all of them whole
+  bool shared;          // chunks come from other threads' copies
 
   __device__ __forceinline__ T& operator[](int i) const { return reinterpret_cast<T*>(base)[i]; }
   __device__ __forceinline__ uint4& chunk(int c) const { return reinterpret_cast<uint4*>(base)[c]; }
 
-  // All threads; ends with a block barrier.
-  __device__ __forceinline__ void load(const Rows& in, int64_t row, int begin, int count, uint8_t* buffer, uint64_t* barrier) {
+  __device__ __forceinline__ void init(uint8_t* buffer, int count) {
     base = buffer;
-    bar = barrier;
     n = count;
     chunks = (n + N - 1) / N;
-    const T* src = static_cast<const T*>(in.logits) + row * in.l_s0 + int64_t(begin) * in.l_s1;
+    half = (chunks + 2 * STEP - 1) / (2 * STEP) * STEP;
+    if (half >= chunks) half = 0;
+  }
+  static __device__ __forceinline__ const T* source(const Rows& in, int64_t row, int begin) {
+    return static_cast<const T*>(in.logits) + row * in.l_s0 + int64_t(begin) * in.l_s1;
+  }
+  // Whether a thread may copy its own chunks of the row, each as soon as it
+  // has done with what lies in its place.
+  static __device__ __forceinline__ bool aligned(const Rows& in, const T* src) {
+    return in.l_s1 == 1 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+  }
+  // The last chunk where it is not whole, by the thread that owns it.
+  __device__ __forceinline__ void load_ragged(const T* src) const {
+    const int whole = n / N;
+    if (whole < chunks && int(threadIdx.x) == whole % THREADS)
+      for (int i = 0; i < N; ++i) (*this)[whole * N + i] = whole * N + i < n ? src[whole * N + i] : Elem<DT>::put(-INFINITY);
+  }
+  __device__ __forceinline__ void load(const Rows& in, int64_t row, int begin) {
+    const T* src = source(in, row, begin);
     const int tid = threadIdx.x;
-    bulk = false;
-    shift = 0;
+    shared = !aligned(in, src);
+    shift = in.l_s1 == 1 ? uint32_t(reinterpret_cast<uintptr_t>(src)) & 15 : 0u;
+    if (!shared) {
+      const uint4* from = reinterpret_cast<const uint4*>(src);
+      const int whole = n / N;
+      int c = tid;
+      for (; c < half; c += THREADS) copy_async(&chunk(c), from + c);
+      copies_end_group();
+      for (; c < whole; c += THREADS) copy_async(&chunk(c), from + c);
+      copies_end_group();
+      load_ragged(src);
+      return;
+    }
+    __syncthreads();  // other threads have done with their chunks of the row before
     if (in.l_s1 == 1) {
-      const uint32_t bytes = uint32_t(n) * sizeof(T);
-      shift = uint32_t(reinterpret_cast<uintptr_t>(src)) & 15;
-      const uint32_t lead = min((16 - shift) & 15, bytes), middle = (bytes - lead) & ~15u;
-      bulk = middle > 0;
-      if (tid == 0 && bulk) {
-        mbar_init(bar, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        mbar_arrive_expect_tx(bar, middle);
-        bulk_load(base + shift + lead, reinterpret_cast<const uint8_t*>(src) + lead, middle, bar);
-      }
+      const int head = min(int((16 - shift) / sizeof(T)), n), middle = (n - head) / N;
       T* landed = reinterpret_cast<T*>(base + shift);
-      const int head = int(lead / sizeof(T)), tail = int((lead + middle) / sizeof(T));
+      const uint4* from = reinterpret_cast<const uint4*>(src + head);
+      uint4* to = reinterpret_cast<uint4*>(landed + head);
+      for (int c = tid; c < middle; c += THREADS) copy_async(to + c, from + c);
+      const int tail = head + middle * N + tid - 32;
       if (tid < head) landed[tid] = src[tid];
-      if (tid >= 32 && tail + tid - 32 < n) landed[tail + tid - 32] = src[tail + tid - 32];
+      if (tid >= 32 && tail < n) landed[tail] = src[tail];
     } else {
       for (int i = tid; i < n; i += THREADS) (*this)[i] = src[i * in.l_s1];
     }
+    copies_end_group();
     if (tid < chunks * N - n)  // the last chunk's unused places
       reinterpret_cast<T*>(base + shift)[n + tid] = Elem<DT>::put(-INFINITY);
-    __syncthreads();
   }
-  // All threads: the slice is there and in place. False if it did not come in time.
-  __device__ __forceinline__ bool wait() const {
-    bool came = true;
-    if (bulk) {
-      uint32_t spins = 0;
-      while (!mbar_try_wait(bar, 0))
-        if (++spins >= WAIT_LIMIT) {
-          came = false;
-          break;
-        }
+  // All threads: after this a thread may read its chunks below `half`, if the
+  // slice is not `shared`, or all of them.
+  __device__ __forceinline__ void arrive() const {
+    if (!shared) {
+      copies_done<1>();
+      return;
     }
+    copies_done<0>();
+    __syncthreads();
     if (shift) {
       // Chunks move down by less than one chunk, THREADS at a time: a round
       // reads only what no earlier round wrote.
@@ -428,10 +492,10 @@ template <int DT> struct Slice {
         __syncthreads();
         if (c < chunks) chunk(c) = q;
       }
-      __syncthreads();
     }
-    return came;
   }
+  // And after this all of its chunks.
+  __device__ __forceinline__ void arrive_rest() const { copies_done<0>(); }
 };
 
 // Masked rows hold the logits in the sums at or above this, where 2^d is 0 but
@@ -465,7 +529,8 @@ template <int N> __device__ __forceinline__ float max_of(const float2* v) {
 }
 
 // This thread's share of a slice as a Record: the fast form, or where that
-// fails the careful one. `mask` is the slice's first word, or null.
+// fails the careful one. `mask` is the slice's first word, or null. The slice
+// has arrived up to `half`.
 template <int DT, bool ENTROPY, bool HAS_MASK>
 __device__ __forceinline__ Record sum_slice(const Slice<DT>& slice, const int32_t* mask, int64_t stride, float scale) {
   constexpr int N = Elem<DT>::N;
@@ -473,6 +538,7 @@ __device__ __forceinline__ Record sum_slice(const Slice<DT>& slice, const int32_
   bool bad = false;
   Acc a = acc_none();
   if (HAS_MASK) {
+    slice.arrive_rest();
     for (int c = tid; c < slice.chunks; c += THREADS) {
       float2 v[N / 2];
       unpack<DT>(slice.chunk(c), v);
@@ -484,17 +550,26 @@ __device__ __forceinline__ Record sum_slice(const Slice<DT>& slice, const int32_
       acc_fast<N, ENTROPY>(a, v, top, scale);
     }
   } else {
-    // Two chunks a step: one look at the maximum for both, and independent
+    // Four chunks a step: one look at the maximum for all, and independent
     // loads and exponentials.
     int c = tid;
-    for (; c + THREADS < slice.chunks; c += 2 * THREADS) {
-      const uint4 q0 = slice.chunk(c), q1 = slice.chunk(c + THREADS);
-      float2 v[N];
-      unpack<DT>(q0, v);
-      unpack<DT>(q1, v + N / 2);
-      acc_fast<2 * N, ENTROPY>(a, v, chunk_max<DT>(q0, q1), scale);
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {
+      if (part) slice.arrive_rest();
+      const int end = part ? slice.chunks : slice.half;
+#pragma unroll 1
+      for (; c + 3 * THREADS < end; c += STEP) {
+        uint4 q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = slice.chunk(c + i * THREADS);
+        const float top = fmaxf(chunk_max<DT>(q[0], q[1]), chunk_max<DT>(q[2], q[3]));
+        float2 v[2 * N];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) unpack<DT>(q[i], v + i * N / 2);
+        acc_fast<4 * N, ENTROPY>(a, v, top, scale);
+      }
     }
-    if (c < slice.chunks) {
+    for (; c < slice.chunks; c += THREADS) {
       const uint4 q = slice.chunk(c);
       float2 v[N / 2];
       unpack<DT>(q, v);
@@ -572,10 +647,11 @@ struct RowScalars {
   float w, inv_q, inv_t;   // distillation: the kept tokens' gradients are w (q inv_q - t inv_t)
 };
 
+// Two of what a row writes while slower warps or ranks may still read the row before's.
 struct Shared {
-  uint64_t bar;
-  Record inbox[MAX_RANKS];
-  Record warps[WARPS];
+  Record inbox[2][MAX_RANKS];
+  Record warps[2][WARPS];
+  uint64_t bar[2];
   RowScalars row;
   float sums[WARPS][3];  // distillation: kept_sums by warp
 };
@@ -617,6 +693,9 @@ __device__ __forceinline__ float warp_top(float v) {
   return warp_all(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
+// A cluster takes rows at a stride of all clusters. While a row's gradient is
+// written, each thread copies the next row's chunks into the places that it
+// has done with: the next row's way from HBM costs no time and no memory.
 template <int DT, int OP, bool GRAD> struct LossRow {
   using E = Elem<DT>;
   using T = typename E::T;
@@ -624,7 +703,7 @@ template <int DT, int OP, bool GRAD> struct LossRow {
   static constexpr bool ENTROPY = OP != DISTILL;
 
   const LossParams& p;
-  int64_t row;
+  int64_t row, stride;
   int rank, ranks, begin, n, tid;
 
   __device__ __forceinline__ T logit(int64_t j) const {
@@ -664,8 +743,8 @@ template <int DT, int OP, bool GRAD> struct LossRow {
   // What the row's scalars need besides the sums, fetched while the row is on its way.
   struct Inputs {
     int64_t token;
-    float z;        // the token's logit
-    bool allowed;
+    T raw;          // the token's logit
+    uint32_t mask;  // its mask word
     float first, second, ref, w;  // logprob: the two incoming gradients; policy: old log-probability
                                   // and advantage; distillation: the teacher's rest
   };
@@ -686,7 +765,8 @@ template <int DT, int OP, bool GRAD> struct LossRow {
   // hangs on it.
   __device__ __forceinline__ void token_scalars(Shared& sh, float m, float s, float u, uint32_t flags, const Scale& scale,
                                                 const Inputs& in) {
-    const Pair log_s = log_pair(s), lp = pair_sum(scaled_gap(in.z, m, scale), negated(log_s));
+    const float z = E::get(in.raw);
+    const Pair log_s = log_pair(s), lp = pair_sum(scaled_gap(z, m, scale), negated(log_s));
     const float inv_s = __frcp_rn(s), gap = u * inv_s * float(LN2);  // log(s) - h
     const float h = value_of({log_s.hi, log_s.lo - gap});
     // A NaN logit makes s NaN, +inf the maximum.
@@ -721,7 +801,7 @@ template <int DT, int OP, bool GRAD> struct LossRow {
     int status = ES_OK;
     if (bad) status = ES_INVALID_INPUT;
     else if (s == 0.f) status = ES_NO_VALID_TOKEN;
-    else if (in.z == -INFINITY || !in.allowed) status = ES_DRAFT_ZERO_PROB;
+    else if (z == -INFINITY || !(in.mask >> (in.token & 31) & 1)) status = ES_DRAFT_ZERO_PROB;
     const bool ok = status == ES_OK;
     if (rank == 0)
       outputs(status, ok ? loss : 0.f, ok ? value_of(lp) : -INFINITY, ok ? kl : 0.f, ok ? h : 0.f);
@@ -846,8 +926,7 @@ template <int DT, int OP, bool GRAD> struct LossRow {
   // The gradient of chunk c from its logits. FORM 0: 2^d a; 1: 2^d (a + b d);
   // 2: the careful form of the latter.
   template <int FORM, bool HAS_MASK>
-  __device__ __forceinline__ uint4 grad_chunk(const uint4& q, int c, const int32_t* mask, const RowScalars& r, float scale,
-                                              int token) const {
+  __device__ __forceinline__ uint4 grad_chunk(const uint4& q, int c, const int32_t* mask, const RowScalars& r, float scale) const {
     float2 v[N / 2];
     unpack<DT>(q, v);
     if (HAS_MASK) {
@@ -865,45 +944,59 @@ template <int DT, int OP, bool GRAD> struct LossRow {
       const float2 e = make_float2(ex2(d.x), ex2(d.y));
       v[i] = mul2(e, FORM == 0 ? both(r.a) : fma2(both(r.b), d, both(r.a)));
     }
-    if (OP != DISTILL && token / N == c) {
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        if (token % N == 2 * i) v[i].x = r.token_grad;
-        if (token % N == 2 * i + 1) v[i].y = r.token_grad;
-      }
-    }
     return pack<DT>(v);
   }
 
-  // The gradient of this rank's slice from its shared copy.
+  // The gradient of this rank's slice from its shared copy. `token`: the row's
+  // token in it, or negative. `next`: the slice's place in the next row, or null.
   template <int FORM, bool HAS_MASK>
-  __device__ __forceinline__ void write_grad(const Slice<DT>& slice, const RowScalars& scalars, float scale, int token) const {
+  __device__ __forceinline__ void write_grad(const Slice<DT>& slice, const RowScalars& scalars, float scale, int token,
+                                             const T* next) const {
     const RowScalars r = scalars;
     const int32_t* mask = HAS_MASK ? p.in.mask.p + row * p.in.mask.s0 + (begin >> 5) * p.in.mask.s1 : nullptr;
+    const bool own = OP != DISTILL && token >= 0 && token / N % THREADS == tid;  // this thread writes the token's chunk
     if (grad_vector()) {
       uint4* out = reinterpret_cast<uint4*>(grad_at(begin));
+      const uint4* from = reinterpret_cast<const uint4*>(next);
       const int whole = n / N;
       int c = tid;
-      for (; c + THREADS < whole; c += 2 * THREADS) {
-        const uint4 q0 = slice.chunk(c), q1 = slice.chunk(c + THREADS);
-        out[c] = grad_chunk<FORM, HAS_MASK>(q0, c, mask, r, scale, token);
-        out[c + THREADS] = grad_chunk<FORM, HAS_MASK>(q1, c + THREADS, mask, r, scale, token);
-      }
-      for (; c < slice.chunks; c += THREADS) {
-        const uint4 q = grad_chunk<FORM, HAS_MASK>(slice.chunk(c), c, mask, r, scale, token);
-        if (c < whole) {
-          out[c] = q;
-        } else {
-          const T* v = reinterpret_cast<const T*>(&q);
-          for (int i = 0; i < n - c * N; ++i) *grad_at(begin + c * N + i) = v[i];
+#pragma unroll 1
+      for (int part = 0; part < 2; ++part) {
+        const int end = part ? whole : slice.half;
+#pragma unroll 1
+        for (; c + 3 * THREADS < end; c += STEP) {
+          uint4 q[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) q[i] = slice.chunk(c + i * THREADS);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) out[c + i * THREADS] = grad_chunk<FORM, HAS_MASK>(q[i], c + i * THREADS, mask, r, scale);
+          if (next) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) copy_async(&slice.chunk(c + i * THREADS), from + c + i * THREADS);
+          }
         }
+        if (part) {
+          for (; c < whole; c += THREADS) {
+            out[c] = grad_chunk<FORM, HAS_MASK>(slice.chunk(c), c, mask, r, scale);
+            if (next) copy_async(&slice.chunk(c), from + c);
+          }
+        }
+        copies_end_group();
       }
+      if (c == whole && whole < slice.chunks) {
+        const uint4 q = grad_chunk<FORM, HAS_MASK>(slice.chunk(c), c, mask, r, scale);
+        const T* v = reinterpret_cast<const T*>(&q);
+        for (int i = 0; i < n - c * N; ++i) *grad_at(begin + c * N + i) = v[i];
+      }
+      if (next) slice.load_ragged(next);
+      if (own) *grad_at(begin + token) = E::put(r.token_grad);
       return;
     }
     // Gradient rows that do not start on 16 bytes, or have a stride: by way of
     // shared memory, in 16-byte pieces from the first aligned address on.
     for (int c = tid; c < slice.chunks; c += THREADS)
-      slice.chunk(c) = grad_chunk<FORM, HAS_MASK>(slice.chunk(c), c, mask, r, scale, token);
+      slice.chunk(c) = grad_chunk<FORM, HAS_MASK>(slice.chunk(c), c, mask, r, scale);
+    if (own) slice[token] = E::put(r.token_grad);
     __syncthreads();
     int done = 0;
     if (p.g_s1 == 1) {
@@ -917,126 +1010,170 @@ template <int DT, int OP, bool GRAD> struct LossRow {
     for (int i = done + tid; i < n; i += THREADS) *grad_at(begin + i) = slice[i];
   }
   template <bool HAS_MASK>
-  __device__ __forceinline__ void write_form(const Slice<DT>& slice, const RowScalars& r, float scale, int token) const {
-    if (r.careful) write_grad<2, HAS_MASK>(slice, r, scale, token);
-    else if (ENTROPY && r.b != 0.f) write_grad<1, HAS_MASK>(slice, r, scale, token);
-    else write_grad<0, HAS_MASK>(slice, r, scale, token);
+  __device__ __forceinline__ void write_form(const Slice<DT>& slice, const RowScalars& r, float scale, int token, const T* next) const {
+    if (r.careful) write_grad<2, HAS_MASK>(slice, r, scale, token, next);
+    else if (ENTROPY && r.b != 0.f) write_grad<1, HAS_MASK>(slice, r, scale, token, next);
+    else write_grad<0, HAS_MASK>(slice, r, scale, token, next);
+  }
+
+  // Distillation: a row's entries into shared memory; false if there are none.
+  __device__ __forceinline__ bool load_entries(const Kept& kept, bool& bad) const {
+    bool any = false;
+    for (int k = tid; k < p.k; k += THREADS) {
+      const int64_t id = p.ids.p[row * p.ids.s0 + k * p.ids.s1];
+      const float value = p.values.p[row * p.values.s0 + k * p.values.s1];
+      any |= id >= 0;
+      bad |= id >= p.in.vocab || (id >= 0 && !(value < INFINITY));
+      const bool usable = id >= 0 && id < p.in.vocab;
+      float x = -INFINITY;
+      if (usable) {
+        x = E::get(logit(id));
+        bad |= !(x < INFINITY);
+        if (!allowed(id)) x = -INFINITY;
+      }
+      kept.id[k] = usable ? int(id) : -1;
+      kept.value[k] = value;
+      kept.x[k] = x;
+    }
+    return __syncthreads_or(any);
   }
 
   __device__ __forceinline__ void run(uint8_t* smem) {
     Shared& sh = *reinterpret_cast<Shared*>(smem);
     uint8_t* buffer = smem + SHARED_BYTES;
     const Kept kept(buffer + slice_bytes<DT>(p.in.slice), p.k);
-
-    // The row's token, or the teacher's entries; rows without are not read.
-    Inputs in{};
-    bool bad = false;
-    if (OP != DISTILL) {
-      in.token = p.tokens[row];
-    } else {
-      bool any = false;
-      for (int k = tid; k < p.k; k += THREADS) {
-        const int64_t id = p.ids.p[row * p.ids.s0 + k * p.ids.s1];
-        const float value = p.values.p[row * p.values.s0 + k * p.values.s1];
-        any |= id >= 0;
-        bad |= id >= p.in.vocab || (id >= 0 && !(value < INFINITY));
-        kept.id[k] = id >= 0 && id < p.in.vocab ? int(id) : -1;
-        kept.value[k] = value;
+    if (tid == 0) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sh.bar[i], 1);
+        mbar_arrive_expect_tx(&sh.bar[i], uint32_t(ranks * sizeof(Record)));
       }
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (OP == DISTILL)
       for (int i = tid; i < p.in.slice / 32; i += THREADS) kept.seen[i] = 0;
-      in.token = __syncthreads_or(any) ? 0 : -1;
-    }
-    if (in.token < 0) {
-      if (GRAD) zero_grad();
-      if (rank == 0 && tid == 0) outputs(ES_OK, 0.f, 0.f, 0.f, 0.f);
-      return;
-    }
-    cluster_arrive();  // this rank's shared memory may be written from now on
-    Slice<DT> slice;
-    slice.load(p.in, row, begin, n, buffer, &sh.bar);
-    const Scale scale = row_scale(p.in, row);
-    bad |= scale.bad;
-    if (tid == 0) {
-      if (OP != DISTILL && in.token < p.in.vocab) {
-        in.z = E::get(logit(in.token));
-        in.allowed = allowed(in.token);
-      }
-      if (OP == LOGPROB && GRAD) {
-        if (p.grad_logprobs.p) in.first = p.grad_logprobs[row];
-        if (p.grad_entropy.p) in.second = p.grad_entropy[row];
-      }
-      if (OP == POLICY) {
-        in.first = p.old_logprobs[row];
-        in.second = p.advantages[row];
-        if (p.ref_logprobs.p) in.ref = p.ref_logprobs[row];
-      }
-      if (OP == DISTILL && p.rest.p) in.first = p.rest[row];
-      if (OP != LOGPROB) in.w = p.weights.p ? p.weights[row] : 1.f;
-    }
-    float value_top = 0.f, x_top = 0.f;
-    if (OP == DISTILL) {
-      for (int k = tid; k < p.k; k += THREADS) {
-        float x = -INFINITY;
-        if (kept.id[k] >= 0) {
-          x = E::get(logit(kept.id[k]));
-          bad |= !(x < INFINITY);
-          if (!allowed(kept.id[k])) x = -INFINITY;
-        }
-        kept.x[k] = x;
-      }
-      __syncthreads();
-      kept_sums(sh, kept, scale, value_top, x_top);
-    }
-    bad |= !slice.wait();
-    if (OP == DISTILL) {
-      // The kept tokens leave the slice, so that what is summed is the others.
-      for (int k = tid; k < p.k; k += THREADS) {
-        const int local = kept.id[k] - begin;
-        if (kept.id[k] >= 0 && local >= 0 && local < n) {
-          bad |= (atomicOr(&kept.seen[local >> 5], 1u << (local & 31)) >> (local & 31)) & 1;
-          slice[local] = E::put(-INFINITY);
-        }
-      }
-      __syncthreads();
-    }
+    __syncthreads();
+    cluster_started();
+    bool peers = false;  // whether every rank is known to have started
 
-    const int32_t* mask = p.in.mask.p ? p.in.mask.p + row * p.in.mask.s0 + (begin >> 5) * p.in.mask.s1 : nullptr;
-    Record rec = mask ? sum_slice<DT, ENTROPY, true>(slice, mask, p.in.mask.s1, scale.log2)
-                      : sum_slice<DT, ENTROPY, false>(slice, nullptr, 0, scale.log2);
-    if (bad) rec.flags |= BAD;
-    rec = warp_record<ENTROPY>(rec, scale.log2);
-    if (lane_id() == 0) sh.warps[warp_id()] = rec;
-    cluster_wait();  // every rank has started
-    __syncthreads();
-    rec = warp_record<ENTROPY>(lane_record(sh.warps, WARPS), scale.log2);
-    if (tid < ranks) cg::this_cluster().map_shared_rank(sh.inbox, tid)[rank] = rec;
-    cluster_arrive();
-    cluster_wait();
-    if (!GRAD && rank != 0) return;
-    rec = warp_record<ENTROPY>(lane_record(sh.inbox, ranks), scale.log2);
-    if (tid == 0) {
-      if (OP == DISTILL) distill_scalars(sh, rec.m, rec.s, rec.flags, scale, in, value_top, x_top);
-      else token_scalars(sh, rec.m, rec.s, rec.u, rec.flags, scale, in);
-    }
-    if (!GRAD) return;
-    __syncthreads();
-    const RowScalars& r = sh.row;
-    if (r.zero) {
-      zero_grad();
-      return;
-    }
-    const int64_t local = in.token - begin;
-    const int at = OP != DISTILL && local >= 0 && local < n ? int(local) : -N;
-    if (mask) write_form<true>(slice, r, scale.log2, at);
-    else write_form<false>(slice, r, scale.log2, at);
-    if (OP == DISTILL) {
-      __syncthreads();  // after the slice's zeros at these places
-      for (int k = tid; k < p.k; k += THREADS) {
-        const int local_id = kept.id[k] - begin;
-        if (kept.id[k] >= 0 && local_id >= 0 && local_id < n)
-          *grad_at(kept.id[k]) = E::put(r.w * (kept.q[k] * r.inv_q - kept.t[k] * r.inv_t));
+    Slice<DT> slice;
+    slice.init(buffer, n);
+    bool loaded = false;  // the row's copies are under way
+    int turn = 0;         // rows taken so far, those without a token aside
+    int64_t next_token = OP != DISTILL ? p.tokens[row] : 0;
+    for (; row < p.in.rows; row += stride) {
+      // The row's token, or the teacher's entries; rows without are not read.
+      Inputs in{};
+      bool bad = false;
+      in.token = next_token;
+      if (OP != DISTILL && row + stride < p.in.rows) next_token = p.tokens[row + stride];
+      if (OP == DISTILL) in.token = load_entries(kept, bad) ? 0 : -1;
+      if (in.token < 0) {
+        if (loaded) {
+          copies_done<0>();  // (distillation learns too late that the row is not needed)
+          loaded = false;
+        }
+        if (GRAD) zero_grad();
+        if (rank == 0 && tid == 0) outputs(ES_OK, 0.f, 0.f, 0.f, 0.f);
+        continue;
       }
+      if (!loaded) slice.load(p.in, row, begin);
+      const Scale scale = row_scale(p.in, row);
+      bad |= scale.bad;
+      if (tid == 0) {
+        in.mask = 0xffffffffu;
+        if (OP != DISTILL && in.token < p.in.vocab) {
+          in.raw = logit(in.token);
+          if (p.in.mask.p) in.mask = uint32_t(p.in.mask.p[row * p.in.mask.s0 + (in.token >> 5) * p.in.mask.s1]);
+        }
+        if (OP == LOGPROB && GRAD) {
+          if (p.grad_logprobs.p) in.first = p.grad_logprobs[row];
+          if (p.grad_entropy.p) in.second = p.grad_entropy[row];
+        }
+        if (OP == POLICY) {
+          in.first = p.old_logprobs[row];
+          in.second = p.advantages[row];
+          if (p.ref_logprobs.p) in.ref = p.ref_logprobs[row];
+        }
+        if (OP == DISTILL && p.rest.p) in.first = p.rest[row];
+        if (OP != LOGPROB) in.w = p.weights.p ? p.weights[row] : 1.f;
+      }
+      float value_top = 0.f, x_top = 0.f;
+      if (OP == DISTILL) kept_sums(sh, kept, scale, value_top, x_top);
+      slice.arrive();
+      if (OP == DISTILL) {
+        slice.arrive_rest();
+        __syncthreads();
+        // The kept tokens leave the slice, so that what is summed is the others.
+        for (int k = tid; k < p.k; k += THREADS) {
+          const int local = kept.id[k] - begin;
+          if (kept.id[k] >= 0 && local >= 0 && local < n) {
+            bad |= (atomicOr(&kept.seen[local >> 5], 1u << (local & 31)) >> (local & 31)) & 1;
+            slice[local] = E::put(-INFINITY);
+          }
+        }
+        __syncthreads();
+      }
+
+      const int32_t* mask = p.in.mask.p ? p.in.mask.p + row * p.in.mask.s0 + (begin >> 5) * p.in.mask.s1 : nullptr;
+      Record rec = mask ? sum_slice<DT, ENTROPY, true>(slice, mask, p.in.mask.s1, scale.log2)
+                        : sum_slice<DT, ENTROPY, false>(slice, nullptr, 0, scale.log2);
+      // (The token's logit is looked at before this rank says that it has done
+      // with the row's memory, which may be the gradient's.)
+      if (OP != DISTILL && tid == 0) bad |= isnan(E::get(in.raw));
+      if (bad) rec.flags |= BAD;
+      // The next row, where its chunks may be copied one by one.
+      const T* next = nullptr;
+      if (row + stride < p.in.rows && next_token >= 0) {
+        next = Slice<DT>::source(p.in, row + stride, begin);
+        if (slice.shared || !Slice<DT>::aligned(p.in, next)) next = nullptr;
+      }
+      rec = lanes_record<ENTROPY, 32>(rec, scale.log2);
+      if (lane_id() == 0) sh.warps[turn & 1][warp_id()] = rec;
+      if (!peers) cluster_wait();
+      peers = true;
+      __syncthreads();
+      rec = join_records<ENTROPY, WARPS>(sh.warps[turn & 1], WARPS, scale.log2);
+      if (tid < ranks) send_record(&sh.inbox[turn & 1][rank], &sh.bar[turn & 1], tid, rec);
+      loaded = next != nullptr;
+      if (!GRAD && loaded) slice.load(p.in, row + stride, begin);
+      const bool came = wait_bar(&sh.bar[turn & 1], turn >> 1 & 1);
+      if (tid == 0) mbar_arrive_expect_tx(&sh.bar[turn & 1], uint32_t(ranks * sizeof(Record)));  // for the row after the next
+      rec = join_records<ENTROPY, MAX_RANKS>(sh.inbox[turn & 1], ranks, scale.log2);
+      ++turn;
+      if (!came) rec.flags |= BAD;
+      if (tid == 0 && (GRAD || rank == 0)) {
+        if (OP == DISTILL) distill_scalars(sh, rec.m, rec.s, rec.flags, scale, in, value_top, x_top);
+        else token_scalars(sh, rec.m, rec.s, rec.u, rec.flags, scale, in);
+      }
+      if (GRAD) {
+        __syncthreads();
+        const RowScalars& r = sh.row;
+        if (r.zero) {
+          zero_grad();
+          if (loaded) slice.load(p.in, row + stride, begin);
+        } else {
+          if (!grad_vector()) loaded = false, next = nullptr;
+          const int64_t local = in.token - begin;
+          const int at = OP != DISTILL && local >= 0 && local < n ? int(local) : -1;
+          if (mask) write_form<true>(slice, r, scale.log2, at, next);
+          else write_form<false>(slice, r, scale.log2, at, next);
+          if (OP == DISTILL) __syncthreads();  // after the slice's zeros at these places
+          if (OP == DISTILL)
+            for (int k = tid; k < p.k; k += THREADS) {
+              const int local_id = kept.id[k] - begin;
+              if (kept.id[k] >= 0 && local_id >= 0 && local_id < n)
+                *grad_at(kept.id[k]) = E::put(r.w * (kept.q[k] * r.inv_q - kept.t[k] * r.inv_t));
+            }
+        }
+      }
+      if (OP == DISTILL)
+        for (int k = tid; k < p.k; k += THREADS) {
+          const int local = kept.id[k] - begin;
+          if (kept.id[k] >= 0 && local >= 0 && local < n) kept.seen[local >> 5] = 0;
+        }
     }
+    copies_done<0>();
+    if (!peers) cluster_wait();
   }
 };
 
@@ -1045,27 +1182,36 @@ __global__ void __launch_bounds__(THREADS, ES_SCORE_BLOCKS) loss_rows(const __gr
   extern __shared__ __align__(128) uint8_t smem[];
   const int ranks = p.in.ranks, rank = int(blockIdx.x % unsigned(ranks));
   const int begin = rank * p.in.slice, n = min(p.in.slice, p.in.vocab - begin);
-  LossRow<DT, OP, GRAD> work{p, int64_t(blockIdx.x / unsigned(ranks)), rank, ranks, begin, n, int(threadIdx.x)};
+  LossRow<DT, OP, GRAD> work{p, int64_t(blockIdx.x / unsigned(ranks)), int64_t(gridDim.x / unsigned(ranks)), rank, ranks, begin, n,
+                             int(threadIdx.x)};
   work.run(smem);
 }
 
-// Launches `rows` clusters of `ranks` blocks. A kernel's attributes are set
-// once per device, to the most that any call needs.
+// What a kernel needs to know of each device: whether its attributes are set
+// (once, to the most that any call needs), and how many clusters of one shape
+// run at a time (a few shapes asked for: the shape in the upper half).
+struct Configured {
+  std::atomic<uint64_t> devices{0};
+  std::atomic<uint64_t> clusters[64][8] = {};
+};
+
+// Launches `rows` clusters of `ranks` blocks, or, where they take the rows at a
+// stride, no more than run at a time.
 template <class P>
-cudaError_t launch_clusters(void (*kernel)(P), const P& p, int64_t rows, int ranks, size_t smem, cudaStream_t stream,
-                            std::atomic<uint64_t>& configured) {
+cudaError_t launch_clusters(void (*kernel)(P), const P& p, bool strided, int64_t rows, int ranks, size_t smem,
+                            cudaStream_t stream, Configured& configured) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  const bool known = dev < 64;
   const uint64_t bit = 1ull << (dev & 63);
-  if (dev > 63 || !(configured.load(std::memory_order_acquire) & bit)) {
+  if (!known || !(configured.devices.load(std::memory_order_acquire) & bit)) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
-    if (dev <= 63) configured.fetch_or(bit, std::memory_order_release);
+    if (known) configured.devices.fetch_or(bit, std::memory_order_release);
   }
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(unsigned(rows * ranks), 1, 1);
   config.blockDim = dim3(THREADS, 1, 1);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
@@ -1076,19 +1222,34 @@ cudaError_t launch_clusters(void (*kernel)(P), const P& p, int64_t rows, int ran
   attr[0].val.clusterDim.z = 1;
   config.attrs = attr;
   config.numAttrs = 1;
+  if (strided) {
+    const uint64_t shape = uint64_t(smem) << 8 | uint64_t(ranks);  // below 2^32
+    std::atomic<uint64_t>& slot = configured.clusters[dev & 63][(smem / 512 + ranks) & 7];
+    const uint64_t seen = slot.load(std::memory_order_relaxed);
+    int most = int(seen & 0xffffffffu);
+    if (!known || seen >> 32 != shape) {
+      config.gridDim = dim3(unsigned(ranks), 1, 1);
+      e = cudaOccupancyMaxActiveClusters(&most, kernel, &config);
+      if (e != cudaSuccess) return e;
+      most = std::max(most, 1);
+      if (known) slot.store(shape << 32 | uint64_t(most), std::memory_order_relaxed);
+    }
+    rows = std::min<int64_t>(rows, most);
+  }
+  config.gridDim = dim3(unsigned(rows * ranks), 1, 1);
   return cudaLaunchKernelEx(&config, kernel, p);
 }
 
-template <int DT, int OP, bool GRAD> cudaError_t launch_one(const LossParams& p, int64_t rows, cudaStream_t stream) {
-  static std::atomic<uint64_t> configured{0};
-  return launch_clusters(loss_rows<DT, OP, GRAD>, p, rows, p.in.ranks, loss_smem<DT>(p.in.slice, p.k), stream, configured);
+template <int DT, int OP, bool GRAD> cudaError_t launch_one(const LossParams& p, cudaStream_t stream) {
+  static Configured configured;
+  return launch_clusters(loss_rows<DT, OP, GRAD>, p, true, p.in.rows, p.in.ranks, loss_smem<DT>(p.in.slice, p.k), stream, configured);
 }
-template <int DT> cudaError_t launch_loss(const LossParams& p, int op, int64_t rows, cudaStream_t stream) {
+template <int DT> cudaError_t launch_loss(const LossParams& p, int op, cudaStream_t stream) {
   const bool grad = p.grad != nullptr;
   switch (op) {
-    case LOGPROB: return grad ? launch_one<DT, LOGPROB, true>(p, rows, stream) : launch_one<DT, LOGPROB, false>(p, rows, stream);
-    case POLICY: return grad ? launch_one<DT, POLICY, true>(p, rows, stream) : launch_one<DT, POLICY, false>(p, rows, stream);
-    default: return grad ? launch_one<DT, DISTILL, true>(p, rows, stream) : launch_one<DT, DISTILL, false>(p, rows, stream);
+    case LOGPROB: return grad ? launch_one<DT, LOGPROB, true>(p, stream) : launch_one<DT, LOGPROB, false>(p, stream);
+    case POLICY: return grad ? launch_one<DT, POLICY, true>(p, stream) : launch_one<DT, POLICY, false>(p, stream);
+    default: return grad ? launch_one<DT, DISTILL, true>(p, stream) : launch_one<DT, DISTILL, false>(p, stream);
   }
 }
 

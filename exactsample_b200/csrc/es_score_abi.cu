@@ -10,12 +10,12 @@
 
 namespace es {
 namespace score {
-extern template cudaError_t launch_loss<ES_F32>(const LossParams&, int, int64_t, cudaStream_t);
-extern template cudaError_t launch_loss<ES_F16>(const LossParams&, int, int64_t, cudaStream_t);
-extern template cudaError_t launch_loss<ES_BF16>(const LossParams&, int, int64_t, cudaStream_t);
-extern template cudaError_t launch_top<ES_F32>(const TopParams&, int64_t, cudaStream_t);
-extern template cudaError_t launch_top<ES_F16>(const TopParams&, int64_t, cudaStream_t);
-extern template cudaError_t launch_top<ES_BF16>(const TopParams&, int64_t, cudaStream_t);
+extern template cudaError_t launch_loss<ES_F32>(const LossParams&, int, cudaStream_t);
+extern template cudaError_t launch_loss<ES_F16>(const LossParams&, int, cudaStream_t);
+extern template cudaError_t launch_loss<ES_BF16>(const LossParams&, int, cudaStream_t);
+extern template cudaError_t launch_top<ES_F32>(const TopParams&, cudaStream_t);
+extern template cudaError_t launch_top<ES_F16>(const TopParams&, cudaStream_t);
+extern template cudaError_t launch_top<ES_BF16>(const TopParams&, cudaStream_t);
 }  // namespace score
 }  // namespace es
 
@@ -138,6 +138,7 @@ int split(Rows& r, const es_rows& in, size_t slice_bytes, size_t (*smem)(int, in
   r.mask = grid2<const int32_t>(in.mask);
   r.temperature = col<const double>(in.temperature);
   r.inv_all = 1. / in.temperature_all;
+  r.rows = in.logits.size[0];
   r.vocab = int32_t(vocab);
   r.slice = int32_t(slice);
   r.ranks = int32_t((vocab + slice - 1) / slice);
@@ -148,7 +149,10 @@ int split(Rows& r, const es_rows& in, size_t slice_bytes, size_t (*smem)(int, in
 size_t loss_bytes(int slice, int32_t dtype, int k) {
   return dtype == ES_F32 ? loss_smem<ES_F32>(slice, k) : loss_smem<ES_F16>(slice, k);
 }
-constexpr size_t LOSS_SLICE_BYTES = 38 * 1024;
+#ifndef LOSS_KB
+#define LOSS_KB 33
+#endif
+constexpr size_t LOSS_SLICE_BYTES = LOSS_KB * 1024;
 
 int launched(cudaError_t e) {
   return e == cudaSuccess ? ES_SUCCESS
@@ -167,9 +171,9 @@ int run_loss(Call& call, LossParams& p, const es_tensor& grad, int op, cudaStrea
   p.g_s1 = grad.stride[1];
   cudaGetLastError();  // clear a stale error so that the check reports this launch's
   switch (call.in.logits.dtype) {
-    case ES_F32: return launched(launch_loss<ES_F32>(p, op, call.rows, stream));
-    case ES_F16: return launched(launch_loss<ES_F16>(p, op, call.rows, stream));
-    default: return launched(launch_loss<ES_BF16>(p, op, call.rows, stream));
+    case ES_F32: return launched(launch_loss<ES_F32>(p, op, stream));
+    case ES_F16: return launched(launch_loss<ES_F16>(p, op, stream));
+    default: return launched(launch_loss<ES_BF16>(p, op, stream));
   }
 }
 
@@ -287,9 +291,9 @@ int top_logits(const es_top_args* a, cudaStream_t stream) {
   p.status = col<int32_t>(a->status);
   cudaGetLastError();
   switch (a->in.logits.dtype) {
-    case ES_F32: return launched(launch_top<ES_F32>(p, call.rows, stream));
-    case ES_F16: return launched(launch_top<ES_F16>(p, call.rows, stream));
-    default: return launched(launch_top<ES_BF16>(p, call.rows, stream));
+    case ES_F32: return launched(launch_top<ES_F32>(p, stream));
+    case ES_F16: return launched(launch_top<ES_F16>(p, stream));
+    default: return launched(launch_top<ES_BF16>(p, stream));
   }
 }
 

@@ -3,7 +3,7 @@
 
 namespace es {
 namespace score {
-template cudaError_t launch_loss<ES_F32>(const LossParams&, int, int64_t, cudaStream_t);
-template cudaError_t launch_top<ES_F32>(const TopParams&, int64_t, cudaStream_t);
+template cudaError_t launch_loss<ES_F32>(const LossParams&, int, cudaStream_t);
+template cudaError_t launch_top<ES_F32>(const TopParams&, cudaStream_t);
 }  // namespace score
 }  // namespace es

@@ -39,7 +39,6 @@ constexpr int COLLECTED = 1024;             // entries rank 0 takes
 static_assert(THREADS >= 8 * MAX_RANKS, "exact_threshold's exchange has a thread per digit and rank");
 
 struct TopShared {
-  uint64_t bar;
   Record inbox[MAX_RANKS];
   Record warps[WARPS];
   uint32_t bound[MAX_RANKS];
@@ -148,11 +147,11 @@ template <int DT> struct TopRow {
   }
 
   __device__ __forceinline__ Record block_record(TopShared& sh, Record rec, float scale) const {
-    rec = warp_record<false>(rec, scale);
+    rec = lanes_record<false, 32>(rec, scale);
     __syncthreads();
     if (lane_id() == 0) sh.warps[warp_id()] = rec;
     __syncthreads();
-    return warp_record<false>(lane_record(sh.warps, WARPS), scale);
+    return join_records<false, WARPS>(sh.warps, WARPS, scale);
   }
 
   __device__ __forceinline__ void run(uint8_t* smem) {
@@ -162,11 +161,13 @@ template <int DT> struct TopRow {
     if (tid == 0) sh.listed = sh.total = 0;
     cluster_arrive();  // this rank's shared memory may be written from now on
     Slice<DT> slice;
-    slice.load(p.in, row, begin, n, buffer, &sh.bar);
+    slice.init(buffer, n);
+    slice.load(p.in, row, begin);
     const Scale temperature = row_scale(p.in, row);
     const float scale = temperature.log2;
     bad |= temperature.bad;
-    bad |= !slice.wait();
+    slice.arrive();
+    slice.arrive_rest();
 
     // This thread's maximum; masked tokens leave the slice.
     const int32_t* mask = p.in.mask.p ? p.in.mask.p + row * p.in.mask.s0 + (begin >> 5) * p.in.mask.s1 : nullptr;
@@ -186,6 +187,7 @@ template <int DT> struct TopRow {
     }
     bad |= !(top < INFINITY);
     const uint32_t key = order_key(top);
+    __syncthreads();
     cluster_wait();  // every rank has started
 
     const uint32_t own = max(thread_bound(key, (p.k + ranks - 1) / ranks), KEY_NONE + 1);
@@ -267,9 +269,9 @@ template <int DT> __global__ void __launch_bounds__(THREADS, ES_SCORE_BLOCKS) to
   work.run(smem);
 }
 
-template <int DT> cudaError_t launch_top(const TopParams& p, int64_t rows, cudaStream_t stream) {
-  static std::atomic<uint64_t> configured{0};
-  return launch_clusters(top_rows<DT>, p, rows, p.in.ranks, top_smem<DT>(p.in.slice), stream, configured);
+template <int DT> cudaError_t launch_top(const TopParams& p, cudaStream_t stream) {
+  static Configured configured;
+  return launch_clusters(top_rows<DT>, p, false, p.in.rows, p.in.ranks, top_smem<DT>(p.in.slice), stream, configured);
 }
 
 }  // namespace score
