@@ -197,7 +197,10 @@ struct Acc {
   float m, r;
   float2 s, u;
 };
-__device__ __forceinline__ Acc acc_none() { return {-INFINITY, 0.f, {0.f, 0.f}, {0.f, 0.f}}; }
+// At or below this a maximum is none yet: in the fast form a masked token's
+// logit lies below it (MASKED), and a real one fails (LARGE_R).
+constexpr float NONE = -1e29f;
+__device__ __forceinline__ Acc acc_none(float m = -INFINITY) { return {m, 0.f, {0.f, 0.f}, {0.f, 0.f}}; }
 __device__ __forceinline__ float exponent(float z, float m, float scale) {
   return max_nan(__fmul_rn(__fsub_rn(z, m), scale), FAR);
 }
@@ -238,7 +241,7 @@ template <int DT> __device__ __forceinline__ float chunk_max_nan(const uint4& q)
 template <int N, bool ENTROPY>
 __device__ __forceinline__ void acc_fast(Acc& a, const float2* v, float top, float scale) {
   if (top > a.m) {
-    const float r = __fmul_rn(top, scale), d = __fsub_rn(a.r, r), f = a.m == -INFINITY ? 0.f : ex2(d);
+    const float r = __fmul_rn(top, scale), d = __fsub_rn(a.r, r), f = a.m <= NONE ? 0.f : ex2(d);
     if (ENTROPY) a.u = mul2(both(f), fma2(both(fmaxf(d, FAR)), a.s, a.u));
     a.s = mul2(both(f), a.s);
     a.m = top;
@@ -289,9 +292,9 @@ constexpr uint32_t BAD = 1, CAREFUL = 2, FULL = 4;
 // s and u against m itself: with m scale = r + rest, 2^(z scale - r) is 2^rest
 // times too large and its exponent off by rest (at most 2^-8).
 template <bool ENTROPY> __device__ __forceinline__ Record acc_exact(const Acc& a, float scale, bool careful) {
-  const float rest = careful || a.m == -INFINITY ? 0.f : __fmaf_rn(a.m, scale, -a.r), f = ex2(-rest);
+  const float rest = careful || a.m <= NONE ? 0.f : __fmaf_rn(a.m, scale, -a.r), f = ex2(-rest);
   const float s = __fadd_rn(a.s.x, a.s.y), u = __fadd_rn(a.u.x, a.u.y);
-  return {fmaxf(a.m, LOWEST), __fmul_rn(f, s), ENTROPY ? __fmul_rn(f, __fmaf_rn(-rest, s, u)) : 0.f, careful ? CAREFUL : 0u};
+  return {careful || a.m > NONE ? fmaxf(a.m, LOWEST) : LOWEST, __fmul_rn(f, s), ENTROPY ? __fmul_rn(f, __fmaf_rn(-rest, s, u)) : 0.f, careful ? CAREFUL : 0u};
 }
 // The records of LANES neighbouring lanes as one, in every lane. Every warp of
 // a block takes it, not in a branch: where the compiler cannot tell that a
@@ -498,28 +501,43 @@ template <int DT> struct Slice {
   __device__ __forceinline__ void arrive_rest() const { copies_done<0>(); }
 };
 
-// Masked rows hold the logits in the sums at or above this, where 2^d is 0 but
-// 0 times d is too. Rows with a real logit near it, or a scale that brings it
-// near 0, take the careful form (SMALL_SCALE, LARGE_R).
+// What a masked token's logit becomes in the fast form: 2^d is 0 there, and 0
+// times d is too. (Rows with a real logit near it, or a scale that brings it
+// near 0, take the careful form: LARGE_R, SMALL_SCALE.) float16 has no such
+// number; its masked logits are -inf and held at MASKED in 32 bits.
 constexpr float MASKED = -1e30f;
 constexpr float SMALL_SCALE = 1e-20f;
-// The N mask bits of a chunk.
-template <int DT> __device__ __forceinline__ uint32_t mask_bits(const int32_t* words, int64_t stride, int first) {
-  return uint32_t(words[(first >> 5) * stride]) >> (first & 31);
+template <int DT> __device__ __forceinline__ uint32_t masked_word() {
+  if constexpr (DT == ES_F32) return __float_as_uint(MASKED);
+  const typename Elem<DT>::T v = Elem<DT>::put(MASKED);
+  const uint32_t bits = *reinterpret_cast<const uint16_t*>(&v);
+  return bits << 16 | bits;
 }
-template <int DT> __device__ __forceinline__ void mask_chunk(uint32_t bits, float value, float2* v) {
+// The N mask bits of a chunk that starts at a slice's token `first`.
+__device__ __forceinline__ uint32_t mask_bits(const uint32_t* words, int first) { return words[first >> 5] >> (first & 31); }
+// Tokens whose bit is clear become `word`'s value.
+template <int DT> __device__ __forceinline__ uint4 mask_chunk(const uint4& q, uint32_t bits, uint32_t word) {
+  uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  if constexpr (DT == ES_F32) {
 #pragma unroll
-  for (int i = 0; i < Elem<DT>::N / 2; ++i) {
-    if (!(bits >> (2 * i) & 1)) v[i].x = value;
-    if (!(bits >> (2 * i + 1) & 1)) v[i].y = value;
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t keep = uint32_t(int32_t(bits << (31 - i)) >> 31);
+      w[i] = (w[i] & keep) | (word & ~keep);
+    }
+  } else {
+    // Bits 2i and 2i + 1 as the signs of two bytes, each spread over a half word.
+    const uint32_t s = (bits & 0x55u) | ((bits & 0xaau) << 7);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t keep;
+      asm("prmt.b32 %0, %1, 0, 0x9988;" : "=r"(keep) : "r"(s << (7 - 2 * i)));  // 8 + b: byte b's sign, eight times
+      w[i] = (w[i] & keep) | (word & ~keep);
+    }
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// Whether a chunk holds a NaN or +inf.
-template <int DT> __device__ __forceinline__ bool chunk_bad(const float2* v) {
-  float top = max_nan(v[0].x, v[0].y);
-#pragma unroll
-  for (int i = 1; i < Elem<DT>::N / 2; ++i) top = max_nan(top, max_nan(v[i].x, v[i].y));
-  return !(top < INFINITY);
+template <int DT> __device__ __forceinline__ uint32_t lowest_word() {  // -inf
+  return DT == ES_F32 ? 0xff800000u : DT == ES_F16 ? 0xfc00fc00u : 0xff80ff80u;
 }
 template <int N> __device__ __forceinline__ float max_of(const float2* v) {
   float top = fmaxf(v[0].x, v[0].y);
@@ -529,65 +547,76 @@ template <int N> __device__ __forceinline__ float max_of(const float2* v) {
 }
 
 // This thread's share of a slice as a Record: the fast form, or where that
-// fails the careful one. `mask` is the slice's first word, or null. The slice
-// has arrived up to `half`.
+// fails the careful one. `words`: the slice's mask; its masked tokens are
+// masked in the slice too. The slice has arrived up to `half`.
 template <int DT, bool ENTROPY, bool HAS_MASK>
-__device__ __forceinline__ Record sum_slice(const Slice<DT>& slice, const int32_t* mask, int64_t stride, float scale) {
+__device__ __forceinline__ Record sum_slice(const Slice<DT>& slice, const uint32_t* words, float scale) {
   constexpr int N = Elem<DT>::N;
+  constexpr bool HOLD = HAS_MASK && ENTROPY && DT == ES_F16;
   const int tid = threadIdx.x;
-  bool bad = false;
-  Acc a = acc_none();
-  if (HAS_MASK) {
-    slice.arrive_rest();
-    for (int c = tid; c < slice.chunks; c += THREADS) {
-      float2 v[N / 2];
-      unpack<DT>(slice.chunk(c), v);
-      bad |= chunk_bad<DT>(v);
-      mask_chunk<DT>(mask_bits<DT>(mask, stride, c * N), -INFINITY, v);
-      const float top = max_of<N>(v);
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) v[i] = make_float2(fmaxf(v[i].x, MASKED), fmaxf(v[i].y, MASKED));
-      acc_fast<N, ENTROPY>(a, v, top, scale);
+  float seen_top = -INFINITY;  // of masked rows' logits, a NaN kept
+  uint32_t any = 0;            // mask bits seen
+  Acc a = acc_none(HAS_MASK ? NONE : -INFINITY);
+  const auto take = [&](uint4& q, int c) {
+    if (HAS_MASK) {
+      const uint32_t bits = mask_bits(words, c * N) & ((1u << N) - 1u);
+      any |= bits;
+      seen_top = max_nan(seen_top, chunk_max_nan<DT>(q));
+      q = mask_chunk<DT>(q, bits, masked_word<DT>());
+      slice.chunk(c) = q;
     }
-  } else {
-    // Four chunks a step: one look at the maximum for all, and independent
-    // loads and exponentials.
-    int c = tid;
+  };
+  // Four chunks a step: one look at the maximum for all, and independent
+  // loads and exponentials.
+  int c = tid;
 #pragma unroll 1
-    for (int part = 0; part < 2; ++part) {
-      if (part) slice.arrive_rest();
-      const int end = part ? slice.chunks : slice.half;
+  for (int part = 0; part < 2; ++part) {
+    if (part) slice.arrive_rest();
+    const int end = part ? slice.chunks : slice.half;
 #pragma unroll 1
-      for (; c + 3 * THREADS < end; c += STEP) {
-        uint4 q[4];
+    for (; c + 3 * THREADS < end; c += STEP) {
+      uint4 q[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = slice.chunk(c + i * THREADS);
-        const float top = fmaxf(chunk_max<DT>(q[0], q[1]), chunk_max<DT>(q[2], q[3]));
-        float2 v[2 * N];
+      for (int i = 0; i < 4; ++i) q[i] = slice.chunk(c + i * THREADS);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) unpack<DT>(q[i], v + i * N / 2);
-        acc_fast<4 * N, ENTROPY>(a, v, top, scale);
+      for (int i = 0; i < 4; ++i) take(q[i], c + i * THREADS);
+      const float top = fmaxf(chunk_max<DT>(q[0], q[1]), chunk_max<DT>(q[2], q[3]));
+      float2 v[2 * N];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) unpack<DT>(q[i], v + i * N / 2);
+      if (HOLD) {
+#pragma unroll
+        for (int i = 0; i < 2 * N; ++i) v[i] = make_float2(fmaxf(v[i].x, MASKED), fmaxf(v[i].y, MASKED));
       }
-    }
-    for (; c < slice.chunks; c += THREADS) {
-      const uint4 q = slice.chunk(c);
-      float2 v[N / 2];
-      unpack<DT>(q, v);
-      acc_fast<N, ENTROPY>(a, v, chunk_max<DT>(q, q), scale);
+      acc_fast<4 * N, ENTROPY>(a, v, top, scale);
     }
   }
-  const bool failed = acc_failed<ENTROPY>(a) || scale < SMALL_SCALE;
+#pragma unroll 1
+  for (; c < slice.chunks; c += THREADS) {
+    uint4 q = slice.chunk(c);
+    take(q, c);
+    float2 v[N / 2];
+    unpack<DT>(q, v);
+    if (HOLD) {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) v[i] = make_float2(fmaxf(v[i].x, MASKED), fmaxf(v[i].y, MASKED));
+    }
+    acc_fast<N, ENTROPY>(a, v, chunk_max<DT>(q, q), scale);
+  }
+  const bool failed = acc_failed<ENTROPY>(a) || scale < SMALL_SCALE || (HAS_MASK && any && a.m <= NONE);
   if (failed) {
     a = acc_none();
-    for (int c = tid; c < slice.chunks; c += THREADS) {
+#pragma unroll 1
+    for (c = tid; c < slice.chunks; c += THREADS) {
+      uint4 q = slice.chunk(c);
+      if (HAS_MASK) q = mask_chunk<DT>(q, mask_bits(words, c * N), lowest_word<DT>());
       float2 v[N / 2];
-      unpack<DT>(slice.chunk(c), v);
-      if (HAS_MASK) mask_chunk<DT>(mask_bits<DT>(mask, stride, c * N), -INFINITY, v);
+      unpack<DT>(q, v);
       acc_careful<N, ENTROPY>(a, v, max_of<N>(v), scale);
     }
   }
   Record r = acc_exact<ENTROPY>(a, scale, failed);
-  if (bad) r.flags |= BAD;
+  if (HAS_MASK && !(seen_top < INFINITY)) r.flags |= BAD;
   return r;
 }
 
@@ -682,8 +711,10 @@ constexpr size_t SHARED_BYTES = (sizeof(Shared) + 15) / 16 * 16;
 template <int DT> __host__ __device__ constexpr size_t slice_bytes(int slice) {
   return size_t(slice) * sizeof(typename Elem<DT>::T) + 32;
 }
-template <int DT> __host__ __device__ constexpr size_t loss_smem(int slice, int k) {
-  return SHARED_BYTES + slice_bytes<DT>(slice) + (k > 0 ? Kept::bytes(k, slice) : 0);
+// Then two rows' mask words, and the distillation's entries.
+__host__ __device__ constexpr size_t mask_bytes(int slice) { return size_t(slice) / 8; }
+template <int DT> __host__ __device__ constexpr size_t loss_smem(int slice, bool mask, int k) {
+  return SHARED_BYTES + slice_bytes<DT>(slice) + (mask ? 2 * mask_bytes(slice) : 0) + (k > 0 ? Kept::bytes(k, slice) : 0);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -924,14 +955,15 @@ template <int DT, int OP, bool GRAD> struct LossRow {
   }
 
   // The gradient of chunk c from its logits. FORM 0: 2^d a; 1: 2^d (a + b d);
-  // 2: the careful form of the latter.
-  template <int FORM, bool HAS_MASK>
-  __device__ __forceinline__ uint4 grad_chunk(const uint4& q, int c, const int32_t* mask, const RowScalars& r, float scale) const {
+  // 2: the careful form of the latter. `words`: the mask, where the slice's
+  // masked tokens are not yet what the form needs.
+  template <int FORM>
+  __device__ __forceinline__ uint4 grad_chunk(uint4 q, int c, const uint32_t* words, const RowScalars& r, float scale) const {
     float2 v[N / 2];
+    if (FORM == 2 && words) q = mask_chunk<DT>(q, mask_bits(words, c * N), lowest_word<DT>());
     unpack<DT>(q, v);
-    if (HAS_MASK) {
-      mask_chunk<DT>(mask_bits<DT>(mask, p.in.mask.s1, c * N), -INFINITY, v);
-      if (FORM == 1) {
+    if (FORM == 1 && DT == ES_F16) {
+      if (words) {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) v[i] = make_float2(fmaxf(v[i].x, MASKED), fmaxf(v[i].y, MASKED));
       }
@@ -949,11 +981,10 @@ template <int DT, int OP, bool GRAD> struct LossRow {
 
   // The gradient of this rank's slice from its shared copy. `token`: the row's
   // token in it, or negative. `next`: the slice's place in the next row, or null.
-  template <int FORM, bool HAS_MASK>
-  __device__ __forceinline__ void write_grad(const Slice<DT>& slice, const RowScalars& scalars, float scale, int token,
-                                             const T* next) const {
+  template <int FORM>
+  __device__ __forceinline__ void write_grad(const Slice<DT>& slice, const uint32_t* words, const RowScalars& scalars, float scale,
+                                             int token, const T* next) const {
     const RowScalars r = scalars;
-    const int32_t* mask = HAS_MASK ? p.in.mask.p + row * p.in.mask.s0 + (begin >> 5) * p.in.mask.s1 : nullptr;
     const bool own = OP != DISTILL && token >= 0 && token / N % THREADS == tid;  // this thread writes the token's chunk
     if (grad_vector()) {
       uint4* out = reinterpret_cast<uint4*>(grad_at(begin));
@@ -969,7 +1000,7 @@ template <int DT, int OP, bool GRAD> struct LossRow {
 #pragma unroll
           for (int i = 0; i < 4; ++i) q[i] = slice.chunk(c + i * THREADS);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) out[c + i * THREADS] = grad_chunk<FORM, HAS_MASK>(q[i], c + i * THREADS, mask, r, scale);
+          for (int i = 0; i < 4; ++i) out[c + i * THREADS] = grad_chunk<FORM>(q[i], c + i * THREADS, words, r, scale);
           if (next) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) copy_async(&slice.chunk(c + i * THREADS), from + c + i * THREADS);
@@ -977,14 +1008,14 @@ template <int DT, int OP, bool GRAD> struct LossRow {
         }
         if (part) {
           for (; c < whole; c += THREADS) {
-            out[c] = grad_chunk<FORM, HAS_MASK>(slice.chunk(c), c, mask, r, scale);
+            out[c] = grad_chunk<FORM>(slice.chunk(c), c, words, r, scale);
             if (next) copy_async(&slice.chunk(c), from + c);
           }
         }
         copies_end_group();
       }
       if (c == whole && whole < slice.chunks) {
-        const uint4 q = grad_chunk<FORM, HAS_MASK>(slice.chunk(c), c, mask, r, scale);
+        const uint4 q = grad_chunk<FORM>(slice.chunk(c), c, words, r, scale);
         const T* v = reinterpret_cast<const T*>(&q);
         for (int i = 0; i < n - c * N; ++i) *grad_at(begin + c * N + i) = v[i];
       }
@@ -995,7 +1026,7 @@ template <int DT, int OP, bool GRAD> struct LossRow {
     // Gradient rows that do not start on 16 bytes, or have a stride: by way of
     // shared memory, in 16-byte pieces from the first aligned address on.
     for (int c = tid; c < slice.chunks; c += THREADS)
-      slice.chunk(c) = grad_chunk<FORM, HAS_MASK>(slice.chunk(c), c, mask, r, scale);
+      slice.chunk(c) = grad_chunk<FORM>(slice.chunk(c), c, words, r, scale);
     if (own) slice[token] = E::put(r.token_grad);
     __syncthreads();
     int done = 0;
@@ -1009,11 +1040,19 @@ template <int DT, int OP, bool GRAD> struct LossRow {
     }
     for (int i = done + tid; i < n; i += THREADS) *grad_at(begin + i) = slice[i];
   }
-  template <bool HAS_MASK>
-  __device__ __forceinline__ void write_form(const Slice<DT>& slice, const RowScalars& r, float scale, int token, const T* next) const {
-    if (r.careful) write_grad<2, HAS_MASK>(slice, r, scale, token, next);
-    else if (ENTROPY && r.b != 0.f) write_grad<1, HAS_MASK>(slice, r, scale, token, next);
-    else write_grad<0, HAS_MASK>(slice, r, scale, token, next);
+  __device__ __forceinline__ void write_form(const Slice<DT>& slice, const uint32_t* words, const RowScalars& r, float scale,
+                                             int token, const T* next) const {
+    if (r.careful) write_grad<2>(slice, words, r, scale, token, next);
+    else if (ENTROPY && r.b != 0.f) write_grad<1>(slice, words, r, scale, token, next);
+    else write_grad<0>(slice, words, r, scale, token, next);
+  }
+
+  // The slice's mask words of row `at` into shared memory; there after
+  // copies_done and a block barrier.
+  __device__ __forceinline__ void load_mask(uint32_t* words, int64_t at) const {
+    const int32_t* from = p.in.mask.p + at * p.in.mask.s0 + (begin >> 5) * p.in.mask.s1;
+    for (int i = tid; i < (n + 31) / 32; i += THREADS)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(words + i)), "l"(from + i * p.in.mask.s1) : "memory");
   }
 
   // Distillation: a row's entries into shared memory; false if there are none.
@@ -1041,7 +1080,9 @@ template <int DT, int OP, bool GRAD> struct LossRow {
   __device__ __forceinline__ void run(uint8_t* smem) {
     Shared& sh = *reinterpret_cast<Shared*>(smem);
     uint8_t* buffer = smem + SHARED_BYTES;
-    const Kept kept(buffer + slice_bytes<DT>(p.in.slice), p.k);
+    uint32_t* const masks = reinterpret_cast<uint32_t*>(buffer + slice_bytes<DT>(p.in.slice));
+    const bool masked = p.in.mask.p != nullptr;
+    const Kept kept(buffer + slice_bytes<DT>(p.in.slice) + (masked ? 2 * mask_bytes(p.in.slice) : 0), p.k);
     if (tid == 0) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&sh.bar[i], 1);
@@ -1076,7 +1117,11 @@ template <int DT, int OP, bool GRAD> struct LossRow {
         if (rank == 0 && tid == 0) outputs(ES_OK, 0.f, 0.f, 0.f, 0.f);
         continue;
       }
-      if (!loaded) slice.load(p.in, row, begin);
+      uint32_t* const words = masked ? masks + (turn & 1) * (p.in.slice / 32) : nullptr;
+      if (!loaded) {
+        if (masked) load_mask(words, row);
+        slice.load(p.in, row, begin);
+      }
       const Scale scale = row_scale(p.in, row);
       bad |= scale.bad;
       if (tid == 0) {
@@ -1100,6 +1145,7 @@ template <int DT, int OP, bool GRAD> struct LossRow {
       float value_top = 0.f, x_top = 0.f;
       if (OP == DISTILL) kept_sums(sh, kept, scale, value_top, x_top);
       slice.arrive();
+      if (masked && OP != DISTILL && !slice.shared) __syncthreads();  // the mask words come from all threads' first copies
       if (OP == DISTILL) {
         slice.arrive_rest();
         __syncthreads();
@@ -1114,9 +1160,8 @@ template <int DT, int OP, bool GRAD> struct LossRow {
         __syncthreads();
       }
 
-      const int32_t* mask = p.in.mask.p ? p.in.mask.p + row * p.in.mask.s0 + (begin >> 5) * p.in.mask.s1 : nullptr;
-      Record rec = mask ? sum_slice<DT, ENTROPY, true>(slice, mask, p.in.mask.s1, scale.log2)
-                        : sum_slice<DT, ENTROPY, false>(slice, nullptr, 0, scale.log2);
+      Record rec = masked ? sum_slice<DT, ENTROPY, true>(slice, words, scale.log2)
+                          : sum_slice<DT, ENTROPY, false>(slice, nullptr, scale.log2);
       // (The token's logit is looked at before this rank says that it has done
       // with the row's memory, which may be the gradient's.)
       if (OP != DISTILL && tid == 0) bad |= isnan(E::get(in.raw));
@@ -1134,7 +1179,9 @@ template <int DT, int OP, bool GRAD> struct LossRow {
       __syncthreads();
       rec = join_records<ENTROPY, WARPS>(sh.warps[turn & 1], WARPS, scale.log2);
       if (tid < ranks) send_record(&sh.inbox[turn & 1][rank], &sh.bar[turn & 1], tid, rec);
+      if (GRAD && !grad_vector()) next = nullptr;
       loaded = next != nullptr;
+      if (masked && loaded) load_mask(masks + (turn + 1 & 1) * (p.in.slice / 32), row + stride);  // in the first group
       if (!GRAD && loaded) slice.load(p.in, row + stride, begin);
       const bool came = wait_bar(&sh.bar[turn & 1], turn >> 1 & 1);
       if (tid == 0) mbar_arrive_expect_tx(&sh.bar[turn & 1], uint32_t(ranks * sizeof(Record)));  // for the row after the next
@@ -1152,11 +1199,9 @@ template <int DT, int OP, bool GRAD> struct LossRow {
           zero_grad();
           if (loaded) slice.load(p.in, row + stride, begin);
         } else {
-          if (!grad_vector()) loaded = false, next = nullptr;
           const int64_t local = in.token - begin;
           const int at = OP != DISTILL && local >= 0 && local < n ? int(local) : -1;
-          if (mask) write_form<true>(slice, r, scale.log2, at, next);
-          else write_form<false>(slice, r, scale.log2, at, next);
+          write_form(slice, words, r, scale.log2, at, next);
           if (OP == DISTILL) __syncthreads();  // after the slice's zeros at these places
           if (OP == DISTILL)
             for (int k = tid; k < p.k; k += THREADS) {
@@ -1198,7 +1243,7 @@ struct Configured {
 // Launches `rows` clusters of `ranks` blocks, or, where they take the rows at a
 // stride, no more than run at a time.
 template <class P>
-cudaError_t launch_clusters(void (*kernel)(P), const P& p, bool strided, int64_t rows, int ranks, size_t smem,
+cudaError_t launch_clusters(void (*kernel)(P), const P& p, bool strided, int64_t rows, int ranks, int threads, size_t smem,
                             cudaStream_t stream, Configured& configured) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -1212,7 +1257,7 @@ cudaError_t launch_clusters(void (*kernel)(P), const P& p, bool strided, int64_t
     if (known) configured.devices.fetch_or(bit, std::memory_order_release);
   }
   cudaLaunchConfig_t config = {};
-  config.blockDim = dim3(THREADS, 1, 1);
+  config.blockDim = dim3(unsigned(threads), 1, 1);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -1242,7 +1287,7 @@ cudaError_t launch_clusters(void (*kernel)(P), const P& p, bool strided, int64_t
 
 template <int DT, int OP, bool GRAD> cudaError_t launch_one(const LossParams& p, cudaStream_t stream) {
   static Configured configured;
-  return launch_clusters(loss_rows<DT, OP, GRAD>, p, true, p.in.rows, p.in.ranks, loss_smem<DT>(p.in.slice, p.k), stream, configured);
+  return launch_clusters(loss_rows<DT, OP, GRAD>, p, true, p.in.rows, p.in.ranks, THREADS, loss_smem<DT>(p.in.slice, p.in.mask.p != nullptr, p.k), stream, configured);
 }
 template <int DT> cudaError_t launch_loss(const LossParams& p, int op, cudaStream_t stream) {
   const bool grad = p.grad != nullptr;

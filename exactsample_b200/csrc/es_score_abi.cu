@@ -3,7 +3,6 @@
 #include <algorithm>
 #include <cmath>
 #include <exception>
-#include <vector>
 
 #include "es_host.h"
 #include "es_top.cuh"
@@ -43,10 +42,18 @@ bool addressable(const es_tensor& t, const char* name) {
 }
 
 // One call's tensors as they are checked: the inputs and the outputs.
+struct Tensors {
+  const es_tensor* list[10];
+  int count = 0;
+  void add(const es_tensor& t) { list[count++] = &t; }
+  const es_tensor* const* begin() const { return list; }
+  const es_tensor* const* end() const { return list + count; }
+};
 struct Call {
   const es_rows& in;
   int64_t rows = 0, vocab = 0;
-  std::vector<const es_tensor*> inputs, outputs;
+  Tensors inputs, outputs;
+  bool in_place = false;  // the gradient is the logits tensor
 
   // The logits, the mask and the temperatures.
   int begin() {
@@ -62,12 +69,12 @@ struct Call {
     rows = logits.size[0];
     vocab = logits.size[1];
     if (vocab < 1) return fail(ES_ERR_ARGUMENT, "logits must have at least one column");
-    inputs.push_back(&logits);
+    inputs.add(logits);
     if (present(in.mask)) {
       if (!check(in.mask, ES_I32, 2, "mask") || !addressable(in.mask, "mask")) return ES_ERR_ARGUMENT;
       if (!(in.mask.size[0] == rows && in.mask.size[1] == (vocab + 31) / 32))
         return fail(ES_ERR_ARGUMENT, "mask shape mismatch");
-      inputs.push_back(&in.mask);
+      inputs.add(in.mask);
     }
     if (present(in.temperature)) {
       if (const int e = column(in.temperature, ES_F64, "temperature", inputs); e != ES_SUCCESS) return e;
@@ -76,16 +83,16 @@ struct Call {
     }
     return ES_SUCCESS;
   }
-  int column(const es_tensor& t, int32_t dtype, const char* name, std::vector<const es_tensor*>& list) {
+  int column(const es_tensor& t, int32_t dtype, const char* name, Tensors& list) {
     if (!check(t, dtype, 1, name) || !addressable(t, name)) return ES_ERR_ARGUMENT;
     if (t.size[0] != rows) return fail(ES_ERR_ARGUMENT, std::string(name) + " must have one value per row");
-    list.push_back(&t);
+    list.add(t);
     return ES_SUCCESS;
   }
-  int grid(const es_tensor& t, int32_t dtype, int64_t width, const char* name, std::vector<const es_tensor*>& list) {
+  int grid(const es_tensor& t, int32_t dtype, int64_t width, const char* name, Tensors& list) {
     if (!check(t, dtype, 2, name) || !addressable(t, name)) return ES_ERR_ARGUMENT;
     if (t.size[0] != rows || t.size[1] != width) return fail(ES_ERR_ARGUMENT, std::string(name) + " shape mismatch");
-    list.push_back(&t);
+    list.add(t);
     return ES_SUCCESS;
   }
   // A gradient: apart from every other tensor, or the logits tensor itself.
@@ -96,16 +103,17 @@ struct Call {
     if (reinterpret_cast<uintptr_t>(g.data) % element_size(g.dtype) != 0)
       return fail(ES_ERR_ALIGNMENT, "grad must be aligned to its elements");
     if (g.data == l.data && g.stride[0] == l.stride[0] && g.stride[1] == l.stride[1])
-      inputs.erase(std::find(inputs.begin(), inputs.end(), &l));
+      in_place = true;
     return ES_SUCCESS;
   }
   int finish() const {
-    for (size_t i = 0; i < outputs.size(); ++i) {
-      if (!no_internal_overlap(*outputs[i])) return fail(ES_ERR_ALIAS, "output has overlapping strides");
+    for (const es_tensor* const& out : outputs) {
+      if (!no_internal_overlap(*out)) return fail(ES_ERR_ALIAS, "output has overlapping strides");
       for (const es_tensor* t : inputs)
-        if (!disjoint(*outputs[i], *t)) return fail(ES_ERR_ALIAS, "exactsample input/output aliasing is forbidden");
-      for (size_t j = 0; j < i; ++j)
-        if (!disjoint(*outputs[i], *outputs[j])) return fail(ES_ERR_ALIAS, "exactsample outputs alias");
+        if (!(in_place && t == &in.logits) && !disjoint(*out, *t))
+          return fail(ES_ERR_ALIAS, "exactsample input/output aliasing is forbidden");
+      for (const es_tensor* const* other = outputs.begin(); other != &out; ++other)
+        if (!disjoint(*out, **other)) return fail(ES_ERR_ALIAS, "exactsample outputs alias");
     }
     return ES_SUCCESS;
   }
@@ -123,14 +131,14 @@ constexpr size_t MAX_SMEM = 227 * 1024;
 // Ranks of a row's cluster: slices of about SLICE_BYTES, the fewest ranks
 // that allow them, at most 16. The rule sees only the vocabulary and the type, so that a
 // row's results do not depend on the batch.
-int split(Rows& r, const es_rows& in, size_t slice_bytes, size_t (*smem)(int, int32_t, int), int k, size_t* bytes) {
+int split(Rows& r, const es_rows& in, size_t slice_bytes, size_t (*smem)(int, int32_t, bool, int), int k, size_t* bytes) {
   const int64_t vocab = in.logits.size[1];
   const int64_t steps = (vocab + SLICE_STEP - 1) / SLICE_STEP;
   const int64_t row_bytes = vocab * int64_t(element_size(in.logits.dtype));
   const int64_t want = std::clamp<int64_t>((row_bytes + int64_t(slice_bytes) - 1) / int64_t(slice_bytes), 1, MAX_RANKS);
   const int64_t slice = (steps + want - 1) / want * SLICE_STEP;
   if (slice > int64_t(MAX_SMEM)) return fail(ES_ERR_UNSUPPORTED, "vocabulary too large for one 16-block cluster's shared memory");
-  *bytes = smem(int(slice), in.logits.dtype, k);
+  *bytes = smem(int(slice), in.logits.dtype, present(in.mask), k);
   if (*bytes > MAX_SMEM) return fail(ES_ERR_UNSUPPORTED, "vocabulary too large for one 16-block cluster's shared memory");
   r.logits = in.logits.data;
   r.l_s0 = in.logits.stride[0];
@@ -146,8 +154,8 @@ int split(Rows& r, const es_rows& in, size_t slice_bytes, size_t (*smem)(int, in
   return ES_SUCCESS;
 }
 
-size_t loss_bytes(int slice, int32_t dtype, int k) {
-  return dtype == ES_F32 ? loss_smem<ES_F32>(slice, k) : loss_smem<ES_F16>(slice, k);
+size_t loss_bytes(int slice, int32_t dtype, bool mask, int k) {
+  return dtype == ES_F32 ? loss_smem<ES_F32>(slice, mask, k) : loss_smem<ES_F16>(slice, mask, k);
 }
 #ifndef LOSS_KB
 #define LOSS_KB 33
@@ -262,10 +270,11 @@ int distill_loss(const es_distill_args* a, cudaStream_t stream) {
   return run_loss(call, p, a->grad, DISTILL, stream);
 }
 
-size_t top_bytes(int slice, int32_t dtype, int) {
-  return dtype == ES_F32 ? top_smem<ES_F32>(slice) : top_smem<ES_F16>(slice);
-}
-constexpr size_t TOP_SLICE_BYTES = 38 * 1024;
+size_t top_bytes(int, int32_t, bool, int) { return sizeof(TopShared); }
+#ifndef TOP_KB
+#define TOP_KB 76
+#endif
+constexpr size_t TOP_SLICE_BYTES = TOP_KB * 1024;
 
 int top_logits(const es_top_args* a, cudaStream_t stream) {
   Call call{a->in};

@@ -13,6 +13,8 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
+#include <array>
+
 #include "exactsample_b200.h"
 
 namespace {
@@ -116,7 +118,7 @@ struct RowCall {
 
   es_tensor use(const Tensor& t, const char* name) const {
     TORCH_CHECK(t.device() == logits.device(), name, " has wrong device, dtype or rank");
-    if (!capturing) c10::cuda::CUDACachingAllocator::recordStream(t.storage().data_ptr(), stream);
+    if (!capturing) c10::cuda::CUDACachingAllocator::recordStream(t.unsafeGetTensorImpl()->unsafe_storage().data_ptr(), stream);
     return describe(t);
   }
   es_tensor use(const OptionalTensor& t, const char* name) const {
@@ -135,8 +137,20 @@ struct RowCall {
     r.temperature_all = temperature_all;
     return r;
   }
-  Tensor floats() const { return at::empty({logits.size(0)}, logits.options().dtype(at::kFloat)); }
-  Tensor statuses() const { return at::empty({logits.size(0)}, logits.options().dtype(at::kInt)); }
+  // The call's per-row outputs, `floats` of float32 and the statuses last, side
+  // by side in one allocation (each starts on 16 bytes).
+  std::array<Tensor, 5> columns(int floats) const {
+    const int64_t rows = logits.size(0), width = (rows + 3) / 4 * 4;
+    const Tensor all = at::empty({width * (floats + 1)}, logits.options().dtype(at::kFloat));
+    std::array<Tensor, 5> out;
+    for (int i = 0; i <= floats; ++i) {
+      const auto type = i < floats ? caffe2::TypeMeta::Make<float>() : caffe2::TypeMeta::Make<int32_t>();
+      out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), type);
+      out[i].unsafeGetTensorImpl()->set_storage_offset(width * i);
+      out[i].unsafeGetTensorImpl()->set_sizes_contiguous({rows});
+    }
+    return out;
+  }
   static void done(int result) { TORCH_CHECK(result == ES_SUCCESS, es_last_error()); }
 };
 
@@ -146,7 +160,7 @@ std::tuple<Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Te
                                                   const OptionalTensor& grad_logprobs,
                                                   const OptionalTensor& grad_entropy) {
   const RowCall call(logits);
-  Tensor logprobs = call.floats(), entropy = call.floats(), status = call.statuses();
+  auto [logprobs, entropy, status, _3, _4] = call.columns(2);
   es_logprob_args a{};
   a.in = call.rows(temperature, temperature_all, mask);
   a.tokens = call.use(tokens, "tokens");
@@ -157,7 +171,7 @@ std::tuple<Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Te
   a.grad_logprobs = call.use(grad_logprobs, "grad_logprobs");
   a.grad_entropy = call.use(grad_entropy, "grad_entropy");
   call.done(es_token_logprobs(&a, call.stream.stream()));
-  return {logprobs, entropy, status};
+  return {std::move(logprobs), std::move(entropy), std::move(status)};
 }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> top_logits(const Tensor& logits, int64_t k, const OptionalTensor& temperature,
@@ -166,7 +180,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> top_logits(const Tensor& logits, int6
   TORCH_CHECK(k >= 1 && k <= ES_MAX_TOP, "k must be in [1, 256]");
   Tensor values = at::empty({logits.size(0), k}, logits.options().dtype(at::kFloat));
   Tensor ids = at::empty({logits.size(0), k}, logits.options().dtype(at::kLong));
-  Tensor rest = call.floats(), status = call.statuses();
+  auto [rest, status, _2, _3, _4] = call.columns(1);
   es_top_args a{};
   a.in = call.rows(temperature, temperature_all, mask);
   a.values = describe(values);
@@ -183,8 +197,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> policy_loss(
     double temperature_all, const OptionalTensor& mask, double clip_low, double clip_high, double kl_coef,
     double entropy_coef, const OptionalTensor& grad) {
   const RowCall call(logits);
-  Tensor loss = call.floats(), logprobs = call.floats(), kl = call.floats(), entropy = call.floats();
-  Tensor status = call.statuses();
+  auto [loss, logprobs, kl, entropy, status] = call.columns(4);
   es_policy_args a{};
   a.in = call.rows(temperature, temperature_all, mask);
   a.tokens = call.use(tokens, "tokens");
@@ -211,7 +224,7 @@ std::tuple<Tensor, Tensor> distill_loss(const Tensor& logits, const Tensor& valu
                                         const OptionalTensor& temperature, double temperature_all,
                                         const OptionalTensor& mask, const OptionalTensor& grad) {
   const RowCall call(logits);
-  Tensor loss = call.floats(), status = call.statuses();
+  auto [loss, status, _2, _3, _4] = call.columns(1);
   es_distill_args a{};
   a.in = call.rows(temperature, temperature_all, mask);
   a.values = call.use(values, "values");

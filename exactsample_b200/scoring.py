@@ -69,15 +69,17 @@ class DistillLoss:
     status: Any  # int32 [rows]
 
 
-_ops = None
+class _Operators:
+    """The torch ops, loaded when one is first asked for."""
 
-
-def _operators():
-    global _ops
-    if _ops is None:
+    def __getattr__(self, name):
         load_library()
-        _ops = torch.ops.exactsample
-    return _ops
+        op = getattr(torch.ops.exactsample, name).default
+        setattr(self, name, op)
+        return op
+
+
+_ops = _Operators()
 
 
 def _temperature(value):
@@ -107,7 +109,7 @@ class _TokenLogprobs(torch.autograd.Function):
         ctx.save_for_backward(logits, tokens, temperature, mask)
         ctx.temperature_all = temperature_all
         ctx.set_materialize_grads(False)
-        out = _operators().token_logprobs(logits, tokens, temperature, temperature_all, mask, None, None, None)
+        out = _ops.token_logprobs(logits, tokens, temperature, temperature_all, mask, None, None, None)
         ctx.mark_non_differentiable(out[2])
         return out
 
@@ -118,7 +120,7 @@ class _TokenLogprobs(torch.autograd.Function):
             return None, None, None, None, None
         logits, tokens, temperature, mask = ctx.saved_tensors
         grad = torch.empty_like(logits)
-        _operators().token_logprobs(logits, tokens, temperature, ctx.temperature_all, mask, grad, grad_logprobs,
+        _ops.token_logprobs(logits, tokens, temperature, ctx.temperature_all, mask, grad, grad_logprobs,
                                     grad_entropy)
         return grad, None, None, None, None
 
@@ -137,7 +139,7 @@ def token_logprobs(logits, tokens, *, temperature=1.0, mask=None, grad=None, gra
     per_row, everywhere = _temperature(temperature)
     if _tracked(logits, grad, per_row, grad_logprobs, grad_entropy):
         return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, per_row, everywhere, mask))
-    return TokenLogprobs(*_operators().token_logprobs(logits, tokens, per_row, everywhere, mask, grad, grad_logprobs,
+    return TokenLogprobs(*_ops.token_logprobs(logits, tokens, per_row, everywhere, mask, grad, grad_logprobs,
                                                       grad_entropy))
 
 
@@ -150,7 +152,7 @@ def top_logits(logits, k: int, *, temperature=1.0, mask=None) -> TopLogits:
     for autograd: it is a teacher's or a server's pass.
     """
     per_row, everywhere = _temperature(temperature)
-    return TopLogits(*_operators().top_logits(logits.detach() if logits.requires_grad else logits, k, per_row,
+    return TopLogits(*_ops.top_logits(logits.detach() if logits.requires_grad else logits, k, per_row,
                                               everywhere, mask))
 
 
@@ -159,7 +161,7 @@ class _PolicyLoss(torch.autograd.Function):
     def forward(ctx, logits, tokens, old, advantages, ref, weights, temperature, temperature_all, mask, coefficients):
         ctx.save_for_backward(logits, tokens, old, advantages, ref, weights, temperature, mask)
         ctx.temperature_all, ctx.coefficients = temperature_all, coefficients
-        out = _operators().policy_loss(logits, tokens, old, advantages, ref, weights, temperature, temperature_all,
+        out = _ops.policy_loss(logits, tokens, old, advantages, ref, weights, temperature, temperature_all,
                                        mask, *coefficients, None)
         ctx.mark_non_differentiable(*out[1:])
         return out
@@ -169,7 +171,7 @@ class _PolicyLoss(torch.autograd.Function):
     def backward(ctx, grad_loss, *_):
         logits, tokens, old, advantages, ref, weights, temperature, mask = ctx.saved_tensors
         grad = torch.empty_like(logits)
-        _operators().policy_loss(logits, tokens, old, advantages, ref,
+        _ops.policy_loss(logits, tokens, old, advantages, ref,
                                  grad_loss if weights is None else weights * grad_loss, temperature,
                                  ctx.temperature_all, mask, *ctx.coefficients, grad)
         return (grad,) + (None,) * 9
@@ -192,7 +194,7 @@ def policy_loss(logits, tokens, old_logprobs, advantages, *, ref_logprobs=None, 
     if _tracked(logits, grad, old_logprobs, advantages, ref_logprobs, weights, per_row):
         return PolicyLoss(*_PolicyLoss.apply(logits, tokens, old_logprobs, advantages, ref_logprobs, weights, per_row,
                                              everywhere, mask, coefficients))
-    return PolicyLoss(*_operators().policy_loss(logits, tokens, old_logprobs, advantages, ref_logprobs, weights,
+    return PolicyLoss(*_ops.policy_loss(logits, tokens, old_logprobs, advantages, ref_logprobs, weights,
                                                 per_row, everywhere, mask, *coefficients, grad))
 
 
@@ -201,7 +203,7 @@ class _DistillLoss(torch.autograd.Function):
     def forward(ctx, logits, values, ids, rest, weights, temperature, temperature_all, mask):
         ctx.save_for_backward(logits, values, ids, rest, weights, temperature, mask)
         ctx.temperature_all = temperature_all
-        out = _operators().distill_loss(logits, values, ids, rest, weights, temperature, temperature_all, mask, None)
+        out = _ops.distill_loss(logits, values, ids, rest, weights, temperature, temperature_all, mask, None)
         ctx.mark_non_differentiable(out[1])
         return out
 
@@ -210,7 +212,7 @@ class _DistillLoss(torch.autograd.Function):
     def backward(ctx, grad_loss, _):
         logits, values, ids, rest, weights, temperature, mask = ctx.saved_tensors
         grad = torch.empty_like(logits)
-        _operators().distill_loss(logits, values, ids, rest, grad_loss if weights is None else weights * grad_loss,
+        _ops.distill_loss(logits, values, ids, rest, grad_loss if weights is None else weights * grad_loss,
                                   temperature, ctx.temperature_all, mask, grad)
         return (grad,) + (None,) * 7
 
@@ -235,5 +237,5 @@ def distill_loss(logits, teacher: TopLogits, *, weights=None, temperature=1.0, m
     if _tracked(logits, grad, teacher.values, rest, weights, per_row):
         return DistillLoss(*_DistillLoss.apply(logits, teacher.values, teacher.ids, rest, weights, per_row, everywhere,
                                                mask))
-    return DistillLoss(*_operators().distill_loss(logits, teacher.values, teacher.ids, rest, weights, per_row,
+    return DistillLoss(*_ops.distill_loss(logits, teacher.values, teacher.ids, rest, weights, per_row,
                                                   everywhere, mask, grad))
