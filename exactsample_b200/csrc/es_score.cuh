@@ -23,7 +23,7 @@
 #define ES_SCORE_THREADS 128
 #endif
 #ifndef ES_SCORE_BLOCKS
-#define ES_SCORE_BLOCKS 6
+#define ES_SCORE_BLOCKS 5
 #endif
 
 namespace es {
@@ -52,15 +52,36 @@ template <class T> struct Grid2 {  // a strided 2-D tensor
   int64_t s0, s1;
 };
 
+// 1 / temperature in two floats, and log2(e) / temperature.
+struct Scale {
+  float log2;      // of the exponents
+  float hi, lo;    // 1 / temperature
+  bool bad;        // not positive and finite, or beyond float32's range
+};
+__host__ __device__ inline Scale scale_of(double temperature) {
+  const double inv = 1. / temperature;
+  Scale s;
+  s.log2 = float(LOG2E * inv);
+  s.bad = !(s.log2 >= 1.17549435e-38f && s.log2 <= 3.402823466e38f);
+  s.hi = float(inv);
+  s.lo = float(inv - double(s.hi));
+  if (s.bad) s = {float(LOG2E), 1.f, 0.f, true};
+  return s;
+}
+
 struct Rows {
   const void* logits;
   int64_t l_s0, l_s1;
   Grid2<const int32_t> mask;
   Column<const double> temperature;
-  double inv_all;  // 1 / temperature where it is one number
+  Scale all;  // where the temperature is one number
   int64_t rows;
   int32_t vocab, ranks, slice;
 };
+
+__device__ __forceinline__ Scale row_scale(const Rows& in, int64_t row) {
+  return in.temperature.p ? scale_of(in.temperature[row]) : in.all;
+}
 
 struct LossParams {
   Rows in;
@@ -360,6 +381,9 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
 __device__ __forceinline__ void copy_async(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
 }
+__device__ __forceinline__ void copy_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int GROUPS> __device__ __forceinline__ void copies_done() {  // all but the last GROUPS groups
   asm volatile("cp.async.wait_group %0;" ::"n"(GROUPS) : "memory");
@@ -367,27 +391,9 @@ template <int GROUPS> __device__ __forceinline__ void copies_done() {  // all bu
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------
-// 1 / temperature in two floats, and log2(e) / temperature.
-struct Scale {
-  float log2;      // of the exponents
-  float hi, lo;    // 1 / temperature
-  bool bad;        // not positive and finite, or beyond float32's range
-};
-__device__ __forceinline__ Scale row_scale(const Rows& in, int64_t row) {
-  const double inv = in.temperature.p ? 1. / in.temperature[row] : in.inv_all;
-  Scale s;
-  s.log2 = float(LOG2E * inv);
-  s.bad = !(s.log2 >= 1.17549435e-38f && s.log2 <= 3.402823466e38f);
-  s.hi = float(inv);
-  s.lo = float(inv - double(s.hi));
-  if (s.bad) s = {float(LOG2E), 1.f, 0.f, true};
-  return s;
-}
-
 // ---------------------------------------------------------------------------
-// 16 bytes at `shift` bytes past p, from two aligned pieces.
-template <int SIZE> __device__ __forceinline__ uint4 shifted_chunk(const uint4* p, uint32_t shift) {
-  const uint4 a = p[0], b = p[1];
+// 16 bytes at `shift` bytes into the 32 of two pieces; shift below 16.
+template <int SIZE> __device__ __forceinline__ uint4 shifted_chunk(const uint4& a, const uint4& b, uint32_t shift) {
   uint32_t w[7] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z};
   if (shift & 8) {
 #pragma unroll
@@ -404,20 +410,37 @@ template <int SIZE> __device__ __forceinline__ uint4 shifted_chunk(const uint4* 
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
+// Chunk c of n elements that start anywhere and lie `stride` apart, -inf past
+// the end. Inside, a chunk that does not start on 16 bytes is cut out of the
+// two aligned pieces that it lies in.
+template <int DT>
+__device__ __forceinline__ uint4 fetch_chunk(const typename Elem<DT>::T* src, int64_t stride, int c, int n) {
+  using T = typename Elem<DT>::T;
+  constexpr int N = Elem<DT>::N;
+  const uint32_t shift = uint32_t(reinterpret_cast<uintptr_t>(src)) & 15;
+  if (stride == 1 && c > 0 && (c + 2) * N <= n) {
+    const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(src) - shift) + c;
+    const uint4 a = from[0], b = from[shift ? 1 : 0];
+    return shifted_chunk<sizeof(T)>(a, b, shift);
+  }
+  uint4 q;
+  T* v = reinterpret_cast<T*>(&q);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = c * N + i < n ? src[(c * N + i) * stride] : Elem<DT>::put(-INFINITY);
+  return q;
+}
 
 // A rank's slice of the row in shared memory, element i at base + i sizeof(T).
-// Chunk c is copied, read and written by thread c mod THREADS alone, so that
-// an aligned row needs no barrier between its copy and its sums. Of a row
-// that does not start on 16 bytes the aligned middle is copied and only the
-// ragged ends come by plain loads; it lands as far off 16 bytes and is then
-// moved into place. Rows without unit stride are gathered.
+// Chunk c is brought, read and written by thread c mod THREADS alone, so that
+// its way needs no barrier. Rows that start on 16 bytes come by asynchronous
+// copies of whole chunks, rows that start on 4 by copies of words (4 a chunk:
+// 33 us more for 1,001 rows of 50,257 float32, where a move through registers
+// costs 150), others through registers.
 template <int DT> struct Slice {
   using T = typename Elem<DT>::T;
   static constexpr int N = Elem<DT>::N;
   uint8_t* base;
-  uint32_t shift;
   int n, chunks, half;  // half: chunks of the first of two groups of copies, all of them whole
-  bool shared;          // chunks come from other threads' copies
 
   __device__ __forceinline__ T& operator[](int i) const { return reinterpret_cast<T*>(base)[i]; }
   __device__ __forceinline__ uint4& chunk(int c) const { return reinterpret_cast<uint4*>(base)[c]; }
@@ -432,72 +455,55 @@ template <int DT> struct Slice {
   static __device__ __forceinline__ const T* source(const Rows& in, int64_t row, int begin) {
     return static_cast<const T*>(in.logits) + row * in.l_s0 + int64_t(begin) * in.l_s1;
   }
-  // Whether a thread may copy its own chunks of the row, each as soon as it
-  // has done with what lies in its place.
-  static __device__ __forceinline__ bool aligned(const Rows& in, const T* src) {
-    return in.l_s1 == 1 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+  // How a row comes: 16 or 4 bytes a copy, or 0 for none.
+  static __device__ __forceinline__ int width(const Rows& in, const T* src) {
+    const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(src)) & 15;
+    return in.l_s1 != 1 ? 0 : off == 0 ? 16 : off % 4 == 0 ? 4 : 0;
+  }
+  // Chunk c of a row that has a width; a whole one.
+  __device__ __forceinline__ void copy(int c, const T* src, int width) const {
+    if (width == 16) {
+      copy_async(&chunk(c), reinterpret_cast<const uint4*>(src) + c);
+    } else {
+      const uint32_t* from = reinterpret_cast<const uint32_t*>(src) + 4 * c;
+      uint32_t* to = reinterpret_cast<uint32_t*>(&chunk(c));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) copy_async4(to + i, from + i);
+    }
   }
   // The last chunk where it is not whole, by the thread that owns it.
-  __device__ __forceinline__ void load_ragged(const T* src) const {
+  __device__ __forceinline__ void load_ragged(const T* src, int64_t stride) const {
     const int whole = n / N;
-    if (whole < chunks && int(threadIdx.x) == whole % THREADS)
-      for (int i = 0; i < N; ++i) (*this)[whole * N + i] = whole * N + i < n ? src[whole * N + i] : Elem<DT>::put(-INFINITY);
+    if (whole < chunks && int(threadIdx.x) == whole % THREADS) chunk(whole) = fetch_chunk<DT>(src, stride, whole, n);
   }
-  __device__ __forceinline__ void load(const Rows& in, int64_t row, int begin) {
+  __device__ __forceinline__ void load(const Rows& in, int64_t row, int begin) const {
     const T* src = source(in, row, begin);
-    const int tid = threadIdx.x;
-    shared = !aligned(in, src);
-    shift = in.l_s1 == 1 ? uint32_t(reinterpret_cast<uintptr_t>(src)) & 15 : 0u;
-    if (!shared) {
-      const uint4* from = reinterpret_cast<const uint4*>(src);
-      const int whole = n / N;
-      int c = tid;
-      for (; c < half; c += THREADS) copy_async(&chunk(c), from + c);
+    const int tid = threadIdx.x, whole = n / N, bytes = width(in, src);
+    int c = tid;
+    if (bytes) {
+      for (; c < half; c += THREADS) copy(c, src, bytes);
       copies_end_group();
-      for (; c < whole; c += THREADS) copy_async(&chunk(c), from + c);
+      for (; c < whole; c += THREADS) copy(c, src, bytes);
       copies_end_group();
-      load_ragged(src);
+      load_ragged(src, 1);
       return;
     }
-    __syncthreads();  // other threads have done with their chunks of the row before
-    if (in.l_s1 == 1) {
-      const int head = min(int((16 - shift) / sizeof(T)), n), middle = (n - head) / N;
-      T* landed = reinterpret_cast<T*>(base + shift);
-      const uint4* from = reinterpret_cast<const uint4*>(src + head);
-      uint4* to = reinterpret_cast<uint4*>(landed + head);
-      for (int c = tid; c < middle; c += THREADS) copy_async(to + c, from + c);
-      const int tail = head + middle * N + tid - 32;
-      if (tid < head) landed[tid] = src[tid];
-      if (tid >= 32 && tail < n) landed[tail] = src[tail];
-    } else {
-      for (int i = tid; i < n; i += THREADS) (*this)[i] = src[i * in.l_s1];
-    }
+    copies_end_group();  // (mask words)
     copies_end_group();
-    if (tid < chunks * N - n)  // the last chunk's unused places
-      reinterpret_cast<T*>(base + shift)[n + tid] = Elem<DT>::put(-INFINITY);
-  }
-  // All threads: after this a thread may read its chunks below `half`, if the
-  // slice is not `shared`, or all of them.
-  __device__ __forceinline__ void arrive() const {
-    if (!shared) {
-      copies_done<1>();
-      return;
-    }
-    copies_done<0>();
-    __syncthreads();
-    if (shift) {
-      // Chunks move down by less than one chunk, THREADS at a time: a round
-      // reads only what no earlier round wrote.
-      for (int first = 0; first < chunks; first += THREADS) {
-        const int c = first + int(threadIdx.x);
-        uint4 q;
-        if (c < chunks) q = shifted_chunk<sizeof(T)>(&chunk(c), shift);
-        __syncthreads();
-        if (c < chunks) chunk(c) = q;
-      }
+#pragma unroll 1
+    for (; c < chunks; c += 4 * THREADS) {
+      uint4 q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i * THREADS < chunks) q[i] = fetch_chunk<DT>(src, in.l_s1, c + i * THREADS, n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i * THREADS < chunks) chunk(c + i * THREADS) = q[i];
     }
   }
-  // And after this all of its chunks.
+  // After this a thread may read its chunks below `half`, and after
+  // arrive_rest all of them.
+  __device__ __forceinline__ void arrive() const { copies_done<1>(); }
   __device__ __forceinline__ void arrive_rest() const { copies_done<0>(); }
 };
 
@@ -707,9 +713,8 @@ struct Kept {
 };
 
 constexpr size_t SHARED_BYTES = (sizeof(Shared) + 15) / 16 * 16;
-// The buffer of a slice and what a shifted one reaches beyond it.
 template <int DT> __host__ __device__ constexpr size_t slice_bytes(int slice) {
-  return size_t(slice) * sizeof(typename Elem<DT>::T) + 32;
+  return size_t(slice) * sizeof(typename Elem<DT>::T);
 }
 // Then two rows' mask words, and the distillation's entries.
 __host__ __device__ constexpr size_t mask_bytes(int slice) { return size_t(slice) / 8; }
@@ -985,60 +990,97 @@ template <int DT, int OP, bool GRAD> struct LossRow {
   __device__ __forceinline__ void write_grad(const Slice<DT>& slice, const uint32_t* words, const RowScalars& scalars, float scale,
                                              int token, const T* next) const {
     const RowScalars r = scalars;
-    const bool own = OP != DISTILL && token >= 0 && token / N % THREADS == tid;  // this thread writes the token's chunk
-    if (grad_vector()) {
-      uint4* out = reinterpret_cast<uint4*>(grad_at(begin));
-      const uint4* from = reinterpret_cast<const uint4*>(next);
-      const int whole = n / N;
-      int c = tid;
+    if (grad_vector() && (next == nullptr || Slice<DT>::width(p.in, next) == 16)) write_aligned<FORM>(slice, words, r, scale, token, next);
+    else write_anywhere<FORM>(slice, words, r, scale, token, next);
+  }
+  template <int FORM>
+  __device__ __forceinline__ void write_aligned(const Slice<DT>& slice, const uint32_t* words, const RowScalars& r, float scale,
+                                                int token, const T* next) const {
+    uint4* out = reinterpret_cast<uint4*>(grad_at(begin));
+    const uint4* from = reinterpret_cast<const uint4*>(next);
+    const int whole = n / N;
+    int c = tid;
 #pragma unroll 1
-      for (int part = 0; part < 2; ++part) {
-        const int end = part ? whole : slice.half;
+    for (int part = 0; part < 2; ++part) {
+      const int end = part ? whole : slice.half;
 #pragma unroll 1
-        for (; c + 3 * THREADS < end; c += STEP) {
-          uint4 q[4];
+      for (; c + 3 * THREADS < end; c += STEP) {
+        uint4 q[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) q[i] = slice.chunk(c + i * THREADS);
+        for (int i = 0; i < 4; ++i) q[i] = slice.chunk(c + i * THREADS);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) out[c + i * THREADS] = grad_chunk<FORM>(q[i], c + i * THREADS, words, r, scale);
-          if (next) {
+        for (int i = 0; i < 4; ++i) out[c + i * THREADS] = grad_chunk<FORM>(q[i], c + i * THREADS, words, r, scale);
+        if (next) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) copy_async(&slice.chunk(c + i * THREADS), from + c + i * THREADS);
-          }
+          for (int i = 0; i < 4; ++i) copy_async(&slice.chunk(c + i * THREADS), from + c + i * THREADS);
         }
-        if (part) {
-          for (; c < whole; c += THREADS) {
-            out[c] = grad_chunk<FORM>(slice.chunk(c), c, words, r, scale);
-            if (next) copy_async(&slice.chunk(c), from + c);
-          }
+      }
+      if (part) {
+        for (; c < whole; c += THREADS) {
+          out[c] = grad_chunk<FORM>(slice.chunk(c), c, words, r, scale);
+          if (next) copy_async(&slice.chunk(c), from + c);
         }
-        copies_end_group();
       }
-      if (c == whole && whole < slice.chunks) {
-        const uint4 q = grad_chunk<FORM>(slice.chunk(c), c, words, r, scale);
-        const T* v = reinterpret_cast<const T*>(&q);
-        for (int i = 0; i < n - c * N; ++i) *grad_at(begin + c * N + i) = v[i];
+      copies_end_group();
+    }
+    if (c == whole && whole < slice.chunks) store_elements(grad_chunk<FORM>(slice.chunk(c), c, words, r, scale), c, 0, N);
+    if (next) slice.load_ragged(next, 1);
+    // The thread that wrote the token's chunk.
+    if (OP != DISTILL && token >= 0 && token / N % THREADS == tid) *grad_at(begin + token) = E::put(r.token_grad);
+  }
+  // Elements [from, to) of chunk c's gradient.
+  __device__ __forceinline__ void store_elements(const uint4& q, int c, int from, int to) const {
+    const T* v = reinterpret_cast<const T*>(&q);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i >= from && i < to && c * N + i < n) *grad_at(begin + c * N + i) = v[i];
+  }
+  // Gradient rows or next rows that do not start on 16 bytes, or have a stride.
+  // A warp's 32 chunks go back to their places in the slice and from there out,
+  // neighbouring words or elements from neighbouring lanes.
+  template <int FORM>
+  __device__ __forceinline__ void write_anywhere(const Slice<DT>& slice, const uint32_t* words, const RowScalars& r, float scale,
+                                                 int token, const T* next) const {
+    const int bytes = next ? Slice<DT>::width(p.in, next) : 0, whole = n / N, lane = lane_id();
+    const bool vector = grad_vector();
+    // Elements to a store: the most that the row's start allows.
+    const int most = p.g_s1 == 1 && reinterpret_cast<uintptr_t>(grad_at(begin)) % 4 == 0 ? 4 / int(sizeof(T)) : 1;
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {
+      const int end = part ? slice.chunks : slice.half;
+#pragma unroll 1
+      for (int c = (part ? slice.half : 0) + tid; c - lane < end; c += THREADS) {
+        if (c < slice.chunks) {
+          uint4 g = grad_chunk<FORM>(slice.chunk(c), c, words, r, scale);
+          if (OP != DISTILL && token >= 0 && token / N == c) {
+            T* v = reinterpret_cast<T*>(&g);
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+              if (token % N == j) v[j] = E::put(r.token_grad);
+          }
+          if (vector && c < whole) *reinterpret_cast<uint4*>(grad_at(begin + c * N)) = g;
+          else slice.chunk(c) = g;
+        }
+        __syncwarp();
+        if (!vector || (c - lane + 32) > whole) {
+          const int from = (vector ? max(c - lane, whole) : c - lane) * N, to = min((c - lane + 32) * N, n);
+          if (most == 2) {
+#pragma unroll 4
+            for (int i = from + 2 * lane; i < to; i += 64) {
+              if (i + 1 < to) *reinterpret_cast<uint32_t*>(grad_at(begin + i)) = *reinterpret_cast<const uint32_t*>(&slice[i]);
+              else *grad_at(begin + i) = slice[i];
+            }
+          } else {
+#pragma unroll 4
+            for (int i = from + lane; i < to; i += 32) *grad_at(begin + i) = slice[i];
+          }
+          __syncwarp();
+        }
+        if (bytes && c < whole) slice.copy(c, next, bytes);
       }
-      if (next) slice.load_ragged(next);
-      if (own) *grad_at(begin + token) = E::put(r.token_grad);
-      return;
+      copies_end_group();
     }
-    // Gradient rows that do not start on 16 bytes, or have a stride: by way of
-    // shared memory, in 16-byte pieces from the first aligned address on.
-    for (int c = tid; c < slice.chunks; c += THREADS)
-      slice.chunk(c) = grad_chunk<FORM>(slice.chunk(c), c, words, r, scale);
-    if (own) slice[token] = E::put(r.token_grad);
-    __syncthreads();
-    int done = 0;
-    if (p.g_s1 == 1) {
-      const int head = min(int(uint32_t(16 - (reinterpret_cast<uintptr_t>(grad_at(begin)) & 15)) / sizeof(T)), n);
-      const int pieces = (n - head) / N;
-      uint4* out = reinterpret_cast<uint4*>(grad_at(begin + head));
-      for (int i = tid; i < pieces; i += THREADS) out[i] = shifted_chunk<sizeof(T)>(&slice.chunk(i), head * sizeof(T));
-      if (tid < head) *grad_at(begin + tid) = slice[tid];
-      done = head + pieces * N;
-    }
-    for (int i = done + tid; i < n; i += THREADS) *grad_at(begin + i) = slice[i];
+    if (bytes) slice.load_ragged(next, 1);
   }
   __device__ __forceinline__ void write_form(const Slice<DT>& slice, const uint32_t* words, const RowScalars& r, float scale,
                                              int token, const T* next) const {
@@ -1145,7 +1187,7 @@ template <int DT, int OP, bool GRAD> struct LossRow {
       float value_top = 0.f, x_top = 0.f;
       if (OP == DISTILL) kept_sums(sh, kept, scale, value_top, x_top);
       slice.arrive();
-      if (masked && OP != DISTILL && !slice.shared) __syncthreads();  // the mask words come from all threads' first copies
+      if (masked && OP != DISTILL) __syncthreads();  // the mask words come from all threads' first copies
       if (OP == DISTILL) {
         slice.arrive_rest();
         __syncthreads();
@@ -1166,12 +1208,8 @@ template <int DT, int OP, bool GRAD> struct LossRow {
       // with the row's memory, which may be the gradient's.)
       if (OP != DISTILL && tid == 0) bad |= isnan(E::get(in.raw));
       if (bad) rec.flags |= BAD;
-      // The next row, where its chunks may be copied one by one.
-      const T* next = nullptr;
-      if (row + stride < p.in.rows && next_token >= 0) {
-        next = Slice<DT>::source(p.in, row + stride, begin);
-        if (slice.shared || !Slice<DT>::aligned(p.in, next)) next = nullptr;
-      }
+      const T* next = row + stride < p.in.rows && next_token >= 0 ? Slice<DT>::source(p.in, row + stride, begin) : nullptr;
+      if (next && Slice<DT>::width(p.in, next) == 0) next = nullptr;
       rec = lanes_record<ENTROPY, 32>(rec, scale.log2);
       if (lane_id() == 0) sh.warps[turn & 1][warp_id()] = rec;
       if (!peers) cluster_wait();
@@ -1179,7 +1217,6 @@ template <int DT, int OP, bool GRAD> struct LossRow {
       __syncthreads();
       rec = join_records<ENTROPY, WARPS>(sh.warps[turn & 1], WARPS, scale.log2);
       if (tid < ranks) send_record(&sh.inbox[turn & 1][rank], &sh.bar[turn & 1], tid, rec);
-      if (GRAD && !grad_vector()) next = nullptr;
       loaded = next != nullptr;
       if (masked && loaded) load_mask(masks + (turn + 1 & 1) * (p.in.slice / 32), row + stride);  // in the first group
       if (!GRAD && loaded) slice.load(p.in, row + stride, begin);

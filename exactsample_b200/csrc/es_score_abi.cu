@@ -131,11 +131,11 @@ constexpr size_t MAX_SMEM = 227 * 1024;
 // Ranks of a row's cluster: slices of about SLICE_BYTES, the fewest ranks
 // that allow them, at most 16. The rule sees only the vocabulary and the type, so that a
 // row's results do not depend on the batch.
-int split(Rows& r, const es_rows& in, size_t slice_bytes, size_t (*smem)(int, int32_t, bool, int), int k, size_t* bytes) {
+int split(Rows& r, const es_rows& in, size_t slice_bytes, int64_t least, size_t (*smem)(int, int32_t, bool, int), int k, size_t* bytes) {
   const int64_t vocab = in.logits.size[1];
   const int64_t steps = (vocab + SLICE_STEP - 1) / SLICE_STEP;
   const int64_t row_bytes = vocab * int64_t(element_size(in.logits.dtype));
-  const int64_t want = std::clamp<int64_t>((row_bytes + int64_t(slice_bytes) - 1) / int64_t(slice_bytes), 1, MAX_RANKS);
+  const int64_t want = std::clamp<int64_t>(std::max((row_bytes + int64_t(slice_bytes) - 1) / int64_t(slice_bytes), least), 1, MAX_RANKS);
   const int64_t slice = (steps + want - 1) / want * SLICE_STEP;
   if (slice > int64_t(MAX_SMEM)) return fail(ES_ERR_UNSUPPORTED, "vocabulary too large for one 16-block cluster's shared memory");
   *bytes = smem(int(slice), in.logits.dtype, present(in.mask), k);
@@ -145,7 +145,7 @@ int split(Rows& r, const es_rows& in, size_t slice_bytes, size_t (*smem)(int, in
   r.l_s1 = in.logits.stride[1];
   r.mask = grid2<const int32_t>(in.mask);
   r.temperature = col<const double>(in.temperature);
-  r.inv_all = 1. / in.temperature_all;
+  r.all = scale_of(in.temperature_all);
   r.rows = in.logits.size[0];
   r.vocab = int32_t(vocab);
   r.slice = int32_t(slice);
@@ -158,7 +158,7 @@ size_t loss_bytes(int slice, int32_t dtype, bool mask, int k) {
   return dtype == ES_F32 ? loss_smem<ES_F32>(slice, mask, k) : loss_smem<ES_F16>(slice, mask, k);
 }
 #ifndef LOSS_KB
-#define LOSS_KB 33
+#define LOSS_KB 38
 #endif
 constexpr size_t LOSS_SLICE_BYTES = LOSS_KB * 1024;
 
@@ -171,7 +171,7 @@ int run_loss(Call& call, LossParams& p, const es_tensor& grad, int op, cudaStrea
   if (const int e = call.gradient(grad); e != ES_SUCCESS) return e;
   if (const int e = call.finish(); e != ES_SUCCESS) return e;
   size_t smem = 0;
-  if (const int e = split(p.in, call.in, LOSS_SLICE_BYTES, loss_bytes, p.k, &smem); e != ES_SUCCESS) return e;
+  if (const int e = split(p.in, call.in, LOSS_SLICE_BYTES, 1, loss_bytes, p.k, &smem); e != ES_SUCCESS) return e;
   if (call.rows == 0) return ES_SUCCESS;
   if (const int e = device_check(); e != ES_SUCCESS) return e;
   p.grad = present(grad) ? grad.data : nullptr;
@@ -270,11 +270,8 @@ int distill_loss(const es_distill_args* a, cudaStream_t stream) {
   return run_loss(call, p, a->grad, DISTILL, stream);
 }
 
-size_t top_bytes(int, int32_t, bool, int) { return sizeof(TopShared); }
-#ifndef TOP_KB
-#define TOP_KB 76
-#endif
-constexpr size_t TOP_SLICE_BYTES = TOP_KB * 1024;
+size_t top_bytes(int slice, int32_t, bool, int) { return top_smem(slice); }
+constexpr size_t TOP_SLICE_BYTES = 76 * 1024;
 
 int top_logits(const es_top_args* a, cudaStream_t stream) {
   Call call{a->in};
@@ -290,7 +287,7 @@ int top_logits(const es_top_args* a, cudaStream_t stream) {
   if (e != ES_SUCCESS) return e;
   TopParams p{};
   size_t smem = 0;
-  e = split(p.in, a->in, TOP_SLICE_BYTES, top_bytes, 0, &smem);
+  e = split(p.in, a->in, TOP_SLICE_BYTES, (k + 31) / 32, top_bytes, 0, &smem);
   if (e != ES_SUCCESS || call.rows == 0) return e;
   if (e = device_check(); e != ES_SUCCESS) return e;
   p.k = int32_t(k);

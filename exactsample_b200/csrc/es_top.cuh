@@ -3,16 +3,17 @@
 // that as many blocks as registers allow keep the memory busy.
 //
 // A row is split over a cluster; a thread goes through every THREADS-th chunk
-// of its rank's slice:
-//   1. each thread takes the maximum and the running sum of its tokens;
+// of its rank's slice, 32 tokens a step:
+//   1. each thread keeps the maximum and the sum of each of its steps;
 //   2. each rank finds the ceil(k / ranks)-th largest of its threads' maxima
-//      (to 18 bits of its key). At least that many of its tokens reach it, so
-//      the smallest of the ranks' values is a bound that at least k tokens of
-//      the row reach, and few more (a thread rarely holds two of the largest);
-//   3. the few threads whose maximum reaches the bound give up their sums.
-//      Their chunks are read again, from L2: tokens at or above the bound are
-//      listed, the others summed. So the rest is summed without the largest,
-//      and one far below them loses no digits to a subtraction;
+//      (to 12 bits of its key from the first in which they differ). At least
+//      that many of its tokens reach it, so the smallest of the ranks' values
+//      is a bound that at least k tokens of the row reach, and few more (a
+//      thread rarely holds two of the largest);
+//   3. the few steps whose maximum reaches the bound give up their sums.
+//      Their tokens are read again, from L2, one to a lane: those at or above
+//      the bound are listed, the others summed. So the rest is summed without
+//      the largest, and one far below them loses no digits to a subtraction;
 //   4. rank 0 has every rank's list, places each entry by the number of larger
 //      ones, and adds the entries past the k-th to the rest.
 // Entries are 64-bit words, the logit's order key above the complement of its
@@ -34,23 +35,23 @@ struct TopParams {
   Column<int32_t> status;
 };
 
-constexpr int TOP_THREADS = 256, TOP_WARPS = TOP_THREADS / 32;
+constexpr int TOP_THREADS = 128, TOP_WARPS = TOP_THREADS / 32;
 constexpr uint32_t KEY_NONE = 0x007fffffu;  // the key of -inf: not a token of the row
-constexpr int COLLECTED = 2048;             // entries rank 0 takes, an equal share from each rank
+constexpr int COLLECTED = 1024;             // entries rank 0 takes, an equal share from each rank
+constexpr int HOT = 128;                    // steps a warp looks at again
 static_assert(COLLECTED >= 2 * MAX_TOP, "a single rank's list holds k entries and more");
 
 struct TopShared {
-  Record inbox[MAX_RANKS], bounds[MAX_RANKS];
-  Record warps[TOP_WARPS];
+  Record inbox[MAX_RANKS * TOP_WARPS], bounds[MAX_RANKS];
   uint64_t bar[2];
   uint32_t keys[TOP_THREADS];
-  uint32_t hot[TOP_WARPS];   // a bit per thread
-  uint16_t owners[TOP_THREADS];
-  uint32_t listed, counts[MAX_RANKS];
+  uint16_t hot[TOP_WARPS][HOT];  // steps to look at again
+  uint32_t listed, entries;
   uint32_t digits[TOP_WARPS][8];
-  uint32_t place[COLLECTED];
   float beyond[COLLECTED];   // values past the k-th, by place
+  alignas(16) uint64_t places[COLLECTED];
   uint64_t collected[COLLECTED];
+  float2 steps[1];           // maximum and sum of each thread's steps, as many as a slice has
 };
 
 __device__ __forceinline__ uint64_t entry_of(uint32_t key, int id) { return (uint64_t(key) << 32) | (0xffffffffu - uint32_t(id)); }
@@ -81,6 +82,7 @@ template <int DT> struct TopRow {
   using E = Elem<DT>;
   using T = typename E::T;
   static constexpr int N = E::N;
+  static constexpr int CHUNKS = 32 / N;  // of a step
 
   const TopParams& p;
   int64_t row;
@@ -89,22 +91,10 @@ template <int DT> struct TopRow {
   __device__ __forceinline__ const T* source() const {
     return static_cast<const T*>(p.in.logits) + row * p.in.l_s0 + int64_t(begin) * p.in.l_s1;
   }
-  // Chunk c of the slice, -inf past its end and at masked tokens. ALIGNED: the
-  // slice starts on 16 bytes (c a whole chunk).
+  // Chunk c of the slice. ALIGNED: the slice starts on 16 bytes (c a whole chunk).
   template <bool ALIGNED> __device__ __forceinline__ uint4 chunk(const T* src, int c) const {
     if (ALIGNED) return __ldg(reinterpret_cast<const uint4*>(src) + c);
-    const uint32_t shift = uint32_t(reinterpret_cast<uintptr_t>(src)) & 15;
-    if (p.in.l_s1 == 1 && shift != 0 && c > 0 && (c + 2) * N <= n) {
-      // Cut out of the two aligned pieces it lies in, both inside the slice.
-      const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(src) - shift) + c;
-      const uint4 pieces[2] = {__ldg(from), __ldg(from + 1)};
-      return shifted_chunk<sizeof(T)>(pieces, shift);
-    }
-    uint4 q;
-    T* v = reinterpret_cast<T*>(&q);
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = c * N + i < n ? src[(c * N + i) * p.in.l_s1] : E::put(-INFINITY);
-    return q;
+    return fetch_chunk<DT>(src, p.in.l_s1, c, n);
   }
   // Sets masked tokens to -inf; looks at them first.
   __device__ __forceinline__ void apply_mask(const int32_t* mask, int c, uint4& q, bool& bad) const {
@@ -112,51 +102,65 @@ template <int DT> struct TopRow {
     q = mask_chunk<DT>(q, uint32_t(mask[(c * N >> 5) * p.in.mask.s1]) >> (c * N & 31), lowest_word<DT>());
   }
 
-  // Every thread's tokens: their maximum and sum.
-  template <bool ALIGNED> __device__ __forceinline__ Record sums(const T* src, const int32_t* mask, float scale, bool& bad) const {
-    const int chunks = (n + N - 1) / N, whole = ALIGNED ? n / N : chunks;
-    Acc a = acc_none();
-    int c = tid;
-#pragma unroll 1
-    for (; c + 3 * TOP_THREADS < whole; c += 4 * TOP_THREADS) {
-      uint4 q[4];
+  // The maximum and the sum of 32 tokens (-inf where there are none).
+  __device__ __forceinline__ float2 step_sum(const uint4* q, float scale) const {
+    float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) q[i] = chunk<ALIGNED>(src, c + i * TOP_THREADS);
+    for (int i = 0; i < CHUNKS; i += 2) top = fmaxf(top, chunk_max<DT>(q[i], q[i + 1]));
+    const float m = fmaxf(top, LOWEST), r = __fmul_rn(m, scale);
+    float2 v[16], s = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) unpack<DT>(q[i], v + i * N / 2);
+    if (fabsf(r) <= LARGE_R && scale >= SMALL_SCALE) {
+      // (r's rounding, at most 2^-24 of it, goes into the sum as a factor.)
+      const float rest = __fmaf_rn(m, scale, -r);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float2 d = fma2(v[i], both(scale), both(-r));
+        s = add2(s, make_float2(ex2(d.x), ex2(d.y)));
+      }
+      return {m, __fmul_rn(__fadd_rn(s.x, s.y), ex2(-rest))};
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      s = add2(s, make_float2(ex2(exponent(v[i].x, m, scale)), ex2(exponent(v[i].y, m, scale))));
+    return {m, __fadd_rn(s.x, s.y)};
+  }
+  // Every thread's steps; returns their maximum.
+  template <bool ALIGNED>
+  __device__ __forceinline__ float sums(TopShared& sh, const T* src, const int32_t* mask, int steps, float scale, bool& bad) const {
+    const int chunks = (n + N - 1) / N, whole = ALIGNED ? n / N : chunks;
+    const uint4 none = make_uint4(lowest_word<DT>(), lowest_word<DT>(), lowest_word<DT>(), lowest_word<DT>());
+    float high = -INFINITY;
+#pragma unroll 1
+    for (int step = 0; step < steps; ++step) {
+      uint4 q[CHUNKS];
+#pragma unroll
+      for (int i = 0; i < CHUNKS; ++i) {
+        const int c = (step * CHUNKS + i) * TOP_THREADS + tid;
+        q[i] = none;
+        if (c < whole) q[i] = chunk<ALIGNED>(src, c);
+        else if (c < chunks) q[i] = chunk<false>(src, c);
+      }
       if (mask) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) apply_mask(mask, c + i * TOP_THREADS, q[i], bad);
+        for (int i = 0; i < CHUNKS; ++i) {
+          const int c = (step * CHUNKS + i) * TOP_THREADS + tid;
+          if (c < chunks) apply_mask(mask, c, q[i], bad);
+        }
       }
-      const float top = fmaxf(chunk_max<DT>(q[0], q[1]), chunk_max<DT>(q[2], q[3]));
-      float2 v[2 * N];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) unpack<DT>(q[i], v + i * N / 2);
-      acc_fast<4 * N, false>(a, v, top, scale);
+      const float2 got = step_sum(q, scale);
+      sh.steps[step * TOP_THREADS + tid] = got;
+      bad |= !(got.y < INFINITY) || got.x == INFINITY;
+      high = fmaxf(high, got.y > 0.f ? got.x : -INFINITY);
     }
-#pragma unroll 1
-    for (; c < chunks; c += TOP_THREADS) {
-      uint4 q = c < whole ? chunk<ALIGNED>(src, c) : chunk<false>(src, c);
-      if (mask) apply_mask(mask, c, q, bad);
-      float2 v[N / 2];
-      unpack<DT>(q, v);
-      acc_fast<N, false>(a, v, chunk_max<DT>(q, q), scale);
-    }
-    const bool failed = acc_failed<false>(a) || scale < SMALL_SCALE;
-    if (failed) {
-      a = acc_none();
-      for (c = tid; c < chunks; c += TOP_THREADS) {
-        uint4 q = chunk<false>(src, c);
-        if (mask) apply_mask(mask, c, q, bad);
-        float2 v[N / 2];
-        unpack<DT>(q, v);
-        acc_careful<N, false>(a, v, max_of<N>(v), scale);
-      }
-    }
-    return acc_exact<false>(a, scale, failed);
+    return high;
   }
 
-  // A bound that at least `need` of the threads' keys reach, its low 14 bits
-  // zero: the keys' common leading bits, then one bit a step. Every warp finds
-  // it for itself. 0 if fewer threads than that have any token.
+  // A bound that at least `need` of the threads' keys reach: their common
+  // leading bits, then 12 more, one a step. Every warp finds it for itself (in
+  // a loop of a fixed length: see lanes_record). 0 if fewer threads than that
+  // have any token.
   __device__ __forceinline__ uint32_t thread_bound(const uint32_t* keys, int need) const {
     uint32_t key[TOP_WARPS], low = 0xffffffffu, high = 0;
 #pragma unroll
@@ -167,26 +171,23 @@ template <int DT> struct TopRow {
     }
     low = __reduce_min_sync(0xffffffffu, low);
     high = __reduce_max_sync(0xffffffffu, high);
-    if (need > TOP_THREADS) return 0;
     const int differ = 31 - __clz(int((low ^ high) | 1u));
-    uint32_t found = high & ~(differ == 31 ? 0xffffffffu : (2u << differ) - 1u);
-    for (int bit = differ; bit >= 14; --bit) {
-      const uint32_t least = found | (1u << bit);
-      int above = 0;
+    uint32_t found = differ == 31 ? 0u : high & ~((2u << differ) - 1u);
+    int shift = differ - 1;  // two bits a step: three candidates' counts side by side
 #pragma unroll
-      for (int i = 0; i < TOP_WARPS; ++i) above += key[i] >= least;
-      if (int(__reduce_add_sync(0xffffffffu, unsigned(above))) >= need) found = least;
+    for (int step = 0; step < 6; ++step, shift -= 2) {
+      const int at = max(shift, 0);
+      uint32_t above = 0;
+#pragma unroll
+      for (int i = 0; i < TOP_WARPS; ++i)
+        above += (key[i] >= (found | 1u << at)) + ((key[i] >= (found | 2u << at)) << 10) + ((key[i] >= (found | 3u << at)) << 20);
+      above = __reduce_add_sync(0xffffffffu, above);
+      const uint32_t digit = (int(above & 1023u) >= need) + (int(above >> 10 & 1023u) >= need) + (int(above >> 20) >= need);
+      if (shift >= 0) found |= digit << at;
     }
-    return found;
+    return need <= TOP_THREADS ? found : 0u;
   }
 
-  __device__ __forceinline__ Record block_record(TopShared& sh, Record rec, float scale) const {
-    rec = lanes_record<false, 32>(rec, scale);
-    __syncthreads();
-    if (lane_id() == 0) sh.warps[warp_id()] = rec;
-    __syncthreads();
-    return join_records<false, TOP_WARPS>(sh.warps, TOP_WARPS, scale);
-  }
   __device__ __forceinline__ void write(int64_t at, float value, int64_t id) const {
     p.values.p[row * p.values.s0 + at * p.values.s1] = value;
     p.ids.p[row * p.ids.s0 + at * p.ids.s1] = id;
@@ -244,7 +245,7 @@ template <int DT> struct TopRow {
     for (int j = tid; j < p.in.vocab; j += TOP_THREADS) {
       const uint64_t entry = entry_at(j);
       if (entry >= least) {
-        sh.collected[atomicAdd(&sh.listed, 1u)] = entry;
+        sh.places[atomicAdd(&sh.listed, 1u)] = entry;
       } else if (entry != 0) {
         const float v = key_value(uint32_t(entry >> 32)), m = fmaxf(rec.m, v);
         rec.s = __fadd_rn(__fmul_rn(ex2(exponent(rec.m, m, scale)), rec.s), ex2(exponent(v, m, scale)));
@@ -259,123 +260,153 @@ template <int DT> struct TopRow {
   __device__ __forceinline__ void run(TopShared& sh) {
     if (tid == 0) {
       mbar_init(&sh.bar[0], 1);
-      mbar_init(&sh.bar[1], ranks);
+      mbar_init(&sh.bar[1], ranks * TOP_WARPS);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       mbar_arrive_expect_tx(&sh.bar[0], uint32_t(ranks * sizeof(Record)));
-      sh.listed = 0;
+      sh.listed = sh.entries = 0;
     }
-    cluster_started();
+    if (rank == 0)
+      for (int i = tid; i < COLLECTED; i += TOP_THREADS) sh.collected[i] = 0;
+    if (rank == 0) cluster_arrive();  // (the cleared places too)
+    else cluster_started();
     const Scale temperature = row_scale(p.in, row);
     const float scale = temperature.log2;
     const T* src = source();
     const int32_t* mask = p.in.mask.p ? p.in.mask.p + row * p.in.mask.s0 + (begin >> 5) * p.in.mask.s1 : nullptr;
     bool bad = temperature.bad;
     const bool aligned = p.in.l_s1 == 1 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
-    Record own = aligned ? sums<true>(src, mask, scale, bad) : sums<false>(src, mask, scale, bad);
-    bad |= !(own.s < INFINITY) || own.m == INFINITY;
-    const uint32_t key = own.s > 0.f ? order_key(own.m) : 0u;
-    sh.keys[tid] = key;
+    const int steps = (n + 32 * TOP_THREADS - 1) / (32 * TOP_THREADS);
+    const float high = aligned ? sums<true>(sh, src, mask, steps, scale, bad) : sums<false>(sh, src, mask, steps, scale, bad);
+    sh.keys[tid] = high > -INFINITY ? order_key(high) : 0u;
     cluster_wait();  // every rank has started
     __syncthreads();
 
     const uint32_t found = max(thread_bound(sh.keys, (p.k + ranks - 1) / ranks), KEY_NONE + 1);
     if (tid < ranks) send_record(&sh.bounds[rank], &sh.bar[0], tid, Record{0.f, 0.f, 0.f, found});
     if (!wait_bar(&sh.bar[0], 0)) bad = true;
-    uint32_t bound = 0xffffffffu;
-    for (int r = 0; r < ranks; ++r) bound = min(bound, sh.bounds[r].flags);
+    uint32_t bound = sh.bounds[min(lane_id(), ranks - 1)].flags;
+    bound = __reduce_min_sync(0xffffffffu, bound);
 
-    // The threads whose maximum reaches the bound, in order (sums are to have
-    // one order too), and their chunks again.
-    const uint32_t hot = __ballot_sync(0xffffffffu, key >= bound);
-    if (lane_id() == 0) sh.hot[warp_id()] = hot;
-    __syncthreads();
-    int owners = 0;
-    for (int w = 0; w < TOP_WARPS; ++w) {
-      if (w == warp_id() && key >= bound) {
-        sh.owners[owners + __popc(hot & ((1u << lane_id()) - 1))] = uint16_t(tid);
-        own = {LOWEST, 0.f, 0.f, 0u};
-      }
-      owners += __popc(sh.hot[w]);
-    }
-    __syncthreads();
-    const int share = COLLECTED / ranks, chunks = (n + N - 1) / N, each = (chunks + TOP_THREADS - 1) / TOP_THREADS;
+    // The steps below the bound add up; the others' tokens are looked at again,
+    // a lane each.
+    const int share = COLLECTED / ranks;
     uint64_t* places = cg::this_cluster().map_shared_rank(sh.collected, 0) + rank * share;
-    Acc a = {own.m, 0.f, {own.s, 0.f}, {0.f, 0.f}};
-    for (int task = tid; task < owners * each; task += TOP_THREADS) {
-      const int c = sh.owners[task / each] + task % each * TOP_THREADS;
-      if (c >= chunks) continue;
-      uint4 q = aligned && (c + 1) * N <= n ? chunk<true>(src, c) : chunk<false>(src, c);
-      if (mask) apply_mask(mask, c, q, bad);
-      float2 v[N / 2];
-      unpack<DT>(q, v);
-      float* f = reinterpret_cast<float*>(v);
+    Record rec = {LOWEST, 0.f, 0.f, 0u};
+    bool full = false;
+    int count = 0;
+#pragma unroll 1
+    for (int step = 0; step < steps; ++step) {
+      const float2 got = sh.steps[step * TOP_THREADS + tid];
+      const bool some = got.y > 0.f, reaches = some && order_key(got.x) >= bound;
+      const uint32_t hot = __ballot_sync(0xffffffffu, reaches);
+      const int at = count + __popc(hot & ((1u << lane_id()) - 1));
+      if (reaches && at < HOT) sh.hot[warp_id()][at] = uint16_t(step * 32 + lane_id());
+      count += __popc(hot);
+      const float m = reaches || !some ? rec.m : fmaxf(rec.m, got.x);
+      rec.s = __fmul_rn(ex2(exponent(rec.m, m, scale)), rec.s);
+      if (some && !reaches) rec.s = __fadd_rn(rec.s, __fmul_rn(ex2(exponent(got.x, m, scale)), got.y));
+      rec.m = m;
+    }
+    if (count > HOT) full = true;  // (they would hardly fit their places either)
+    __syncwarp();
+#pragma unroll 1
+    for (int first = 0; first < min(count, HOT); first += 4) {
+      int token[4];
+      float v[4], m = rec.m;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (order_key(f[i]) >= bound) {
-          const uint32_t at = atomicAdd(&sh.listed, 1u);
-          if (int(at) < share) places[at] = entry_of(order_key(f[i]), begin + c * N + i);
-          f[i] = -INFINITY;
-        }
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t hot = first + i < count ? sh.hot[warp_id()][first + i] : 0u;
+        token[i] = (((hot >> 5) * CHUNKS + lane_id() / N) * TOP_THREADS + warp_id() * 32 + (hot & 31)) * N + lane_id() % N;
+        v[i] = -INFINITY;
+        if (first + i < count && token[i] < n) v[i] = E::get(src[token[i] * p.in.l_s1]);
       }
-      acc_careful<N, false>(a, v, max_of<N>(v), scale);
+      if (mask) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (v[i] > -INFINITY && !(uint32_t(mask[(token[i] >> 5) * p.in.mask.s1]) >> (token[i] & 31) & 1)) v[i] = -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (order_key(v[i]) >= bound) {
+          const uint32_t place = atomicAdd(&sh.listed, 1u);
+          if (int(place) < share) places[place] = entry_of(order_key(v[i]), begin + token[i]);
+          else full = true;
+          v[i] = -INFINITY;
+        }
+        m = fmaxf(m, v[i]);
+      }
+      rec.s = __fmul_rn(ex2(exponent(rec.m, m, scale)), rec.s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rec.s = __fadd_rn(rec.s, ex2(exponent(v[i], m, scale)));
+      rec.m = m;
     }
-    Record rec = acc_exact<false>(a, scale, true);
-    rec.flags = bad ? BAD : 0u;
-    rec = block_record(sh, rec, scale);
-    if (tid == 0) {
-      const uint32_t listed = sh.listed;
-      rec.flags |= int(listed) > share ? FULL : 0u;
-      cg::this_cluster().map_shared_rank(sh.inbox, 0)[rank] = rec;
-      cg::this_cluster().map_shared_rank(sh.counts, 0)[rank] = listed;
-      arrive_at(&sh.bar[1], 0);
-    }
+    rec.flags = (bad ? BAD : 0u) | (full ? FULL : 0u);
+    rec = lanes_record<false, 32>(rec, scale);
+    if (lane_id() == 0) cg::this_cluster().map_shared_rank(sh.inbox, 0)[rank * TOP_WARPS + warp_id()] = rec;
+    __syncwarp();
+    if (lane_id() == 0) arrive_at(&sh.bar[1], 0);
     if (rank != 0) return;
 
     const bool came = wait_cluster(&sh.bar[1]);
-    rec = join_records<false, MAX_RANKS>(sh.inbox, ranks, scale);
+    rec = {LOWEST, 0.f, 0.f, 0u};
+#pragma unroll
+    for (int i = 0; i < MAX_RANKS * TOP_WARPS / 32; ++i) {
+      const int at = i * 32 + lane_id();
+      if (i * 32 >= ranks * TOP_WARPS) break;
+      Record more = sh.inbox[min(at, ranks * TOP_WARPS - 1)];
+      if (at >= ranks * TOP_WARPS) more.s = 0.f, more.m = LOWEST;
+      const float m = fmaxf(rec.m, more.m);
+      rec.s = __fadd_rn(__fmul_rn(ex2(exponent(rec.m, m, scale)), rec.s), __fmul_rn(ex2(exponent(more.m, m, scale)), more.s));
+      rec.m = m;
+      rec.flags |= more.flags;
+    }
+    rec = lanes_record<false, 32>(rec, scale);
     bad = (rec.flags & BAD) || !came;
+    // The ranks' lists side by side.
+    uint64_t mine[COLLECTED / TOP_THREADS];
+    count = 0;
+#pragma unroll
+    for (int i = 0; i < COLLECTED / TOP_THREADS; ++i) {
+      mine[i] = sh.collected[i * TOP_THREADS + tid];
+      count += mine[i] != 0;
+    }
+    int upto = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int below = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane_id() >= o) upto += below;
+    }
+    __syncthreads();
+    int at = 0;
+    if (lane_id() == 31) at = int(atomicAdd(&sh.entries, uint32_t(upto)));
+    at = __shfl_sync(0xffffffffu, at, 31) + upto - count;
+#pragma unroll
+    for (int i = 0; i < COLLECTED / TOP_THREADS; ++i)
+      if (mine[i]) sh.places[at++] = mine[i];
+    __syncthreads();
+    int entries = int(sh.entries);
     Record more = {LOWEST, 0.f, 0.f, 0u};
-    int entries = 0;
-    if (!bad && (rec.flags & FULL)) {
+    if (bad) {
+      entries = 0;
+    } else if (rec.flags & FULL) {
       entries = exact_entries(sh, scale, more);
       rec = {LOWEST, 0.f, 0.f, 0u};
-    } else if (!bad) {
-      // The ranks' lists side by side.
-      uint64_t mine[COLLECTED / TOP_THREADS];
-#pragma unroll
-      for (int i = 0; i < COLLECTED / TOP_THREADS; ++i) {
-        const int at = i * TOP_THREADS + tid, r = at / share;
-        mine[i] = r < ranks && at % share < int(sh.counts[r]) ? sh.collected[at] : 0;
-      }
-      if (tid == 0) sh.listed = 0;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < COLLECTED / TOP_THREADS; ++i)
-        if (mine[i]) sh.collected[atomicAdd(&sh.listed, 1u)] = mine[i];
-      __syncthreads();
-      entries = int(sh.listed);
     }
-    // Places, several threads to an entry where there are few.
-    for (int i = tid; i < entries; i += TOP_THREADS) sh.place[i] = 0;
+    // Each entry's place: the larger ones, two at a time (0 is none).
+    if (tid == 0) sh.places[min(entries, COLLECTED - 1)] = entries < COLLECTED ? 0 : sh.places[COLLECTED - 1];
     __syncthreads();
-    const int parts = max(1, TOP_THREADS / max(entries, 1)), length = (entries + parts - 1) / parts;
-    for (int i = tid; i < entries * parts; i += TOP_THREADS) {
-      const int mine = i % entries, from = i / entries * length, to = min(from + length, entries);
-      const uint64_t entry = sh.collected[mine];
-      uint32_t larger = 0;
-#pragma unroll 4
-      for (int j = from; j < to; ++j) larger += sh.collected[j] > entry;
-      if (larger) atomicAdd(&sh.place[mine], larger);
-    }
-    __syncthreads();
+#pragma unroll 1
     for (int i = tid; i < entries; i += TOP_THREADS) {
-      const uint64_t entry = sh.collected[i];
-      const float value = key_value(uint32_t(entry >> 32));
-      if (int(sh.place[i]) < p.k) {
-        write(sh.place[i], value, int64_t(0xffffffffu - uint32_t(entry)));
-      } else {
-        sh.beyond[sh.place[i]] = value;
+      const uint64_t entry = sh.places[i];
+      int place = 0;
+#pragma unroll 4
+      for (int j = 0; j < entries; j += 2) {
+        const ulonglong2 pair = *reinterpret_cast<const ulonglong2*>(&sh.places[j]);
+        place += (pair.x > entry) + (pair.y > entry);
       }
+      const float value = key_value(uint32_t(entry >> 32));
+      if (place < p.k) write(place, value, int64_t(0xffffffffu - uint32_t(entry)));
+      else sh.beyond[place] = value;
     }
     for (int i = entries + tid; i < p.k; i += TOP_THREADS) write(i, -INFINITY, -1);
     __syncthreads();
@@ -384,18 +415,23 @@ template <int DT> struct TopRow {
       more.s = __fadd_rn(__fmul_rn(ex2(exponent(more.m, m, scale)), more.s), ex2(exponent(sh.beyond[i], m, scale)));
       more.m = m;
     }
-    more = block_record(sh, more, scale);
+    more = lanes_record<false, 32>(more, scale);
+    if (lane_id() == 0) sh.inbox[warp_id()] = more;
+    __syncthreads();
     if (tid == 0) {
-      const float m = fmaxf(more.m, rec.m);
-      const float s = __fadd_rn(__fmul_rn(more.s, ex2(exponent(more.m, m, scale))), __fmul_rn(rec.s, ex2(exponent(rec.m, m, scale))));
+      for (int w = 0; w < TOP_WARPS; ++w) {
+        const float m = fmaxf(rec.m, sh.inbox[w].m);
+        rec.s = __fadd_rn(__fmul_rn(ex2(exponent(rec.m, m, scale)), rec.s), __fmul_rn(ex2(exponent(sh.inbox[w].m, m, scale)), sh.inbox[w].s));
+        rec.m = m;
+      }
       const bool ok = !bad && entries > 0;
-      p.rest[row] = ok && s > 0 ? value_of(pair_sum(scaled_gap(m, 0.f, temperature), log_pair(s))) : -INFINITY;
+      p.rest[row] = ok && rec.s > 0 ? value_of(pair_sum(scaled_gap(rec.m, 0.f, temperature), log_pair(rec.s))) : -INFINITY;
       p.status[row] = bad ? ES_INVALID_INPUT : ok ? ES_OK : ES_NO_VALID_TOKEN;
     }
   }
 };
 
-template <int DT> __global__ void __launch_bounds__(TOP_THREADS, 4) top_rows(const __grid_constant__ TopParams p) {
+template <int DT> __global__ void __launch_bounds__(TOP_THREADS, 8) top_rows(const __grid_constant__ TopParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   const int ranks = p.in.ranks, rank = int(blockIdx.x % unsigned(ranks));
   const int begin = rank * p.in.slice, n = min(p.in.slice, p.in.vocab - begin);
@@ -403,9 +439,12 @@ template <int DT> __global__ void __launch_bounds__(TOP_THREADS, 4) top_rows(con
   work.run(*reinterpret_cast<TopShared*>(smem));
 }
 
+inline size_t top_smem(int slice) {
+  return sizeof(TopShared) + size_t((slice + 32 * TOP_THREADS - 1) / (32 * TOP_THREADS)) * TOP_THREADS * sizeof(float2);
+}
 template <int DT> cudaError_t launch_top(const TopParams& p, cudaStream_t stream) {
   static Configured configured;
-  return launch_clusters(top_rows<DT>, p, false, p.in.rows, p.in.ranks, TOP_THREADS, sizeof(TopShared), stream, configured);
+  return launch_clusters(top_rows<DT>, p, false, p.in.rows, p.in.ranks, TOP_THREADS, top_smem(p.in.slice), stream, configured);
 }
 
 }  // namespace score
