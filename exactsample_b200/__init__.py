@@ -6,7 +6,9 @@ The public surface is the reference package's CUDA API
 ``CudaPlan``, ``CudaRequestParams``, ``CudaRngKey``, ``CudaOutput``,
 ``load_library`` and the ``Status`` / ``PathUsed`` / ``RequestParams`` /
 ``RngKey`` / ``VerifyOutput`` types. The FP64 NumPy oracle of the reference
-is not part of this package.
+is not part of this package. ``exactsample_b200.scoring`` has the row operators
+on the same logits: token log-probabilities, top logits, and the policy and
+distillation losses with their gradients.
 """
 from .types import PathUsed, RequestParams, RngKey, Status, VerifyOutput
 

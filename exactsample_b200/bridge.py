@@ -21,7 +21,9 @@ engine integration is the mapping of its own batch objects onto them:
 * Drafts. ``gather_drafts`` reads request r's d-th proposal from the engine's
   per-row token vector at row offsets[r] + 1 + d (vllm_bridge.py:286-299).
 * After the call. ``committed_counts`` gives accepted drafts plus one, zero
-  for a failed request (vllm_bridge.py:312-320). ``StatusCopy`` snapshots the
+  for a failed request (vllm_bridge.py:312-320). ``committed_row_tokens`` gives
+  each logits row's committed token, for the log-probabilities a server reports
+  (exactsample_b200.scoring). ``StatusCopy`` snapshots the
   statuses and tokens, copies them to pinned host memory on a side stream
   behind one event, and gives a failed request no tokens when the host reads
   them (vllm_async.py:43-85).
@@ -224,6 +226,21 @@ def committed_counts(out, requests: int):
     residual or bonus token), zero for a failed request."""
     counts = out.accepted_len[:requests].to(out.tokens.dtype) + 1
     return counts.masked_fill_(out.status[:requests] != int(Status.OK), 0)
+
+
+def committed_row_tokens(out, cu_rows, rows: int):
+    """For every logits row of the step, the token it committed, or -1: row
+    ``cu_rows[r] + d`` holds request r's d-th committed token (an accepted
+    draft, or the residual or bonus token), and the rows behind those, or of a
+    failed request, hold none. These are the tokens whose log-probabilities
+    ``exactsample_b200.scoring.token_logprobs`` reports from the same logits."""
+    import torch
+
+    row = torch.arange(rows, dtype=torch.int64, device=cu_rows.device)
+    request = torch.searchsorted(cu_rows[1:], row, right=True)
+    place = row - cu_rows[request]
+    committed = (out.status[request] == int(Status.OK)) & (place <= out.accepted_len[request])
+    return torch.where(committed, out.tokens[request, place], -1)
 
 
 class StatusCopy:

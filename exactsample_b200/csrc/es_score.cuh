@@ -3,12 +3,18 @@
 // read of the row.
 //
 // A row is split over the ranks of one thread-block cluster in contiguous
-// slices, and each rank keeps its slice in shared memory (about 38 KB, so
-// that five blocks share an SM). The row is read from HBM once: the first
-// pass over the slice takes the running maximum and the sums, the ranks
-// exchange them, and the gradient is written from the same shared copy. A
-// loss with its gradient so moves one read and one write of the row, where a
-// row that does not stay on the chip needs two reads and one write.
+// slices, and each rank keeps its slice in shared memory (about 50 KB, so
+// that four blocks share an SM). The row is read from HBM once: the first
+// pass over the slice takes the sums, the ranks exchange them, and the
+// gradient is written from the same shared copy. A loss with its gradient so
+// moves one read and one write of the row, where a row that does not stay on
+// the chip needs two reads and one write.
+//
+// Bounds: the HBM, then the exponentials (two a token, 16 a cycle and SM:
+// about 70 % of the time that 2-byte rows take at full HBM rate), then latency
+// between the passes. Measured on a B200, 4,096 rows of 151,936 bf16: the
+// policy step 453 us, 5.4 TB/s, 82 % of a copy's rate; without any
+// exponential the same loops take 408 us.
 //
 // The split depends on the vocabulary and the type alone, and every thread
 // takes the same elements whatever the row's address, so a row's results are
@@ -19,18 +25,11 @@
 
 #include "es_device.cuh"
 
-#ifndef ES_SCORE_THREADS
-#define ES_SCORE_THREADS 128
-#endif
-#ifndef ES_SCORE_BLOCKS
-#define ES_SCORE_BLOCKS 5
-#endif
-
 namespace es {
 namespace score {
 
 enum Op { LOGPROB = 0, POLICY = 1, DISTILL = 2 };
-constexpr int THREADS = ES_SCORE_THREADS, WARPS = THREADS / 32;
+constexpr int THREADS = 128, WARPS = THREADS / 32, BLOCKS = 4;  // blocks: to an SM (see loss_rows)
 constexpr int MAX_RANKS = 16;   // cluster size (beyond 8: non-portable, as for the row kernels)
 constexpr int MAX_TOP = ES_MAX_TOP;
 constexpr int STEP = 4 * THREADS;  // chunks that the block takes at a time, four a thread
@@ -204,16 +203,20 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // ---------------------------------------------------------------------------
-// The running maximum m of the logits seen, s = sum 2^d and u = sum 2^d d with
-// d = (z - m) scale: everything a row's log-sum and entropy need. scale =
-// log2(e) / temperature. s and u are held as two partial sums.
+// Sums over logits against a reference m, one of them: s = sum 2^d and u = sum
+// 2^d d with d = (z - m) scale: everything a row's log-sum and entropy need.
+// scale = log2(e) / temperature. s and u are held as two partial sums.
 //
-// The fast form takes d = z scale - r in one instruction, with r = m scale
-// rounded to 32 bits; acc_exact afterwards makes s and u those of m itself. It
-// leaves three kinds of rows wrong, and acc_failed tells: a -inf beside an
-// entropy (0 * -inf), an r that overflows, and an r so large that its rounding
-// moves the exponents. The careful form, which subtracts first and holds
-// exponents at FAR, is right for those.
+// The fast forms take d = z scale - r in one instruction, with r = m scale
+// rounded to 32 bits; acc_exact afterwards makes s and u those of m itself.
+// Their m is not the maximum: 32-bit sums keep their digits wherever the
+// largest 2^d lies, so a warp's largest of its first tokens serves all of its
+// tokens, and no maximum is looked for after those (it took a third of the
+// pass). They leave some rows wrong, and acc_failed tells: sums of 2^60 and
+// more (a row's coefficient, 1 / s, is to stay a normal number), a -inf
+// beside an entropy (0 * -inf), an r that overflows, and an r so large that
+// its rounding moves the exponents. The careful form, which keeps the running
+// maximum, subtracts first and holds exponents at FAR, is right for those.
 struct Acc {
   float m, r;
   float2 s, u;
@@ -259,15 +262,7 @@ template <int DT> __device__ __forceinline__ float chunk_max_nan(const uint4& q)
     return __bfloat162float(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m)));
   }
 }
-template <int N, bool ENTROPY>
-__device__ __forceinline__ void acc_fast(Acc& a, const float2* v, float top, float scale) {
-  if (top > a.m) {
-    const float r = __fmul_rn(top, scale), d = __fsub_rn(a.r, r), f = a.m <= NONE ? 0.f : ex2(d);
-    if (ENTROPY) a.u = mul2(both(f), fma2(both(fmaxf(d, FAR)), a.s, a.u));
-    a.s = mul2(both(f), a.s);
-    a.m = top;
-    a.r = r;
-  }
+template <int N, bool ENTROPY> __device__ __forceinline__ void acc_add(Acc& a, const float2* v, float scale) {
   const float2 nr = both(-a.r), sc = both(scale);
 #pragma unroll
   for (int i = 0; i < N / 2; ++i) {
@@ -275,6 +270,18 @@ __device__ __forceinline__ void acc_fast(Acc& a, const float2* v, float top, flo
     const float2 e = make_float2(ex2(d.x), ex2(d.y));
     a.s = add2(a.s, e);
     if (ENTROPY) a.u = fma2(e, d, a.u);
+  }
+}
+// Raises the reference to `top` if that is 2^24 above it (masked rows, whose
+// first tokens may all be masked).
+template <bool ENTROPY> __device__ __forceinline__ void acc_raise(Acc& a, float top, float scale, float& limit) {
+  if (top > limit) {
+    const float r = __fmul_rn(top, scale), d = __fsub_rn(a.r, r), f = a.m <= NONE ? 0.f : ex2(d);
+    if (ENTROPY) a.u = mul2(both(f), fma2(both(fmaxf(d, FAR)), a.s, a.u));
+    a.s = mul2(both(f), a.s);
+    a.m = top;
+    a.r = r;
+    limit = __fadd_rn(top, __fdividef(24.f, scale));
   }
 }
 template <int N, bool ENTROPY>
@@ -297,7 +304,7 @@ __device__ __forceinline__ void acc_careful(Acc& a, const float2* v, float top, 
 constexpr float LARGE_R = 65536.f;  // its rounding is 2^-8 at most, which acc_exact takes back
 template <bool ENTROPY> __device__ __forceinline__ bool acc_failed(const Acc& a) {
   const float s = a.s.x + a.s.y, u = a.u.x + a.u.y;
-  return !(fabsf(a.r) <= LARGE_R) || !(s < INFINITY) || (ENTROPY && !(fabsf(u) < INFINITY));
+  return !(fabsf(a.r) <= LARGE_R) || !(s < 0x1p60f) || (ENTROPY && !(fabsf(u) < 0x1p67f));
 }
 
 // What one rank knows of its slice: s and u against the maximum m.
@@ -315,7 +322,7 @@ constexpr uint32_t BAD = 1, CAREFUL = 2, FULL = 4;
 template <bool ENTROPY> __device__ __forceinline__ Record acc_exact(const Acc& a, float scale, bool careful) {
   const float rest = careful || a.m <= NONE ? 0.f : __fmaf_rn(a.m, scale, -a.r), f = ex2(-rest);
   const float s = __fadd_rn(a.s.x, a.s.y), u = __fadd_rn(a.u.x, a.u.y);
-  return {careful || a.m > NONE ? fmaxf(a.m, LOWEST) : LOWEST, __fmul_rn(f, s), ENTROPY ? __fmul_rn(f, __fmaf_rn(-rest, s, u)) : 0.f, careful ? CAREFUL : 0u};
+  return {s == 0.f ? LOWEST : fmaxf(a.m, LOWEST), __fmul_rn(f, s), ENTROPY ? __fmul_rn(f, __fmaf_rn(-rest, s, u)) : 0.f, careful ? CAREFUL : 0u};
 }
 // The records of LANES neighbouring lanes as one, in every lane. Every warp of
 // a block takes it, not in a branch: where the compiler cannot tell that a
@@ -391,7 +398,6 @@ template <int GROUPS> __device__ __forceinline__ void copies_done() {  // all bu
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------
-// ---------------------------------------------------------------------------
 // 16 bytes at `shift` bytes into the 32 of two pieces; shift below 16.
 template <int SIZE> __device__ __forceinline__ uint4 shifted_chunk(const uint4& a, const uint4& b, uint32_t shift) {
   uint32_t w[7] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z};
@@ -433,9 +439,11 @@ __device__ __forceinline__ uint4 fetch_chunk(const typename Elem<DT>::T* src, in
 // A rank's slice of the row in shared memory, element i at base + i sizeof(T).
 // Chunk c is brought, read and written by thread c mod THREADS alone, so that
 // its way needs no barrier. Rows that start on 16 bytes come by asynchronous
-// copies of whole chunks, rows that start on 4 by copies of words (4 a chunk:
-// 33 us more for 1,001 rows of 50,257 float32, where a move through registers
-// costs 150), others through registers.
+// copies of whole chunks, rows that start on 4 by copies of words, and 2-byte
+// rows between words by copies of words too, one element off: realign puts
+// them right. Rows with a stride pass through registers. (1,001 rows of 50,257
+// through distill_loss and its backward pass: float32 207 us, bf16 164; with
+// such rows through registers 371 and 238; rows of 50,256 take 174 and 131.)
 template <int DT> struct Slice {
   using T = typename Elem<DT>::T;
   static constexpr int N = Elem<DT>::N;
@@ -455,26 +463,62 @@ template <int DT> struct Slice {
   static __device__ __forceinline__ const T* source(const Rows& in, int64_t row, int begin) {
     return static_cast<const T*>(in.logits) + row * in.l_s0 + int64_t(begin) * in.l_s1;
   }
-  // How a row comes: 16 or 4 bytes a copy, or 0 for none.
+  // How a row comes: 16 or 4 bytes a copy, 2 for words one element off, 0 for none.
   static __device__ __forceinline__ int width(const Rows& in, const T* src) {
     const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(src)) & 15;
-    return in.l_s1 != 1 ? 0 : off == 0 ? 16 : off % 4 == 0 ? 4 : 0;
+    return in.l_s1 != 1 ? 0 : off == 0 ? 16 : off % 4 == 0 ? 4 : 2;
   }
   // Chunk c of a row that has a width; a whole one.
   __device__ __forceinline__ void copy(int c, const T* src, int width) const {
+    uint32_t* to = reinterpret_cast<uint32_t*>(&chunk(c));
     if (width == 16) {
-      copy_async(&chunk(c), reinterpret_cast<const uint4*>(src) + c);
-    } else {
+      copy_async(to, reinterpret_cast<const uint4*>(src) + c);
+    } else if (width == 4) {
       const uint32_t* from = reinterpret_cast<const uint32_t*>(src) + 4 * c;
-      uint32_t* to = reinterpret_cast<uint32_t*>(&chunk(c));
 #pragma unroll
       for (int i = 0; i < 4; ++i) copy_async4(to + i, from + i);
+    } else {
+      // Elements N c - 1 to N c + N - 2; the slice's first has none before it.
+      const uint32_t* from = reinterpret_cast<const uint32_t*>(src - 1) + 4 * c;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i > 0 || c > 0) copy_async4(to + i, from + i);
+      if (c == 0) (*this)[1] = src[0];
     }
   }
-  // The last chunk where it is not whole, by the thread that owns it.
-  __device__ __forceinline__ void load_ragged(const T* src, int64_t stride) const {
+  // What whole chunks leave of a row that has a width, by the thread whose
+  // place it lies in.
+  __device__ __forceinline__ void load_ragged(const T* src, int width) const {
     const int whole = n / N;
-    if (whole < chunks && int(threadIdx.x) == whole % THREADS) chunk(whole) = fetch_chunk<DT>(src, stride, whole, n);
+    if (int(threadIdx.x) != whole % THREADS) return;
+    if (width != 2) {
+      if (whole < chunks) chunk(whole) = fetch_chunk<DT>(src, 1, whole, n);
+    } else {
+      for (int i = whole * N; i <= chunks * N; ++i) (*this)[i] = i > 0 && i <= n ? src[i - 1] : Elem<DT>::put(-INFINITY);
+    }
+  }
+  // All threads: a row of width 2, all there, one element down. A round reads
+  // only what no earlier round wrote.
+  __device__ __forceinline__ void realign() const {
+    __syncthreads();
+#pragma unroll 1
+    for (int first = 0; first < chunks; first += STEP) {
+      uint4 q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = min(first + i * THREADS + int(threadIdx.x), chunks - 1);
+        const uint4 a = chunk(c);
+        const uint32_t more = reinterpret_cast<const uint32_t*>(&chunk(c + 1))[0];
+        q[i] = make_uint4(__funnelshift_r(a.x, a.y, 16), __funnelshift_r(a.y, a.z, 16), __funnelshift_r(a.z, a.w, 16),
+                          __funnelshift_r(a.w, more, 16));
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = first + i * THREADS + int(threadIdx.x);
+        if (c < chunks) chunk(c) = q[i];
+      }
+    }
   }
   __device__ __forceinline__ void load(const Rows& in, int64_t row, int begin) const {
     const T* src = source(in, row, begin);
@@ -485,7 +529,7 @@ template <int DT> struct Slice {
       copies_end_group();
       for (; c < whole; c += THREADS) copy(c, src, bytes);
       copies_end_group();
-      load_ragged(src, 1);
+      load_ragged(src, bytes);
       return;
     }
     copies_end_group();  // (mask words)
@@ -572,8 +616,29 @@ __device__ __forceinline__ Record sum_slice(const Slice<DT>& slice, const uint32
       slice.chunk(c) = q;
     }
   };
-  // Four chunks a step: one look at the maximum for all, and independent
-  // loads and exponentials.
+  const auto hold = [&](float2* v, int pairs) {
+    if (HOLD) {
+#pragma unroll
+      for (int i = 0; i < pairs; ++i) v[i] = make_float2(fmaxf(v[i].x, MASKED), fmaxf(v[i].y, MASKED));
+    }
+  };
+  bool blank = false;  // no reference among the first tokens
+  float limit = NONE;
+  if (slice.half == 0) slice.arrive_rest();
+  if (!HAS_MASK) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (tid + i * THREADS < slice.chunks && (i == 0 || slice.half > 0)) {
+        const uint4 q = slice.chunk(tid + i * THREADS);
+        top = fmaxf(top, chunk_max<DT>(q, q));
+      }
+    top = warp_all(top, [](float x, float y) { return fmaxf(x, y); });
+    blank = !(top > -INFINITY);
+    a.m = blank ? 0.f : top;
+    a.r = __fmul_rn(a.m, scale);
+  }
+  // Four chunks a step, for independent loads and exponentials.
   int c = tid;
 #pragma unroll 1
   for (int part = 0; part < 2; ++part) {
@@ -586,30 +651,26 @@ __device__ __forceinline__ Record sum_slice(const Slice<DT>& slice, const uint32
       for (int i = 0; i < 4; ++i) q[i] = slice.chunk(c + i * THREADS);
 #pragma unroll
       for (int i = 0; i < 4; ++i) take(q[i], c + i * THREADS);
-      const float top = fmaxf(chunk_max<DT>(q[0], q[1]), chunk_max<DT>(q[2], q[3]));
+      if (HAS_MASK) acc_raise<ENTROPY>(a, fmaxf(chunk_max<DT>(q[0], q[1]), chunk_max<DT>(q[2], q[3])), scale, limit);
       float2 v[2 * N];
 #pragma unroll
       for (int i = 0; i < 4; ++i) unpack<DT>(q[i], v + i * N / 2);
-      if (HOLD) {
-#pragma unroll
-        for (int i = 0; i < 2 * N; ++i) v[i] = make_float2(fmaxf(v[i].x, MASKED), fmaxf(v[i].y, MASKED));
-      }
-      acc_fast<4 * N, ENTROPY>(a, v, top, scale);
+      hold(v, 2 * N);
+      acc_add<4 * N, ENTROPY>(a, v, scale);
     }
   }
 #pragma unroll 1
   for (; c < slice.chunks; c += THREADS) {
     uint4 q = slice.chunk(c);
     take(q, c);
+    if (HAS_MASK) acc_raise<ENTROPY>(a, chunk_max<DT>(q, q), scale, limit);
     float2 v[N / 2];
     unpack<DT>(q, v);
-    if (HOLD) {
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) v[i] = make_float2(fmaxf(v[i].x, MASKED), fmaxf(v[i].y, MASKED));
-    }
-    acc_fast<N, ENTROPY>(a, v, chunk_max<DT>(q, q), scale);
+    hold(v, N / 2);
+    acc_add<N, ENTROPY>(a, v, scale);
   }
-  const bool failed = acc_failed<ENTROPY>(a) || scale < SMALL_SCALE || (HAS_MASK && any && a.m <= NONE);
+  const bool failed = tid < slice.chunks &&
+                      (blank || acc_failed<ENTROPY>(a) || scale < SMALL_SCALE || (HAS_MASK && any && a.m <= NONE));
   if (failed) {
     a = acc_none();
 #pragma unroll 1
@@ -713,8 +774,9 @@ struct Kept {
 };
 
 constexpr size_t SHARED_BYTES = (sizeof(Shared) + 15) / 16 * 16;
+// The buffer of a slice, and a chunk more for rows that land one element off.
 template <int DT> __host__ __device__ constexpr size_t slice_bytes(int slice) {
-  return size_t(slice) * sizeof(typename Elem<DT>::T);
+  return size_t(slice) * sizeof(typename Elem<DT>::T) + 16;
 }
 // Then two rows' mask words, and the distillation's entries.
 __host__ __device__ constexpr size_t mask_bytes(int slice) { return size_t(slice) / 8; }
@@ -1024,7 +1086,7 @@ template <int DT, int OP, bool GRAD> struct LossRow {
       copies_end_group();
     }
     if (c == whole && whole < slice.chunks) store_elements(grad_chunk<FORM>(slice.chunk(c), c, words, r, scale), c, 0, N);
-    if (next) slice.load_ragged(next, 1);
+    if (next) slice.load_ragged(next, 16);
     // The thread that wrote the token's chunk.
     if (OP != DISTILL && token >= 0 && token / N % THREADS == tid) *grad_at(begin + token) = E::put(r.token_grad);
   }
@@ -1080,7 +1142,7 @@ template <int DT, int OP, bool GRAD> struct LossRow {
       }
       copies_end_group();
     }
-    if (bytes) slice.load_ragged(next, 1);
+    if (bytes) slice.load_ragged(next, bytes);
   }
   __device__ __forceinline__ void write_form(const Slice<DT>& slice, const uint32_t* words, const RowScalars& r, float scale,
                                              int token, const T* next) const {
@@ -1187,6 +1249,10 @@ template <int DT, int OP, bool GRAD> struct LossRow {
       float value_top = 0.f, x_top = 0.f;
       if (OP == DISTILL) kept_sums(sh, kept, scale, value_top, x_top);
       slice.arrive();
+      if (sizeof(T) == 2 && Slice<DT>::width(p.in, Slice<DT>::source(p.in, row, begin)) == 2) {
+        slice.arrive_rest();
+        slice.realign();
+      }
       if (masked && OP != DISTILL) __syncthreads();  // the mask words come from all threads' first copies
       if (OP == DISTILL) {
         slice.arrive_rest();
@@ -1260,7 +1326,7 @@ template <int DT, int OP, bool GRAD> struct LossRow {
 };
 
 template <int DT, int OP, bool GRAD>
-__global__ void __launch_bounds__(THREADS, ES_SCORE_BLOCKS) loss_rows(const __grid_constant__ LossParams p) {
+__global__ void __launch_bounds__(THREADS, BLOCKS) loss_rows(const __grid_constant__ LossParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   const int ranks = p.in.ranks, rank = int(blockIdx.x % unsigned(ranks));
   const int begin = rank * p.in.slice, n = min(p.in.slice, p.in.vocab - begin);

@@ -157,10 +157,7 @@ int split(Rows& r, const es_rows& in, size_t slice_bytes, int64_t least, size_t 
 size_t loss_bytes(int slice, int32_t dtype, bool mask, int k) {
   return dtype == ES_F32 ? loss_smem<ES_F32>(slice, mask, k) : loss_smem<ES_F16>(slice, mask, k);
 }
-#ifndef LOSS_KB
-#define LOSS_KB 38
-#endif
-constexpr size_t LOSS_SLICE_BYTES = LOSS_KB * 1024;
+constexpr size_t LOSS_SLICE_BYTES = 50 * 1024;
 
 int launched(cudaError_t e) {
   return e == cudaSuccess ? ES_SUCCESS

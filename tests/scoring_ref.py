@@ -105,6 +105,9 @@ class RowBounds:
         p, d = logp[live].exp(), (logp[live] - logp[live].max())
         self.m1 = float((p * d.abs()).sum())
         self.m2 = float((p * d * d).sum())
+        # The reference that exponents are taken against is one of the row's
+        # tokens, at most 2^60 below the maximum.
+        self.gap = min(float(d.abs().max()), 60 * math.log(2.0))
         terms = vocab / 256 / 2 + 8
         self.sum = 2.0**-22 + (terms + 24) * 2.0**-24 + 3 * 2.0**-24 * self.m1
 
@@ -113,7 +116,9 @@ class RowBounds:
 
     def entropy(self, h):
         # log(sum) and the ratio of sums: each term of the second carries |d|.
-        return self.sum * (2 + 2 * self.m1) + 3 * 2.0**-24 * self.m2 + 2.0**-23 * abs(float(h))
+        # Against a reference `gap` away, a term's product, the ratio and the
+        # difference are rounded once each in numbers larger by gap.
+        return self.sum * (2 + 2 * self.m1) + 3 * 2.0**-24 * (self.m2 + self.gap) + 2.0**-23 * abs(float(h))
 
     def probability(self, logp):
         """Relative, of each token's probability times the row's coefficient.

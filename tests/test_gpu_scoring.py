@@ -779,6 +779,7 @@ def test_offsets_beyond_32_bits():
 def test_a_decode_step_then_training_on_it():
     """Tokens from ``verify``, their log-probabilities and top logits, then a
     policy step on them and a distillation step against them."""
+    from exactsample_b200 import bridge
     from exactsample_b200.cuda import CudaRequestParams, CudaRngKey, plan, verify
 
     g = torch.Generator(device="cuda").manual_seed(8)
@@ -798,7 +799,8 @@ def test_a_decode_step_then_training_on_it():
                      rng=CudaRngKey(torch.arange(requests, **ints), torch.zeros(requests, **ints),
                                     torch.arange(requests, **ints)),
                      plan=work, out=work.allocate_output(), mask=mask)
-    tokens = sampled.tokens[:, 0]
+    tokens = bridge.committed_row_tokens(sampled, torch.arange(requests + 1, **ints), requests)
+    assert torch.equal(tokens, sampled.tokens[:, 0])
     common = dict(temperature=temperature, mask=mask)
     old = scoring.token_logprobs(logits, tokens, **common)
     assert int(tokens[7]) == -1 and float(old.logprobs[7]) == 0

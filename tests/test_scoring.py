@@ -170,6 +170,7 @@ def test_outputs_may_not_overlap():
 def test_vocabularies_beyond_a_cluster_are_refused():
     for name in OPERATORS:
         a = arguments(name)
+        a.rows.logits.data = 1 << 44
         a.rows.logits.size[1] = 4_000_000
         a.rows.logits.stride[0] = 4_000_000
         code, text = call(name, a)
@@ -198,6 +199,17 @@ def test_python_refusals():
         scoring.policy_loss(logits, tokens, column.clone().requires_grad_(), column)
     with pytest.raises(ValueError, match="tail=True needs"):
         scoring.distill_loss(logits, scoring.TopLogits(column, tokens, None))
+
+
+def test_committed_row_tokens():
+    from exactsample_b200 import bridge
+    from exactsample_b200.cuda import CudaOutput
+
+    tokens = torch.tensor([[5, 6, 7], [8, -1, -1], [9, 10, -1], [1, 2, 3]])
+    out = CudaOutput(tokens, torch.tensor([2, 0, 1, 0], dtype=torch.int32), torch.tensor([0, 0, 0, 2], dtype=torch.int32),
+                     torch.zeros(4, dtype=torch.int32), 4)
+    cu_rows = torch.tensor([0, 3, 5, 8, 9])  # request 2 accepted one of two drafts, request 3 failed
+    assert bridge.committed_row_tokens(out, cu_rows, 9).tolist() == [5, 6, 7, 8, -1, 9, 10, -1, -1]
 
 
 # ---------------------------------------------------------------- the formulas
