@@ -13,7 +13,7 @@ from tests import scoring_ref as ref
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
-# One token to several slices: a rank's slice holds 38 KB of a row (16 ranks at most).
+# One token to several slices: a rank's slice holds 50 KB of a row (16 ranks at most).
 VOCABS = [1, 2, 7, 31, 33, 128, 129, 1000, 4099, 19_500, 50_257]
 
 
@@ -581,6 +581,52 @@ def test_a_row_has_the_same_bits_in_any_batch(dtype, vocab):
         part = scoring.TopLogits(teacher.values[at], teacher.ids[at], teacher.rest[at])
         moved = place(logits[at].cpu(), "odd")
         for got, want in zip(all_outputs(moved, tokens[at], part, [c[at] for c in columns]), whole):
+            assert torch.equal(got, want[at])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
+@pytest.mark.parametrize("vocab", [1003, 1008, 13_001, 60_016])
+@pytest.mark.parametrize("masked", [False, True], ids=["open", "masked"])
+def test_rows_that_share_a_cluster(dtype, vocab, masked):
+    """More rows than clusters run at a time, so that rows are copied beside
+    the row before: bad, hard and padded ones between others, with and without
+    a gradient, against the same rows in small batches."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    rows, piece = 1400 if vocab < 20_000 else 520, 50
+    logits = (torch.randn(rows, vocab, device="cuda", generator=g) * 3).to(dtype)
+    logits[3::7, ::5] = -math.inf   # the careful form
+    logits[5::11, 1] = math.nan
+    logits[8::13] = -math.inf
+    logits[10::17, :900] = -math.inf
+    tokens = torch.randint(vocab, (rows,), device="cuda", generator=g)
+    tokens[torch.rand(rows, device="cuda", generator=g) < 0.3] = -1
+    allowed = torch.rand(rows, vocab, device="cuda", generator=g) < 0.5
+    allowed[4::9] = False
+    mask = ref.pack_mask(allowed.cpu()).cuda() if masked else None
+    ids = torch.stack([torch.randint(i * vocab // 9, (i + 1) * vocab // 9, (rows,), device="cuda", generator=g) for i in range(9)], 1)
+    ids[torch.rand(rows, device="cuda", generator=g) < 0.3] = -1
+    values, rest = torch.randn(rows, 9, device="cuda", generator=g), torch.randn(rows, device="cuda", generator=g)
+    columns = [torch.randn(rows, device="cuda", generator=g) for _ in range(4)]
+
+    def calls(at, with_grad):
+        x = logits[at]
+        common = dict(temperature=0.7, mask=None if mask is None else mask[at])
+        grads = [torch.full_like(x, 7.0) if with_grad else None for _ in range(3)]
+        c = [column[at] for column in columns]
+        incoming = dict(grad_logprobs=c[0], grad_entropy=c[1]) if with_grad else {}
+        outs = [scoring.token_logprobs(x, tokens[at], grad=grads[0], **incoming, **common),
+                scoring.policy_loss(x, tokens[at], c[0], c[1], ref_logprobs=c[2], weights=c[3], kl_coef=0.1, entropy_coef=0.02,
+                                    grad=grads[1], **common),
+                scoring.distill_loss(x, scoring.TopLogits(values[at], ids[at], rest[at]), weights=c[3], grad=grads[2], **common)]
+        return [getattr(o, n) for o in outs for n in o.__slots__], grads
+    whole, whole_grads = calls(slice(0, rows), True)
+    forward, _ = calls(slice(0, rows), False)
+    for got, want in zip(forward, whole):
+        assert torch.equal(got, want)
+    for first in range(0, rows, piece):
+        at = slice(first, first + piece)
+        part, part_grads = calls(at, True)
+        for got, want in zip(part + part_grads, whole + whole_grads):
             assert torch.equal(got, want[at])
 
 
