@@ -20,6 +20,12 @@
 // id, so that all are distinct and equal logits rank by the lowest id. Where a
 // rank lists more than its places on rank 0 (equal values, in the main), rank
 // 0 finds the exact threshold by a digit-by-digit count over the whole row.
+//
+// Bounds: the latency of the steps after the streaming, each of which waits
+// for the other ranks. Measured on a B200: the 64 largest of 2,048 rows of
+// 151,936 bf16 take 177 us (3.5 TB/s), of which the first step alone is 129.
+// More blocks to an SM hide more of it (six: 204, eight: 177). A row that lay
+// in shared memory, for the second look, took 483.
 #pragma once
 #include "es_score.cuh"
 
@@ -36,6 +42,7 @@ struct TopParams {
 };
 
 constexpr int TOP_THREADS = 128, TOP_WARPS = TOP_THREADS / 32;
+constexpr int TOP_BLOCKS = 8;  // to an SM (64 of 2,048 rows: 177 us; ten 185, twelve 210: fewer registers for loads in flight)
 constexpr uint32_t KEY_NONE = 0x007fffffu;  // the key of -inf: not a token of the row
 constexpr int COLLECTED = 1024;             // entries rank 0 takes, an equal share from each rank
 constexpr int HOT = 128;                    // steps a warp looks at again
@@ -48,10 +55,15 @@ struct TopShared {
   uint16_t hot[TOP_WARPS][HOT];  // steps to look at again
   uint32_t listed, entries;
   uint32_t digits[TOP_WARPS][8];
-  float beyond[COLLECTED];   // values past the k-th, by place
-  alignas(16) uint64_t places[COLLECTED];
-  uint64_t collected[COLLECTED];
-  float2 steps[1];           // maximum and sum of each thread's steps, as many as a slice has
+  alignas(16) uint64_t places[COLLECTED];  // rank 0: each rank's list at its share, then all side by side
+  // Maximum and sum of each thread's steps, as many as a slice has; then, on
+  // rank 0, when all its warps have done with those, values past the k-th by
+  // place. (Memory of its own for each list leaves room for six blocks to an
+  // SM: 204 us for 64 of 2,048 rows of 151,936 bf16, against 177.)
+  union {
+    float2 steps[COLLECTED / 2];
+    float beyond[COLLECTED];
+  };
 };
 
 __device__ __forceinline__ uint64_t entry_of(uint32_t key, int id) { return (uint64_t(key) << 32) | (0xffffffffu - uint32_t(id)); }
@@ -266,7 +278,7 @@ template <int DT> struct TopRow {
       sh.listed = sh.entries = 0;
     }
     if (rank == 0)
-      for (int i = tid; i < COLLECTED; i += TOP_THREADS) sh.collected[i] = 0;
+      for (int i = tid; i < COLLECTED; i += TOP_THREADS) sh.places[i] = 0;
     if (rank == 0) cluster_arrive();  // (the cleared places too)
     else cluster_started();
     const Scale temperature = row_scale(p.in, row);
@@ -290,7 +302,7 @@ template <int DT> struct TopRow {
     // The steps below the bound add up; the others' tokens are looked at again,
     // a lane each.
     const int share = COLLECTED / ranks;
-    uint64_t* places = cg::this_cluster().map_shared_rank(sh.collected, 0) + rank * share;
+    uint64_t* places = cg::this_cluster().map_shared_rank(sh.places, 0) + rank * share;
     Record rec = {LOWEST, 0.f, 0.f, 0u};
     bool full = false;
     int count = 0;
@@ -367,7 +379,7 @@ template <int DT> struct TopRow {
     count = 0;
 #pragma unroll
     for (int i = 0; i < COLLECTED / TOP_THREADS; ++i) {
-      mine[i] = sh.collected[i * TOP_THREADS + tid];
+      mine[i] = sh.places[i * TOP_THREADS + tid];
       count += mine[i] != 0;
     }
     int upto = count;
@@ -431,7 +443,7 @@ template <int DT> struct TopRow {
   }
 };
 
-template <int DT> __global__ void __launch_bounds__(TOP_THREADS, 8) top_rows(const __grid_constant__ TopParams p) {
+template <int DT> __global__ void __launch_bounds__(TOP_THREADS, TOP_BLOCKS) top_rows(const __grid_constant__ TopParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   const int ranks = p.in.ranks, rank = int(blockIdx.x % unsigned(ranks));
   const int begin = rank * p.in.slice, n = min(p.in.slice, p.in.vocab - begin);
@@ -440,7 +452,8 @@ template <int DT> __global__ void __launch_bounds__(TOP_THREADS, 8) top_rows(con
 }
 
 inline size_t top_smem(int slice) {
-  return sizeof(TopShared) + size_t((slice + 32 * TOP_THREADS - 1) / (32 * TOP_THREADS)) * TOP_THREADS * sizeof(float2);
+  const size_t steps = size_t((slice + 32 * TOP_THREADS - 1) / (32 * TOP_THREADS)) * TOP_THREADS * sizeof(float2);
+  return std::max(sizeof(TopShared), offsetof(TopShared, steps) + steps);
 }
 template <int DT> cudaError_t launch_top(const TopParams& p, cudaStream_t stream) {
   static Configured configured;
