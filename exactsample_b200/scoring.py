@@ -34,7 +34,6 @@ from dataclasses import dataclass
 from typing import Any
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .cuda import load_library
 
@@ -103,28 +102,6 @@ def _tracked(logits, grad, *others) -> bool:
     return True
 
 
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, temperature, temperature_all, mask):
-        ctx.save_for_backward(logits, tokens, temperature, mask)
-        ctx.temperature_all = temperature_all
-        ctx.set_materialize_grads(False)
-        out = _ops.token_logprobs(logits, tokens, temperature, temperature_all, mask, None, None, None)
-        ctx.mark_non_differentiable(out[2])
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_logprobs, grad_entropy, _):
-        if grad_logprobs is None and grad_entropy is None:
-            return None, None, None, None, None
-        logits, tokens, temperature, mask = ctx.saved_tensors
-        grad = torch.empty_like(logits)
-        _ops.token_logprobs(logits, tokens, temperature, ctx.temperature_all, mask, grad, grad_logprobs,
-                                    grad_entropy)
-        return grad, None, None, None, None
-
-
 def token_logprobs(logits, tokens, *, temperature=1.0, mask=None, grad=None, grad_logprobs=None,
                    grad_entropy=None) -> TokenLogprobs:
     """log p[token] and the entropy of each row of ``logits`` [rows, vocab] (float16, bfloat16 or float32).
@@ -138,7 +115,9 @@ def token_logprobs(logits, tokens, *, temperature=1.0, mask=None, grad=None, gra
     """
     per_row, everywhere = _temperature(temperature)
     if _tracked(logits, grad, per_row, grad_logprobs, grad_entropy):
-        return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, per_row, everywhere, mask))
+        if grad_logprobs is not None or grad_entropy is not None:
+            raise ValueError("grad_logprobs and grad_entropy need grad")
+        return TokenLogprobs(*_ops.token_logprobs_tracked(logits, tokens, per_row, everywhere, mask))
     return TokenLogprobs(*_ops.token_logprobs(logits, tokens, per_row, everywhere, mask, grad, grad_logprobs,
                                                       grad_entropy))
 
@@ -156,27 +135,6 @@ def top_logits(logits, k: int, *, temperature=1.0, mask=None) -> TopLogits:
                                               everywhere, mask))
 
 
-class _PolicyLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, old, advantages, ref, weights, temperature, temperature_all, mask, coefficients):
-        ctx.save_for_backward(logits, tokens, old, advantages, ref, weights, temperature, mask)
-        ctx.temperature_all, ctx.coefficients = temperature_all, coefficients
-        out = _ops.policy_loss(logits, tokens, old, advantages, ref, weights, temperature, temperature_all,
-                                       mask, *coefficients, None)
-        ctx.mark_non_differentiable(*out[1:])
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_loss, *_):
-        logits, tokens, old, advantages, ref, weights, temperature, mask = ctx.saved_tensors
-        grad = torch.empty_like(logits)
-        _ops.policy_loss(logits, tokens, old, advantages, ref,
-                                 grad_loss if weights is None else weights * grad_loss, temperature,
-                                 ctx.temperature_all, mask, *ctx.coefficients, grad)
-        return (grad,) + (None,) * 9
-
-
 def policy_loss(logits, tokens, old_logprobs, advantages, *, ref_logprobs=None, weights=None, temperature=1.0,
                 mask=None, clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0,
                 entropy_coef: float = 0.0, grad=None) -> PolicyLoss:
@@ -192,29 +150,10 @@ def policy_loss(logits, tokens, old_logprobs, advantages, *, ref_logprobs=None, 
     per_row, everywhere = _temperature(temperature)
     coefficients = (float(clip_low), float(clip_high), float(kl_coef), float(entropy_coef))
     if _tracked(logits, grad, old_logprobs, advantages, ref_logprobs, weights, per_row):
-        return PolicyLoss(*_PolicyLoss.apply(logits, tokens, old_logprobs, advantages, ref_logprobs, weights, per_row,
-                                             everywhere, mask, coefficients))
+        return PolicyLoss(*_ops.policy_loss_tracked(logits, tokens, old_logprobs, advantages, ref_logprobs, weights,
+                                                    per_row, everywhere, mask, *coefficients))
     return PolicyLoss(*_ops.policy_loss(logits, tokens, old_logprobs, advantages, ref_logprobs, weights,
                                                 per_row, everywhere, mask, *coefficients, grad))
-
-
-class _DistillLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, values, ids, rest, weights, temperature, temperature_all, mask):
-        ctx.save_for_backward(logits, values, ids, rest, weights, temperature, mask)
-        ctx.temperature_all = temperature_all
-        out = _ops.distill_loss(logits, values, ids, rest, weights, temperature, temperature_all, mask, None)
-        ctx.mark_non_differentiable(out[1])
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_loss, _):
-        logits, values, ids, rest, weights, temperature, mask = ctx.saved_tensors
-        grad = torch.empty_like(logits)
-        _ops.distill_loss(logits, values, ids, rest, grad_loss if weights is None else weights * grad_loss,
-                                  temperature, ctx.temperature_all, mask, grad)
-        return (grad,) + (None,) * 7
 
 
 def distill_loss(logits, teacher: TopLogits, *, weights=None, temperature=1.0, mask=None, tail: bool = True,
@@ -235,7 +174,7 @@ def distill_loss(logits, teacher: TopLogits, *, weights=None, temperature=1.0, m
         raise ValueError("tail=True needs the teacher's rest")
     rest = teacher.rest if tail else None
     if _tracked(logits, grad, teacher.values, rest, weights, per_row):
-        return DistillLoss(*_DistillLoss.apply(logits, teacher.values, teacher.ids, rest, weights, per_row, everywhere,
-                                               mask))
+        return DistillLoss(*_ops.distill_loss_tracked(logits, teacher.values, teacher.ids, rest, weights, per_row,
+                                                      everywhere, mask))
     return DistillLoss(*_ops.distill_loss(logits, teacher.values, teacher.ids, rest, weights, per_row,
                                                   everywhere, mask, grad))

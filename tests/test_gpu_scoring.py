@@ -695,6 +695,56 @@ def test_a_changed_input_is_noticed_by_autograd():
         out.logprobs.sum().backward()
 
 
+def test_autograd_once_and_no_more():
+    g = torch.Generator(device="cuda").manual_seed(31)
+    rows, vocab = 6, 700
+    logits = torch.randn(rows, vocab, device="cuda", generator=g)
+    tokens = torch.randint(vocab, (rows,), device="cuda", generator=g)
+    columns = [torch.randn(rows, device="cuda", generator=g) for _ in range(2)]
+    teacher = scoring.top_logits(logits * 0.8, 9)
+    calls = [lambda x: scoring.token_logprobs(x, tokens).logprobs, lambda x: scoring.token_logprobs(x, tokens).entropy,
+             lambda x: scoring.policy_loss(x, tokens, *columns, entropy_coef=0.1).loss,
+             lambda x: scoring.distill_loss(x, teacher, weights=columns[0]).loss]
+    for call in calls:
+        leaf = logits.clone().requires_grad_()
+        out = call(leaf)
+        (first,) = torch.autograd.grad(out.sum(), leaf, retain_graph=True)
+        (again,) = torch.autograd.grad(out.sum(), leaf, create_graph=True)  # the graph is kept: the same once more
+        assert torch.equal(first, again)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            again.square().sum().backward()
+        call(leaf).sum().backward()
+        assert torch.equal(leaf.grad, first)
+        call(leaf).sum().backward()  # gradients add up
+        assert torch.equal(leaf.grad, first + first)
+        out = call(leaf)
+        out.sum().backward()
+        with pytest.raises(RuntimeError, match="second time"):
+            out.sum().backward()
+    # Through what broadcasts the logits, and half of the rows through each of two calls.
+    leaf = logits[:1].clone().requires_grad_()
+    scoring.token_logprobs(leaf.expand(rows, vocab), tokens).logprobs.sum().backward()
+    whole = logits[:1].expand(rows, vocab).contiguous().requires_grad_()
+    scoring.token_logprobs(whole, tokens).logprobs.sum().backward()
+    assert torch.equal(leaf.grad, whole.grad.sum(0, keepdim=True))
+    leaf = logits.clone().requires_grad_()
+    loss = scoring.token_logprobs(leaf[:2], tokens[:2]).logprobs.sum() + scoring.token_logprobs(leaf[2:], tokens[2:]).logprobs.sum()
+    loss.backward()
+    whole = logits.clone().requires_grad_()
+    scoring.token_logprobs(whole, tokens).logprobs.sum().backward()
+    assert torch.equal(leaf.grad, whole.grad)
+    status = scoring.token_logprobs(leaf, tokens).status
+    assert not status.requires_grad
+    with pytest.raises(ValueError, match="need grad"):
+        scoring.token_logprobs(leaf, tokens, grad_logprobs=columns[0])
+    with pytest.raises(RuntimeError, match="tokens has wrong"):
+        scoring.token_logprobs(leaf, tokens.int())
+    with torch.no_grad():
+        assert not scoring.token_logprobs(leaf, tokens).logprobs.requires_grad
+    with torch.inference_mode():
+        scoring.policy_loss(leaf, tokens, *columns)
+
+
 def test_rows_without_any_and_refusals_on_the_device():
     logits = torch.randn(4, 64, device="cuda")
     tokens = torch.zeros(4, dtype=torch.int64, device="cuda")
