@@ -249,6 +249,21 @@ template <int DT> __device__ __forceinline__ float chunk_max(const uint4& p, con
   }
 }
 // The same, and NaN if there is one.
+// Whether a chunk holds a -inf.
+template <int DT> __device__ __forceinline__ bool chunk_has_lowest(const uint4& q) {
+  if constexpr (DT == ES_F32) {
+    const float* a = reinterpret_cast<const float*>(&q);
+    return fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) == -INFINITY;
+  } else if constexpr (DT == ES_F16) {
+    const __half2* a = reinterpret_cast<const __half2*>(&q);
+    const float2 m = __half22float2(__hmin2(__hmin2(a[0], a[1]), __hmin2(a[2], a[3])));
+    return fminf(m.x, m.y) == -INFINITY;
+  } else {
+    const __nv_bfloat162* a = reinterpret_cast<const __nv_bfloat162*>(&q);
+    const float2 m = __bfloat1622float2(__hmin2(__hmin2(a[0], a[1]), __hmin2(a[2], a[3])));
+    return fminf(m.x, m.y) == -INFINITY;
+  }
+}
 template <int DT> __device__ __forceinline__ float chunk_max_nan(const uint4& q) {
   if constexpr (DT == ES_F32) {
     return max_nan(max_nan(__uint_as_float(q.x), __uint_as_float(q.y)), max_nan(__uint_as_float(q.z), __uint_as_float(q.w)));
@@ -313,9 +328,10 @@ struct alignas(16) Record {
   uint32_t flags;
 };
 // BAD: an invalid row (a NaN or +inf, a repeated id, a copy that did not
-// arrive). CAREFUL: the gradient needs the careful form too. FULL: top_rows'
+// arrive). CAREFUL: the gradient needs the careful form too. HELD: it needs
+// the slice's -inf held at MASKED. FULL: top_rows'
 // lists did not fit.
-constexpr uint32_t BAD = 1, CAREFUL = 2, FULL = 4;
+constexpr uint32_t BAD = 1, CAREFUL = 2, FULL = 4, HELD = 8;
 
 // s and u against m itself: with m scale = r + rest, 2^(z scale - r) is 2^rest
 // times too large and its exponent off by rest (at most 2^-8).
@@ -586,6 +602,21 @@ template <int DT> __device__ __forceinline__ uint4 mask_chunk(const uint4& q, ui
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
+// A chunk's -inf at MASKED (not for float16).
+template <int DT> __device__ __forceinline__ uint4 hold_chunk(const uint4& q) {
+  uint4 r = q;
+  if constexpr (DT == ES_F32) {
+    float* v = reinterpret_cast<float*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = max_nan(v[i], MASKED);
+  } else if constexpr (DT == ES_BF16) {
+    __nv_bfloat162* v = reinterpret_cast<__nv_bfloat162*>(&r);
+    const uint32_t word = masked_word<DT>();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __hmax2_nan(v[i], reinterpret_cast<const __nv_bfloat162&>(word));
+  }
+  return r;
+}
 template <int DT> __device__ __forceinline__ uint32_t lowest_word() {  // -inf
   return DT == ES_F32 ? 0xff800000u : DT == ES_F16 ? 0xfc00fc00u : 0xff80ff80u;
 }
@@ -597,42 +628,59 @@ template <int N> __device__ __forceinline__ float max_of(const float2* v) {
 }
 
 // This thread's share of a slice as a Record: the fast form, or where that
-// fails the careful one. `words`: the slice's mask; its masked tokens are
-// masked in the slice too. The slice has arrived up to `half`.
-template <int DT, bool ENTROPY, bool HAS_MASK>
+// fails the careful one. The slice has arrived up to `half`. `words`: a
+// MASKED_ROW's mask; its masked tokens are masked in the slice too. An
+// OPEN_ROW's warps that see a -inf among their first tokens (rows that were
+// masked before) hold every -inf at MASKED instead; those that meet one later
+// take the careful form. (1,024 rows of 151,936 bf16 with a
+// fifth of -inf, log-probabilities and policy step: 137 and 191 us in
+// the careful form, 81 and 131 so, 74 and 127 without a -inf.)
+enum RowKind { OPEN_ROW, MASKED_ROW, HELD_ROW };
+template <int DT, bool ENTROPY, int KIND>
 __device__ __forceinline__ Record sum_slice(const Slice<DT>& slice, const uint32_t* words, float scale) {
   constexpr int N = Elem<DT>::N;
-  constexpr bool HOLD = HAS_MASK && ENTROPY && DT == ES_F16;
-  const int tid = threadIdx.x;
+  constexpr bool HAS_MASK = KIND == MASKED_ROW, RAISE = KIND != OPEN_ROW;
+  constexpr bool HOLD = RAISE && ENTROPY && DT == ES_F16;
+  const int tid = threadIdx.x, whole = slice.n / N;
   float seen_top = -INFINITY;  // of masked rows' logits, a NaN kept
-  uint32_t any = 0;            // mask bits seen
-  Acc a = acc_none(HAS_MASK ? NONE : -INFINITY);
+  uint32_t any = 0;            // mask bits seen, or whether a token is not -inf
+  Acc a = acc_none(RAISE ? NONE : -INFINITY);
+  // A chunk as it is summed; returns its maximum where that is asked for.
   const auto take = [&](uint4& q, int c) {
+    float top = -INFINITY;
+    if (KIND == HELD_ROW) {
+      top = chunk_max<DT>(q, q);
+      any |= top > -INFINITY;
+      q = hold_chunk<DT>(q);
+    }
     if (HAS_MASK) {
       const uint32_t bits = mask_bits(words, c * N) & ((1u << N) - 1u);
       any |= bits;
       seen_top = max_nan(seen_top, chunk_max_nan<DT>(q));
       q = mask_chunk<DT>(q, bits, masked_word<DT>());
-      slice.chunk(c) = q;
     }
+    if (HAS_MASK) slice.chunk(c) = q;
+    return top;
   };
   const auto hold = [&](float2* v, int pairs) {
-    if (HOLD) {
 #pragma unroll
-      for (int i = 0; i < pairs; ++i) v[i] = make_float2(fmaxf(v[i].x, MASKED), fmaxf(v[i].y, MASKED));
-    }
+    for (int i = 0; i < pairs; ++i) v[i] = make_float2(max_nan(v[i].x, MASKED), max_nan(v[i].y, MASKED));
   };
+  bool held = KIND == HELD_ROW;
   bool blank = false;  // no reference among the first tokens
   float limit = NONE;
   if (slice.half == 0) slice.arrive_rest();
-  if (!HAS_MASK) {
+  if (KIND == OPEN_ROW) {
     float top = -INFINITY;
+    bool lowest = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (tid + i * THREADS < slice.chunks && (i == 0 || slice.half > 0)) {
         const uint4 q = slice.chunk(tid + i * THREADS);
         top = fmaxf(top, chunk_max<DT>(q, q));
+        if (ENTROPY) lowest |= chunk_has_lowest<DT>(q);
       }
+    if (ENTROPY && __any_sync(0xffffffffu, lowest)) return sum_slice<DT, ENTROPY, ENTROPY ? HELD_ROW : OPEN_ROW>(slice, words, scale);
     top = warp_all(top, [](float x, float y) { return fmaxf(x, y); });
     blank = !(top > -INFINITY);
     a.m = blank ? 0.f : top;
@@ -643,34 +691,39 @@ __device__ __forceinline__ Record sum_slice(const Slice<DT>& slice, const uint32
 #pragma unroll 1
   for (int part = 0; part < 2; ++part) {
     if (part) slice.arrive_rest();
-    const int end = part ? slice.chunks : slice.half;
+    const int end = part ? whole : slice.half;
 #pragma unroll 1
     for (; c + 3 * THREADS < end; c += STEP) {
       uint4 q[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) q[i] = slice.chunk(c + i * THREADS);
+      float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) take(q[i], c + i * THREADS);
-      if (HAS_MASK) acc_raise<ENTROPY>(a, fmaxf(chunk_max<DT>(q[0], q[1]), chunk_max<DT>(q[2], q[3])), scale, limit);
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, take(q[i], c + i * THREADS));
+      if (HAS_MASK) top = fmaxf(chunk_max<DT>(q[0], q[1]), chunk_max<DT>(q[2], q[3]));
+      if (RAISE) acc_raise<ENTROPY>(a, top, scale, limit);
       float2 v[2 * N];
 #pragma unroll
       for (int i = 0; i < 4; ++i) unpack<DT>(q[i], v + i * N / 2);
-      hold(v, 2 * N);
+      if (HOLD) hold(v, 2 * N);
       acc_add<4 * N, ENTROPY>(a, v, scale);
     }
   }
 #pragma unroll 1
   for (; c < slice.chunks; c += THREADS) {
     uint4 q = slice.chunk(c);
-    take(q, c);
-    if (HAS_MASK) acc_raise<ENTROPY>(a, chunk_max<DT>(q, q), scale, limit);
+    float top = take(q, c);
+    if (HAS_MASK) top = chunk_max<DT>(q, q);
+    if (RAISE) acc_raise<ENTROPY>(a, top, scale, limit);
     float2 v[N / 2];
     unpack<DT>(q, v);
-    hold(v, N / 2);
+    if (HOLD || (ENTROPY && c >= whole)) hold(v, N / 2);  // (the last chunk is filled up with -inf)
+    if (ENTROPY && c >= whole)
+      for (int i = c * N; i < slice.n; ++i) held |= Elem<DT>::get(slice[i]) == -INFINITY;
     acc_add<N, ENTROPY>(a, v, scale);
   }
   const bool failed = tid < slice.chunks &&
-                      (blank || acc_failed<ENTROPY>(a) || scale < SMALL_SCALE || (HAS_MASK && any && a.m <= NONE));
+                      (blank || acc_failed<ENTROPY>(a) || scale < SMALL_SCALE || (RAISE && any && a.m <= NONE));
   if (failed) {
     a = acc_none();
 #pragma unroll 1
@@ -684,6 +737,7 @@ __device__ __forceinline__ Record sum_slice(const Slice<DT>& slice, const uint32
   }
   Record r = acc_exact<ENTROPY>(a, scale, failed);
   if (HAS_MASK && !(seen_top < INFINITY)) r.flags |= BAD;
+  if (held) r.flags |= HELD;
   return r;
 }
 
@@ -702,11 +756,13 @@ __device__ __forceinline__ Pair pair_sum(Pair a, Pair b) {
 }
 __device__ __forceinline__ Pair negated(Pair a) { return {-a.hi, -a.lo}; }
 __device__ __forceinline__ float value_of(Pair a) { return __fadd_rn(a.hi, a.lo); }
-// (a - b) / temperature.
+// (a - b) / temperature; of finite numbers a finite one (a type's lowest value
+// over a temperature below 1 leaves the range, and pairs of infinities are NaN).
 __device__ __forceinline__ Pair scaled_gap(float a, float b, const Scale& s) {
   const float hi = __fsub_rn(a, b), t = __fadd_rn(hi, b);
   const float rest = __fsub_rn(__fsub_rn(a, t), __fsub_rn(b, __fsub_rn(t, hi)));  // a - b = hi + rest
   const float p = __fmul_rn(hi, s.hi);
+  if (fabsf(p) == INFINITY && fabsf(a) < INFINITY && fabsf(b) < INFINITY) return {copysignf(-LOWEST, hi), 0.f};
   return {p, __fmaf_rn(hi, s.hi, -p) + (hi * s.lo + rest * s.hi)};
 }
 // log(s) for a positive, normal s, to about 2^-32: with s = 2^k f, f in
@@ -740,6 +796,7 @@ __device__ __forceinline__ float exp_beyond_first_order(float x, float exp_less_
 struct RowScalars {
   float m, r, a, b, token_grad;
   int32_t zero, careful;   // a row without a gradient; the form
+  int32_t held;            // -inf is held at MASKED
   float w, inv_q, inv_t;   // distillation: the kept tokens' gradients are w (q inv_q - t inv_t)
 };
 
@@ -912,6 +969,7 @@ template <int DT, int OP, bool GRAD> struct LossRow {
       // log p_j = d ln 2 - log s and h = log s - gap.
       set_scalars(r, m, scale.log2, -(slope - on_entropy * gap) * inv_s, -on_entropy * float(LN2) * inv_s,
                   flags & CAREFUL || scale.log2 < SMALL_SCALE);
+      r.held = flags & HELD;
       r.token_grad = -slope * expm1f(value_of(lp)) - on_entropy * expf(value_of(lp)) * (value_of(lp) + h);
     }
   }
@@ -1028,9 +1086,10 @@ template <int DT, int OP, bool GRAD> struct LossRow {
   __device__ __forceinline__ uint4 grad_chunk(uint4 q, int c, const uint32_t* words, const RowScalars& r, float scale) const {
     float2 v[N / 2];
     if (FORM == 2 && words) q = mask_chunk<DT>(q, mask_bits(words, c * N), lowest_word<DT>());
+    if (FORM == 1 && r.held) q = hold_chunk<DT>(q);
     unpack<DT>(q, v);
     if (FORM == 1 && DT == ES_F16) {
-      if (words) {
+      if (words || r.held) {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) v[i] = make_float2(fmaxf(v[i].x, MASKED), fmaxf(v[i].y, MASKED));
       }
@@ -1268,8 +1327,8 @@ template <int DT, int OP, bool GRAD> struct LossRow {
         __syncthreads();
       }
 
-      Record rec = masked ? sum_slice<DT, ENTROPY, true>(slice, words, scale.log2)
-                          : sum_slice<DT, ENTROPY, false>(slice, nullptr, scale.log2);
+      Record rec = masked ? sum_slice<DT, ENTROPY, MASKED_ROW>(slice, words, scale.log2)
+                          : sum_slice<DT, ENTROPY, OPEN_ROW>(slice, nullptr, scale.log2);
       // (The token's logit is looked at before this rank says that it has done
       // with the row's memory, which may be the gradient's.)
       if (OP != DISTILL && tid == 0) bad |= isnan(E::get(in.raw));

@@ -258,7 +258,8 @@ int es_ipc_free(void* ptr);
  * when no token is allowed or every allowed one is -inf; ES_DRAFT_ZERO_PROB
  * when a token that the operator needs has probability zero. A row whose
  * status is not ES_OK has log-probability -inf, loss, KL and entropy 0, and
- * a gradient of zeros.
+ * a gradient of zeros. A log-probability below float32's range (the type's
+ * lowest logit over a temperature below 1) is float32's lowest number.
  *
  * A gradient has the logits' type and shape. It may be the logits tensor
  * itself (same address and strides): the row is then replaced by its

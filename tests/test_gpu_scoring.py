@@ -74,7 +74,8 @@ def check_logprobs(x, tokens, temperatures, allowed, out, grad=None, on_lp=None,
         logp = ref.logp_of(z[r], allowed[r], temperature)
         h = float(ref.entropy_of(logp))
         bounds = ref.RowBounds(logp, vocab)
-        assert abs(got[0] - float(logp[t])) <= bounds.logprob(logp[t])
+        # (a log-probability below float32's range is held at its lowest number)
+        assert abs(got[0] - max(float(logp[t]), torch.finfo(torch.float32).min)) <= bounds.logprob(logp[t])
         assert abs(got[1] - h) <= bounds.entropy(h)
         if grad is not None:
             a, b = float(on_lp[r]), float(on_h[r])
@@ -118,6 +119,68 @@ def test_token_logprobs(dtype, vocab, layout):
     if layout in ("odd", "gaps"):  # what lies between the rows' elements is untouched
         backing = logits._base
         assert int(torch.isnan(backing).sum()) == backing.numel() - rows * vocab
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
+@pytest.mark.parametrize("vocab", [40, 1003, 19_500, 50_257])
+def test_token_logprobs_of_rows_with_infinities(dtype, vocab):
+    """Rows masked by -inf before: a fifth of them, nearly all, only late ones,
+    and beside the type's lowest values, with and without an entropy gradient."""
+    g = torch.Generator().manual_seed(vocab + 1)
+    x = ref.test_rows(g, 9, vocab, dtype)
+    few = torch.randperm(vocab, generator=g)[:5]
+    lowest = torch.finfo(dtype).min
+    x[0, ::5] = -math.inf
+    x[1, torch.rand(vocab, generator=g) < 0.9] = -math.inf
+    x[2] = -math.inf
+    x[2, few] = torch.randn(5, generator=g).to(dtype)
+    x[3, vocab // 2:] = -math.inf
+    x[4, vocab - 1] = -math.inf
+    x[5] = -math.inf
+    x[5, few] = lowest                    # all that is left
+    x[6, ::3] = -math.inf
+    x[6, 1::3] = lowest
+    x[7, ::2] = -math.inf
+    x[7, 1] = math.nan
+    x[8, :vocab // 3] = -math.inf
+    tokens = torch.stack([(row > -math.inf).float().argmax() for row in x])
+    tokens[5] = few[0]
+    tokens[1:3] = torch.stack([row.float().argmax() for row in x[1:3]])
+    allowed = torch.ones(x.shape, dtype=torch.bool)
+    for temperature in (1.0, 0.3, 1e9):
+        temperatures = torch.full((9,), temperature, dtype=torch.float64)
+        for with_entropy in (True, False):
+            on_lp = torch.randn(9, generator=g)
+            on_h = torch.randn(9, generator=g) if with_entropy else torch.zeros(9)
+            grad = torch.full_like(x, 3.0, device="cuda")
+            out = scoring.token_logprobs(x.cuda(), tokens.cuda(), temperature=temperature, grad=grad, grad_logprobs=on_lp.cuda(),
+                                         grad_entropy=on_h.cuda() if with_entropy else None)
+            check_logprobs(x, tokens, temperatures, allowed, out, grad, on_lp, on_h)
+
+
+def test_lowest_values_over_a_small_temperature():
+    """A teacher and a student masked by float32's lowest value, which leaves
+    the range when divided: the same as masked by -inf."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    rows, vocab, k = 4, 900, 16
+    lowest = torch.finfo(torch.float32).min
+    student = torch.randn(rows, vocab, device="cuda", generator=g)
+    hidden = torch.rand(rows, vocab, device="cuda", generator=g) < 0.995
+    hidden[:, 3] = False
+    teacher = (student + 0.1).masked_fill(hidden, lowest)
+    assert bool((hidden.sum(1) > vocab - k).all())  # some of the k are lowest values
+    top = scoring.top_logits(teacher, k, temperature=0.25)
+    exact = scoring.top_logits(teacher.masked_fill(hidden, -math.inf), k, temperature=0.25)
+    kept = exact.ids >= 0
+    assert torch.equal(top.values[kept], exact.values[kept]) and bool((top.values[~kept] == lowest).all())
+    assert bool((top.rest == lowest).all()) and not bool(top.status.any())
+    grads = [torch.empty_like(student) for _ in range(2)]
+    for x in (student, student.masked_fill(hidden, lowest)):
+        one = scoring.distill_loss(x, top, temperature=0.25, grad=grads[0])
+        two = scoring.distill_loss(x, exact, temperature=0.25, grad=grads[1])
+        assert not bool(one.status.any()) and not bool(two.status.any())
+        torch.testing.assert_close(one.loss, two.loss, rtol=1e-5, atol=1e-6)
+        torch.testing.assert_close(grads[0], grads[1], rtol=1e-5, atol=1e-6)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=names)
