@@ -231,16 +231,21 @@ def committed_counts(out, requests: int):
 def committed_row_tokens(out, cu_rows, rows: int):
     """For every logits row of the step, the token it committed, or -1: row
     ``cu_rows[r] + d`` holds request r's d-th committed token (an accepted
-    draft, or the residual or bonus token), and the rows behind those, or of a
-    failed request, hold none. These are the tokens whose log-probabilities
+    draft, or the residual or bonus token), and the rows behind those, of a
+    failed request, or behind the last request, hold none. These are the tokens whose log-probabilities
     ``exactsample_b200.scoring.token_logprobs`` reports from the same logits."""
     import torch
 
-    row = torch.arange(rows, dtype=torch.int64, device=cu_rows.device)
+    row = torch.arange(rows, dtype=cu_rows.dtype, device=cu_rows.device)
+    requests = cu_rows.numel() - 1
+    if requests == 0 or rows == 0:
+        return torch.full((rows,), -1, dtype=out.tokens.dtype, device=cu_rows.device)
     request = torch.searchsorted(cu_rows[1:], row, right=True)
+    asked = request < requests  # logits may have rows behind the last request's
+    request = request.clamp(max=requests - 1)
     place = row - cu_rows[request]
-    committed = (out.status[request] == int(Status.OK)) & (place <= out.accepted_len[request])
-    return torch.where(committed, out.tokens[request, place], -1)
+    committed = asked & (out.status[request] == int(Status.OK)) & (place <= out.accepted_len[request])
+    return torch.where(committed, out.tokens[request, place.clamp(0, out.tokens.shape[1] - 1)], -1)
 
 
 class StatusCopy:

@@ -209,7 +209,16 @@ def test_committed_row_tokens():
     out = CudaOutput(tokens, torch.tensor([2, 0, 1, 0], dtype=torch.int32), torch.tensor([0, 0, 0, 2], dtype=torch.int32),
                      torch.zeros(4, dtype=torch.int32), 4)
     cu_rows = torch.tensor([0, 3, 5, 8, 9])  # request 2 accepted one of two drafts, request 3 failed
-    assert bridge.committed_row_tokens(out, cu_rows, 9).tolist() == [5, 6, 7, 8, -1, 9, 10, -1, -1]
+    for offsets in (cu_rows, cu_rows.int()):
+        assert bridge.committed_row_tokens(out, offsets, 9).tolist() == [5, 6, 7, 8, -1, 9, 10, -1, -1]
+        # Logits padded to more rows than the requests have, fewer rows, none, and no requests.
+        assert bridge.committed_row_tokens(out, offsets, 16).tolist() == [5, 6, 7, 8, -1, 9, 10, -1, -1] + [-1] * 7
+        assert bridge.committed_row_tokens(out, offsets, 4).tolist() == [5, 6, 7, 8]
+        assert bridge.committed_row_tokens(out, offsets, 0).tolist() == []
+        assert bridge.committed_row_tokens(out, offsets[:1], 3).tolist() == [-1, -1, -1]
+    # A request with no rows between others.
+    gap = CudaOutput(out.tokens[:3], out.accepted_len[:3], out.status[:3], out.path_used[:3], 3)
+    assert bridge.committed_row_tokens(gap, torch.tensor([0, 3, 3, 6]), 6).tolist() == [5, 6, 7, 9, 10, -1]
 
 
 # ---------------------------------------------------------------- the formulas
