@@ -1051,14 +1051,19 @@ template <int DT, int OP, bool GRAD> struct LossRow {
     const Total t = total_of(t_sum, tail && in.first > -INFINITY ? 1.f : 0.f,
                              pair_sum({in.first, 0.f}, negated(scaled_gap(value_top, 0.f, scale))));
     const Total q = total_of(q_sum, s, scaled_gap(m, x_top, scale));
-    float loss = 0.f, pull = 1.f;   // pull, of the tokens not kept: 1 - t_rest / q_rest
+    float loss = 0.f;
+    // Of the tokens not kept: their gradient is q_j - t_rest q_j / q_rest, in
+    // which their exponential against m is multiplied with this.
+    float others = q.other_share;
     bool lost = cross == INFINITY;  // the student has no mass where the teacher has some
     if (t_sum > 0.f) loss = (cross + t_sum * value_of(pair_sum(q.to_entries, negated(t.to_entries)))) * t.entry_share;
     if (t.other_share > 0.f) {
       // log t_rest - log q_rest
       const float off = value_of(pair_sum(pair_sum(q.to_others, negated(t.to_others)), negated(log_pair(s))));
       loss += t.other_share * off;
-      pull = -expm1f(off);
+      // Near t_rest = q_rest the difference would lose its digits. Elsewhere
+      // t_rest / q_rest may leave the range where its product with q does not.
+      others = fabsf(off) < 1.f ? -expm1f(off) * q.other_share : q.other_share - __fdiv_rn(t.other_share, s);
       lost |= !(s > 0.f);
     }
     const bool bad = (flags & BAD) || !(s < INFINITY) || !(t.total > 0.f && t.total < INFINITY) || (tail && !(in.first < INFINITY));
@@ -1075,7 +1080,7 @@ template <int DT, int OP, bool GRAD> struct LossRow {
       r.w = in.w * scale.hi;
       r.inv_q = q.entry_share;
       r.inv_t = t.entry_share;
-      set_scalars(r, m, scale.log2, s > 0.f ? r.w * pull * q.other_share : 0.f, 0.f, flags & CAREFUL || scale.log2 < SMALL_SCALE);
+      set_scalars(r, m, scale.log2, s > 0.f ? r.w * others : 0.f, 0.f, flags & CAREFUL || scale.log2 < SMALL_SCALE);
     }
   }
 
