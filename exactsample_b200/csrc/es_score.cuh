@@ -790,6 +790,11 @@ __device__ __forceinline__ float exp_beyond_first_order(float x, float exp_less_
   return sum * x * x;
 }
 
+// Above this an exponential of the row's scalars is taken in 64 bits, since
+// its product with an advantage or a coefficient may be in float32's range
+// where it is not.
+constexpr float WIDE = 80.f;
+
 // One row's scalars for the gradient: every token's is 2^d (a + b d), in the
 // fast form with d = z scale - r, in the careful form with d = (z - m) scale;
 // the row's token has its own.
@@ -931,22 +936,35 @@ template <int DT, int OP, bool GRAD> struct LossRow {
       slope = in.first;
       on_entropy = in.second;
     } else {
-      const float ratio = expf((lp.hi - in.first) + lp.lo);
+      const float rise_of_lp = (lp.hi - in.first) + lp.lo;
       // In 64 bits: where the ratio meets a border.
-      const double r = ratio, clipped = fmin(fmax(r, p.ratio_low), p.ratio_high);
+      const double r = rise_of_lp < WIDE ? double(expf(rise_of_lp)) : exp(double(rise_of_lp));
+      const double clipped = fmin(fmax(r, p.ratio_low), p.ratio_high);
       const bool through = r * in.second <= clipped * in.second;
-      loss = through ? -ratio * in.second : float(-clipped * in.second);
-      slope = through ? -ratio * in.second : 0.f;
+      loss = float(through ? -r * in.second : -clipped * in.second);
+      slope = through ? loss : 0.f;
       bad |= !isfinite(in.first) || !isfinite(in.second);
       if (p.ref_logprobs.p) {
-        const float x = (in.ref - lp.hi) - lp.lo, rise = expm1f(x);
-        kl = exp_beyond_first_order(x, rise);
-        loss += float(p.kl_coef) * kl;
-        slope -= float(p.kl_coef) * rise;
+        const float x = (in.ref - lp.hi) - lp.lo;
+        if (x < WIDE) {
+          const float rise = expm1f(x);
+          kl = exp_beyond_first_order(x, rise);
+          loss += float(p.kl_coef) * kl;
+          slope -= float(p.kl_coef) * rise;
+        } else {
+          // (A KL that is only watched is held at the largest number and
+          // leaves the loss alone.)
+          const double rise = exp(double(x)) - 1., wide = rise - x;
+          kl = float(fmin(wide, double(-LOWEST)));
+          if (p.kl_coef != 0.) {
+            loss += float(p.kl_coef * wide);
+            slope -= float(p.kl_coef * rise);
+          }
+        }
         bad |= !isfinite(in.ref);
       }
       loss -= float(p.entropy_coef) * h;
-      bad |= s > 0.f && isfinite(lp.hi) && !(isfinite(loss) && isfinite(slope) && isfinite(kl));
+      bad |= s > 0.f && isfinite(lp.hi) && !(isfinite(loss) && isfinite(slope));
       // Weights multiply as they are: an infinite or NaN one (an overflowed
       // loss scale) shows in the loss and the gradient.
       loss *= in.w;

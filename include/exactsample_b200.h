@@ -304,11 +304,15 @@ int es_top_logits(const es_top_args* args, void* stream);
 
 /* The clipped policy-ratio loss of each row's token, with r = exp(log p[token]
  * - old_logprobs), A = advantages, d = ref_logprobs - log p[token]:
- *   kl   = exp(d) - d - 1 (0 without ref_logprobs)
+ *   kl   = exp(d) - d - 1 (0 without ref_logprobs; float32's largest number
+ *          where it is beyond)
  *   loss = weights * (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
  *                     + kl_coef * kl - entropy_coef * H).
- * Where r A equals the clipped product the gradient goes through r. Negative
- * tokens as in es_token_logprobs. With `grad`: the gradient of the losses' sum. */
+ * Where r A equals the clipped product the gradient goes through r. A row whose
+ * loss, before its weight, or whose gradient by log p[token] is beyond
+ * float32's range is ES_INVALID_INPUT; with kl_coef 0 the KL takes no part in
+ * either. Negative tokens as in es_token_logprobs. With `grad`: the gradient of
+ * the losses' sum. */
 typedef struct es_policy_args {
   es_rows in;
   es_tensor tokens;        /* i64 [rows] */

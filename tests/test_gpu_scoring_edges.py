@@ -108,3 +108,69 @@ def test_distillation_where_the_student_has_almost_nothing_beside_the_kept(dtype
         limit = limit + w * slope.abs() * ref.HALF_STEP[dtype] * 1.01 + ref.SMALLEST[dtype]
         difference = (grad[r].cpu().double() - w * slope).abs()
         assert bool((difference <= limit).all()), (r, float((difference / limit).max()))
+
+
+# ---------------------------------------------------------------- policy
+def policy_case(rows=6, vocab=700, dtype=torch.float32, seed=11):
+    g = torch.Generator().manual_seed(seed)
+    x = ref.test_rows(g, rows, vocab, dtype)
+    tokens = torch.randint(vocab, (rows,), generator=g)
+    lp = torch.log_softmax(x.double(), 1).gather(1, tokens[:, None])[:, 0]
+    return g, x, tokens, lp
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
+def test_a_kl_that_is_only_watched_does_not_fail_its_row(dtype):
+    """kl_coef 0 with ref_logprobs: a KL beyond float32 is its largest number,
+    and the loss, its gradient and the log-probability are those without one."""
+    g, x, tokens, lp = policy_case(dtype=dtype)
+    gap = torch.tensor([1.0, 88.0, 89.0, 104.0, 800.0, 1e5])
+    old, adv = (lp - 0.05).float().cuda(), torch.randn(6, generator=g).cuda()
+    grads = [torch.full_like(x, 5.0, device="cuda") for _ in range(2)]
+    args = (x.cuda(), tokens.cuda(), old, adv)
+    watched = scoring.policy_loss(*args, ref_logprobs=(lp + gap).float().cuda(), entropy_coef=0.01, grad=grads[0])
+    without = scoring.policy_loss(*args, entropy_coef=0.01, grad=grads[1])
+    assert watched.status.cpu().tolist() == [0] * 6
+    for name in ("loss", "logprobs", "entropy", "status"):
+        assert torch.equal(getattr(watched, name), getattr(without, name)), name
+    assert torch.equal(*grads)
+    largest = torch.finfo(torch.float32).max
+    assert watched.kl[2:].cpu().tolist() == [largest] * 4
+    # exp(d) - 1 - d moves by a factor of d's error: log p's 2^-24 |log p|, the
+    # input's own rounding, d's two, and the sums' (2^-18 is above all of them).
+    for r, rise in ((0, 1.0), (1, 88.0)):
+        d = float((lp + gap).float()[r].double() - lp[r])
+        want = math.expm1(d) - d
+        assert abs(float(watched.kl[r]) - want) <= want * 2.0**-16 * max(1.0, 1 / rise)
+
+
+def test_losses_whose_factors_alone_leave_the_range():
+    """A ratio or a KL beyond float32 times a small advantage or coefficient."""
+    g, x, tokens, lp = policy_case()
+    x, tokens, lp = x[:4], tokens[:4], lp[:4]
+    old = torch.stack([lp[0] - 100, lp[1] - 95, lp[2], lp[3] - 100]).float()
+    adv = torch.tensor([-1e-8, -1e-6, 1.0, -1.0])
+    reference = torch.stack([lp[0], lp[1], lp[2] + 100, lp[3]]).float()
+    grad = torch.full_like(x, 5.0, device="cuda")
+    out = scoring.policy_loss(x.cuda(), tokens.cuda(), old.cuda(), adv.cuda(), ref_logprobs=reference.cuda(),
+                              kl_coef=1e-8, grad=grad)
+    assert out.status.cpu().tolist() == [0, 0, 0, 2]  # the last row's loss is beyond float32
+    p = torch.softmax(x.double(), 1)
+    for r in range(3):
+        ratio = math.exp(float(lp[r] - old[r].double()))
+        d = float(reference[r].double() - lp[r])
+        clipped = min(max(ratio, 0.8), 1.2)
+        a = float(adv[r])
+        through = ratio * a <= clipped * a
+        want = -min(ratio * a, clipped * a) + 1e-8 * (math.expm1(d) - d)
+        slope = (-ratio * a if through else 0.0) - 1e-8 * math.expm1(d)
+        # ratio and exp(d) move with log p: its rounding (2^-24 |log p|) and
+        # its sums' (sum_error), 2^-18 with room for their arguments' roundings
+        # at 100 (two of 2^-24 100 each).
+        relative = 2.0**-24 * (4 * 100 + 2 * abs(float(lp[r]))) + sum_error(x[r].double(), 700) + 2.0**-21
+        assert abs(float(out.loss[r]) - want) <= relative * max(abs(want), 1.0), r
+        row = -p[r] * slope
+        row[tokens[r]] += slope
+        limit = abs(slope) * (p[r] + (1 - p[r][tokens[r]]) * (torch.arange(700) == tokens[r])) * (2 * relative + 2.0**-20) + 1e-30
+        assert bool(((grad[r].cpu().double() - row).abs() <= limit).all()), r
+    assert float(out.kl[2]) == torch.finfo(torch.float32).max
