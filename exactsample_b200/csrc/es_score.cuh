@@ -929,6 +929,7 @@ template <int DT, int OP, bool GRAD> struct LossRow {
     const Pair log_s = log_pair(s), lp = pair_sum(scaled_gap(z, m, scale), negated(log_s));
     const float inv_s = __frcp_rn(s), gap = u * inv_s * float(LN2);  // log(s) - h
     const float h = value_of({log_s.hi, log_s.lo - gap});
+    const bool mass = z > -INFINITY && (in.mask >> (in.token & 31) & 1);
     // A NaN logit makes s NaN, +inf the maximum.
     bool bad = (flags & BAD) || !(s < INFINITY) || m == INFINITY || in.token >= p.in.vocab;
     float slope = 0.f, on_entropy = 0.f, loss = 0.f, kl = 0.f;  // gradients of lp and of h
@@ -964,7 +965,8 @@ template <int DT, int OP, bool GRAD> struct LossRow {
         bad |= !isfinite(in.ref);
       }
       loss -= float(p.entropy_coef) * h;
-      bad |= s > 0.f && isfinite(lp.hi) && !(isfinite(loss) && isfinite(slope));
+      // (Of a token without mass there is no loss that could leave the range.)
+      bad |= mass && !(isfinite(loss) && isfinite(slope));
       // Weights multiply as they are: an infinite or NaN one (an overflowed
       // loss scale) shows in the loss and the gradient.
       loss *= in.w;
@@ -974,7 +976,7 @@ template <int DT, int OP, bool GRAD> struct LossRow {
     int status = ES_OK;
     if (bad) status = ES_INVALID_INPUT;
     else if (s == 0.f) status = ES_NO_VALID_TOKEN;
-    else if (z == -INFINITY || !(in.mask >> (in.token & 31) & 1)) status = ES_DRAFT_ZERO_PROB;
+    else if (!mass) status = ES_DRAFT_ZERO_PROB;
     const bool ok = status == ES_OK;
     if (rank == 0)
       outputs(status, ok ? loss : 0.f, ok ? value_of(lp) : -INFINITY, ok ? kl : 0.f, ok ? h : 0.f);

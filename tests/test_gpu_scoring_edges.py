@@ -174,3 +174,26 @@ def test_losses_whose_factors_alone_leave_the_range():
         limit = abs(slope) * (p[r] + (1 - p[r][tokens[r]]) * (torch.arange(700) == tokens[r])) * (2 * relative + 2.0**-20) + 1e-30
         assert bool(((grad[r].cpu().double() - row).abs() <= limit).all()), r
     assert float(out.kl[2]) == torch.finfo(torch.float32).max
+
+
+@pytest.mark.parametrize("adv", [1.0, -1.0])
+@pytest.mark.parametrize("above", [10.0, 200.0, 1e30])
+def test_a_masked_token_is_one_without_probability(adv, above):
+    """Whatever its hidden logit is and wherever the ratio goes."""
+    g, x, tokens, _ = policy_case(rows=3)
+    allowed = torch.ones(3, 700, dtype=torch.bool)
+    allowed[torch.arange(3), tokens] = False
+    x[torch.arange(3), tokens] = above
+    x[1, tokens[1]] = -math.inf
+    mask = ref.pack_mask(allowed).cuda()
+    column = torch.tensor([-5.0, -5.0, -5.0]).cuda()
+    grad = torch.full_like(x, 5.0, device="cuda")
+    out = scoring.policy_loss(x.cuda(), tokens.cuda(), column, torch.full((3,), adv, device="cuda"), ref_logprobs=column,
+                              kl_coef=0.1, mask=mask, grad=grad)
+    alone = scoring.token_logprobs(x.cuda(), tokens.cuda(), mask=mask)
+    assert out.status.cpu().tolist() == alone.status.cpu().tolist() == [int(Status.DRAFT_ZERO_PROB)] * 3
+    assert bool((grad == 0).all()) and bool((out.loss == 0).all()) and bool((out.kl == 0).all())
+    # A bad input says so first, as it does for a token with probability.
+    column[2] = math.nan
+    out = scoring.policy_loss(x.cuda(), tokens.cuda(), column, torch.full((3,), adv, device="cuda"), mask=mask)
+    assert out.status.cpu().tolist() == [3, 3, 2]
