@@ -573,6 +573,15 @@ template <int DT> struct Slice {
 // number; its masked logits are -inf and held at MASKED in 32 bits.
 constexpr float MASKED = -1e30f;
 constexpr float SMALL_SCALE = 1e-20f;
+// The gradient 2^d (a + b d) is 0 at such a token if b d is finite: in float16
+// d is MASKED scale there at the lowest, elsewhere a logit may bring it down to
+// the type's lowest number. Rows with a larger b take the careful form, whose
+// d stops at FAR (a gradient with an entropy part of 1,024 rows of 151,936
+// bf16: 125 us, 129 in the careful form; a product more in every row's fast
+// form made a policy step of 4,096 rows 0.5 to 2 % slower).
+template <int DT> __device__ __forceinline__ float largest_b(float scale) {
+  return DT == ES_F16 ? __fdividef(1e8f, scale) : 0.99f;
+}
 template <int DT> __device__ __forceinline__ uint32_t masked_word() {
   if constexpr (DT == ES_F32) return __float_as_uint(MASKED);
   const typename Elem<DT>::T v = Elem<DT>::put(MASKED);
@@ -914,7 +923,7 @@ template <int DT, int OP, bool GRAD> struct LossRow {
   __device__ __forceinline__ void set_scalars(RowScalars& r, float m, float scale, float a, float b, bool careful) const {
     r.m = m;
     r.r = __fmul_rn(m, scale);
-    r.careful = careful || !(fabsf(r.r) <= LARGE_R);
+    r.careful = careful || !(fabsf(r.r) <= LARGE_R) || fabsf(b) > largest_b<DT>(scale);
     const float rest = r.careful ? 0.f : __fmaf_rn(m, scale, -r.r), x = rest * float(LN2);
     const float f = 1.f - x * (1.f - 0.5f * x);
     r.a = f * (a - b * rest);

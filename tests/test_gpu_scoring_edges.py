@@ -197,3 +197,50 @@ def test_a_masked_token_is_one_without_probability(adv, above):
     column[2] = math.nan
     out = scoring.policy_loss(x.cuda(), tokens.cuda(), column, torch.full((3,), adv, device="cuda"), mask=mask)
     assert out.status.cpu().tolist() == [3, 3, 2]
+
+
+# ---------------------------------------------------------------- far logits
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
+@pytest.mark.parametrize("far", [-1e30, -1.7e38, -2.3e38, "lowest", "mask", -math.inf])
+@pytest.mark.parametrize("incoming", [0.4, 3.0, -700.0, 65536.0, 1e12])
+def test_entropy_gradients_beside_very_low_logits(dtype, far, incoming):
+    """A token without probability has a gradient of 0, however far below the
+    others its logit lies and however large the incoming gradient is."""
+    lowest = torch.finfo(dtype).min
+    if not isinstance(far, str) and far != -math.inf and far < lowest:
+        pytest.skip("not a number of the type")
+    g = torch.Generator().manual_seed(3)
+    rows, vocab = 3, 4200
+    x = ref.test_rows(g, rows, vocab, dtype)
+    live = torch.rand(rows, vocab, generator=g) < 0.4
+    live[0] = False
+    live[0, [7, 4100]] = True       # a row of two tokens
+    live[1, :1100] = True           # the others lie behind a warp's first tokens
+    tokens = live.float().argmax(1)
+    mask = None
+    if far == "mask":
+        mask = ref.pack_mask(live).cuda()
+    else:
+        x = torch.where(live, x, torch.tensor(lowest if far == "lowest" else far).to(dtype))
+    on_lp = torch.tensor([0.5, -1.0, 2.0])
+    for temperature in (1.0, 2.0, 0.2):
+        grad = torch.full_like(x, 5.0, device="cuda")
+        out = scoring.token_logprobs(x.cuda(), tokens.cuda(), temperature=temperature, mask=mask, grad=grad,
+                                     grad_logprobs=on_lp.cuda(), grad_entropy=torch.full((rows,), incoming).cuda())
+        assert out.status.cpu().tolist() == [0] * rows
+        for r in range(rows):
+            logp = ref.logp_of(x[r].double(), live[r], temperature)
+            h = float(ref.entropy_of(logp))
+            p = logp.exp()
+            want = -p * float(on_lp[r]) - incoming * torch.where(live[r], p * (logp + h), 0.0)
+            want[tokens[r]] += float(on_lp[r])
+            want /= temperature
+            bounds = ref.RowBounds(logp, vocab)
+            bounds.sum = sum_error(x[r].double() / temperature if far != "mask" else
+                                   (x[r].double() / temperature).masked_fill(~live[r], -math.inf), vocab)
+            limit = ref.token_grad_bound(bounds, logp, want, int(tokens[r]), float(on_lp[r]), incoming, h, temperature, dtype)
+            got = grad[r].cpu().double()
+            over = want.abs() > torch.finfo(dtype).max  # (float16 and a large incoming gradient)
+            off = (got - want).abs()
+            assert bool((off <= limit)[~over].all()), (temperature, r, float((off / limit)[~over].max()))
+            assert bool((got[~live[r]] == 0).all())
