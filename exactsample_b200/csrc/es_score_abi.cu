@@ -41,6 +41,12 @@ bool addressable(const es_tensor& t, const char* name) {
   return true;
 }
 
+// The kernels load and store whole elements.
+int aligned(const es_tensor& t, const char* name, const char* whose = "its") {
+  if (numel(t) == 0 || reinterpret_cast<uintptr_t>(t.data) % element_size(t.dtype) == 0) return ES_SUCCESS;
+  return fail(ES_ERR_ALIGNMENT, std::string(name) + " must be aligned to " + whose + " elements");
+}
+
 // One call's tensors as they are checked: the inputs and the outputs.
 struct Tensors {
   const es_tensor* list[10];
@@ -64,8 +70,7 @@ struct Call {
       return fail(ES_ERR_ARGUMENT, "row operators require float16/bfloat16/float32 logits");
     if (logits.stride[0] < 0 || logits.stride[1] < 0) return fail(ES_ERR_ARGUMENT, "logits has a negative stride");
     if (!addressable(logits, "logits")) return ES_ERR_ARGUMENT;
-    if (reinterpret_cast<uintptr_t>(logits.data) % element_size(logits.dtype) != 0)
-      return fail(ES_ERR_ALIGNMENT, "logits must be aligned to their elements");
+    if (const int e = aligned(logits, "logits", "their"); e != ES_SUCCESS) return e;
     rows = logits.size[0];
     vocab = logits.size[1];
     if (vocab < 1) return fail(ES_ERR_ARGUMENT, "logits must have at least one column");
@@ -74,6 +79,7 @@ struct Call {
       if (!check(in.mask, ES_I32, 2, "mask") || !addressable(in.mask, "mask")) return ES_ERR_ARGUMENT;
       if (!(in.mask.size[0] == rows && in.mask.size[1] == (vocab + 31) / 32))
         return fail(ES_ERR_ARGUMENT, "mask shape mismatch");
+      if (const int e = aligned(in.mask, "mask"); e != ES_SUCCESS) return e;
       inputs.add(in.mask);
     }
     if (present(in.temperature)) {
@@ -87,21 +93,19 @@ struct Call {
     if (!check(t, dtype, 1, name) || !addressable(t, name)) return ES_ERR_ARGUMENT;
     if (t.size[0] != rows) return fail(ES_ERR_ARGUMENT, std::string(name) + " must have one value per row");
     list.add(t);
-    return ES_SUCCESS;
+    return aligned(t, name);
   }
   int grid(const es_tensor& t, int32_t dtype, int64_t width, const char* name, Tensors& list) {
     if (!check(t, dtype, 2, name) || !addressable(t, name)) return ES_ERR_ARGUMENT;
     if (t.size[0] != rows || t.size[1] != width) return fail(ES_ERR_ARGUMENT, std::string(name) + " shape mismatch");
     list.add(t);
-    return ES_SUCCESS;
+    return aligned(t, name);
   }
   // A gradient: apart from every other tensor, or the logits tensor itself.
   int gradient(const es_tensor& g) {
     if (!present(g)) return ES_SUCCESS;
     const es_tensor& l = in.logits;
     if (const int e = grid(g, l.dtype, vocab, "grad", outputs); e != ES_SUCCESS) return e;
-    if (reinterpret_cast<uintptr_t>(g.data) % element_size(g.dtype) != 0)
-      return fail(ES_ERR_ALIGNMENT, "grad must be aligned to its elements");
     if (g.data == l.data && g.stride[0] == l.stride[0] && g.stride[1] == l.stride[1])
       in_place = true;
     return ES_SUCCESS;

@@ -261,9 +261,10 @@ int es_ipc_free(void* ptr);
  * a gradient of zeros. A log-probability below float32's range (the type's
  * lowest logit over a temperature below 1) is float32's lowest number.
  *
- * A gradient has the logits' type and shape. It may be the logits tensor
- * itself (same address and strides): the row is then replaced by its
- * gradient. */
+ * Every tensor is aligned to its elements (ES_ERR_ALIGNMENT), with any strides
+ * that are not negative. A gradient has the logits' type and shape. It may be
+ * the logits tensor itself (same address and strides): the row is then
+ * replaced by its gradient. */
 typedef struct es_rows {
   es_tensor logits;       /* f32/f16/bf16 [rows, vocab] */
   es_tensor mask;         /* optional i32 [rows, ceil(vocab / 32)], as in es_args */
