@@ -244,6 +244,15 @@ std::tuple<Tensor, Tensor> distill_loss(const Tensor& logits, const Tensor& valu
 }
 
 // ---- row operators under autograd ----
+// Of forward-mode derivatives there are none, and a call that ran below
+// autograd would return its results with tangents of zero.
+template <class T> bool has_tangent(const T&) { return false; }
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const OptionalTensor& t) { return t.has_value() && has_tangent(*t); }
+template <class... A> void refuse_tangents(const A&... args) {
+  TORCH_CHECK(!(has_tangent(args) || ...), "row operators have no forward-mode derivative");
+}
+
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
@@ -348,6 +357,7 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
 std::tuple<Tensor, Tensor, Tensor> token_logprobs_tracked(const Tensor& logits, const Tensor& tokens,
                                                           const OptionalTensor& temperature, double temperature_all,
                                                           const OptionalTensor& mask) {
+  refuse_tangents(logits, temperature);
   const variable_list out = TokenLogprobs::apply(logits, tokens, temperature, temperature_all, mask);
   return {out[0], out[1], out[2]};
 }
@@ -356,6 +366,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> policy_loss_tracked(
     const OptionalTensor& ref_logprobs, const OptionalTensor& weights, const OptionalTensor& temperature,
     double temperature_all, const OptionalTensor& mask, double clip_low, double clip_high, double kl_coef,
     double entropy_coef) {
+  refuse_tangents(logits, old_logprobs, advantages, ref_logprobs, weights, temperature);
   const variable_list out = PolicyLoss::apply(logits, tokens, old_logprobs, advantages, ref_logprobs, weights, temperature,
                                               temperature_all, mask, clip_low, clip_high, kl_coef, entropy_coef);
   return {out[0], out[1], out[2], out[3], out[4]};
@@ -364,9 +375,23 @@ std::tuple<Tensor, Tensor> distill_loss_tracked(const Tensor& logits, const Tens
                                                 const OptionalTensor& rest, const OptionalTensor& weights,
                                                 const OptionalTensor& temperature, double temperature_all,
                                                 const OptionalTensor& mask) {
+  refuse_tangents(logits, values, rest, weights, temperature);
   const variable_list out = DistillLoss::apply(logits, values, ids, rest, weights, temperature, temperature_all, mask);
   return {out[0], out[1]};
 }
+// ---- the operators as the dispatcher calls them, below autograd ----
+constexpr char TOKEN_LOGPROBS[] = "exactsample::token_logprobs", TOP_LOGITS[] = "exactsample::top_logits",
+               POLICY_LOSS[] = "exactsample::policy_loss", DISTILL_LOSS[] = "exactsample::distill_loss";
+
+template <const char* NAME, class F> struct BelowAutograd;
+template <const char* NAME, class R, class... A> struct BelowAutograd<NAME, R(A...)> {
+  static R call(c10::DispatchKeySet keys, A... args) {
+    refuse_tangents(args...);
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(NAME, "").typed<R(A...)>();
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return op.redispatch(keys & c10::after_ADInplaceOrView_keyset, args...);
+  }
+};
 }  // namespace
 
 TORCH_LIBRARY(exactsample, m) {
@@ -406,4 +431,10 @@ TORCH_LIBRARY_IMPL(exactsample, CUDA, m) {
   m.impl("top_logits", &top_logits);
   m.impl("policy_loss", &policy_loss);
   m.impl("distill_loss", &distill_loss);
+}
+TORCH_LIBRARY_IMPL(exactsample, Autograd, m) {
+  m.impl("token_logprobs", &BelowAutograd<TOKEN_LOGPROBS, decltype(token_logprobs)>::call);
+  m.impl("top_logits", &BelowAutograd<TOP_LOGITS, decltype(top_logits)>::call);
+  m.impl("policy_loss", &BelowAutograd<POLICY_LOSS, decltype(policy_loss)>::call);
+  m.impl("distill_loss", &BelowAutograd<DISTILL_LOSS, decltype(distill_loss)>::call);
 }

@@ -24,7 +24,8 @@ Gradients come in two ways. With ``grad=`` a tensor of the logits' type and
 shape (the logits themselves too, which it then replaces), the call fills it
 with the gradient of the sum of the row losses: nothing is recorded for
 autograd. Without it, on logits that require a gradient, the result is
-differentiable by the logits, and the backward pass reads them a second time.
+differentiable by the logits, once and in reverse mode (forward-mode
+derivatives are refused), and the backward pass reads them a second time.
 To capture a whole training step in a CUDA graph, ``grad=`` is the way that
 does not depend on what autograd's accumulation nodes were made on.
 """
@@ -131,8 +132,7 @@ def top_logits(logits, k: int, *, temperature=1.0, mask=None) -> TopLogits:
     for autograd: it is a teacher's or a server's pass.
     """
     per_row, everywhere = _temperature(temperature)
-    return TopLogits(*_ops.top_logits(logits.detach() if logits.requires_grad else logits, k, per_row,
-                                              everywhere, mask))
+    return TopLogits(*_ops.top_logits(logits, k, per_row, everywhere, mask))
 
 
 def policy_loss(logits, tokens, old_logprobs, advantages, *, ref_logprobs=None, weights=None, temperature=1.0,

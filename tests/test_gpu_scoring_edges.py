@@ -244,3 +244,42 @@ def test_entropy_gradients_beside_very_low_logits(dtype, far, incoming):
             off = (got - want).abs()
             assert bool((off <= limit)[~over].all()), (temperature, r, float((off / limit)[~over].max()))
             assert bool((got[~live[r]] == 0).all())
+
+
+# ---------------------------------------------------------------- the calls
+def step_inputs(rows=6, vocab=700, seed=21):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    logits = torch.randn(rows, vocab, device="cuda", generator=g)
+    tokens = torch.randint(vocab, (rows,), device="cuda", generator=g)
+    columns = [torch.randn(rows, device="cuda", generator=g) - 6 * (i == 0) for i in range(3)]
+    return g, logits, tokens, columns, scoring.top_logits(logits * 0.8, 9)
+
+
+def operator_calls(tokens, columns, teacher):
+    return [lambda x, **kw: scoring.token_logprobs(x, tokens, **kw).logprobs,
+            lambda x, **kw: scoring.policy_loss(x, tokens, columns[0], columns[1], entropy_coef=0.1, **kw).loss,
+            lambda x, **kw: scoring.distill_loss(x, teacher, weights=columns[2], **kw).loss,
+            lambda x, **kw: scoring.top_logits(x, 5, **kw).rest]
+
+
+def test_forward_derivatives_are_refused():
+    """None has one: a tangent of zeros would pass for it."""
+    import torch.autograd.forward_ad as forward
+
+    _, logits, tokens, columns, teacher = step_inputs()
+    for call in operator_calls(tokens, columns, teacher):
+        want = call(logits)
+        with pytest.raises(RuntimeError, match="forward"):
+            torch.func.jvp(call, (logits,), (torch.ones_like(logits),))
+        for tracked in (False, True):
+            with forward.dual_level():
+                dual = forward.make_dual(logits.clone().requires_grad_(tracked), torch.ones_like(logits))
+                with pytest.raises(RuntimeError, match="forward"):
+                    call(dual)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward"):
+                    torch.ops.exactsample.token_logprobs(dual, tokens, None, 1.0, None, None, None, None)
+        assert torch.equal(call(logits), want)  # nothing is left behind
+    with forward.dual_level():  # an input other than the logits
+        weights = forward.make_dual(torch.ones(6, device="cuda"), torch.ones(6, device="cuda"))
+        with pytest.raises(RuntimeError, match="forward"):
+            scoring.policy_loss(logits, tokens, *columns[:2], weights=weights)

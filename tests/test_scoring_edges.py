@@ -1,7 +1,8 @@
 """Refusals of the row operators without a GPU, beside those of test_scoring.py."""
 import pytest
+import torch
 
-from exactsample_b200 import capi
+from exactsample_b200 import capi, scoring
 from tests.test_scoring import OPERATORS, arguments, call
 
 OPTIONAL = {"es_token_logprobs": ("grad", "grad_logprobs", "grad_entropy"), "es_top_logits": (),
@@ -19,3 +20,29 @@ def test_every_tensor_is_aligned_to_its_elements(name, field):
         tensor = getattr(a.rows if field in ("mask", "temperature") else a, field)
         tensor.data += shift
         assert call(name, a) == (-3, f"{field} must be aligned to its elements"), shift
+
+
+def test_forward_derivatives_are_refused():
+    """None of the operators has one: a tangent of zeros would pass for it.
+    (The check comes before the device's, so that it needs no GPU.)"""
+    import torch.autograd.forward_ad as forward
+
+    x, tokens, column = torch.randn(3, 8), torch.zeros(3, dtype=torch.int64), torch.zeros(3)
+    teacher = scoring.TopLogits(torch.zeros(3, 2), torch.arange(6).view(3, 2), column)
+    calls = [lambda z: scoring.token_logprobs(z, tokens).logprobs, lambda z: scoring.top_logits(z, 2).values,
+             lambda z: scoring.policy_loss(z, tokens, column, column).loss, lambda z: scoring.distill_loss(z, teacher).loss]
+    for call_of in calls:
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            torch.func.jvp(call_of, (x,), (torch.ones_like(x),))
+        for tracked in (False, True):
+            with forward.dual_level():
+                dual = forward.make_dual(x.clone().requires_grad_(tracked), torch.ones_like(x))
+                with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call_of(dual)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call_of(dual)
+    with forward.dual_level():  # of an input beside the logits
+        weights = forward.make_dual(torch.ones(3), torch.ones(3))
+        for z in (x, x.clone().requires_grad_()):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                scoring.policy_loss(z, tokens, column, column, weights=weights)
