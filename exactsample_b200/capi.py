@@ -21,7 +21,7 @@ ERRORS = {0: "ES_SUCCESS", -1: "ES_ERR_ARGUMENT", -2: "ES_ERR_CAPACITY", -3: "ES
 # Every function the header declares.
 EXPORTS = ["es_workspace_bytes", "es_verify", "es_verify_timed", "es_verify_static", "es_verify_sharded",
            "es_shard_exchange_bytes", "es_shard_signal", "es_shard_wait", "es_shard_finish", "es_ipc_alloc", "es_ipc_open", "es_ipc_close", "es_ipc_free",
-           "es_token_logprobs", "es_top_logits", "es_policy_loss", "es_distill_loss",
+           "es_token_logprobs", "es_top_logits", "es_policy_loss", "es_distill_loss", "es_distill_loss_status",
            "es_last_error", "es_abi_version"]
 MAX_SHARDS = 8  # ES_MAX_SHARDS
 STATIC_MAX_ROWS = 4096  # ES_STATIC_MAX_ROWS
@@ -120,6 +120,8 @@ def load(path: str | Path | None = None) -> ctypes.CDLL:
         for name, args in ROW_OPERATORS.items():
             getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
             getattr(lib, name).restype = ctypes.c_int
+        lib.es_distill_loss_status.argtypes = [ctypes.POINTER(DistillArgs), ctypes.POINTER(Tensor), ctypes.c_void_p]
+        lib.es_distill_loss_status.restype = ctypes.c_int
         lib.es_last_error.argtypes = []
         lib.es_last_error.restype = ctypes.c_char_p
         lib.es_abi_version.argtypes = []
@@ -220,8 +222,9 @@ def row_operator(name: str, tensors: dict, *, stream=None, temperature_all: floa
 
     ``tensors`` maps the operator's field names, and ``logits``, ``mask`` and
     ``temperature``, to tensors (optional ones may be absent or None);
-    ``scalars`` are es_policy_args' coefficients. ``stream`` is a
-    torch.cuda.Stream (default: current).
+    ``scalars`` are es_policy_args' coefficients. es_distill_loss takes a
+    ``teacher_status`` beside its fields. ``stream`` is a torch.cuda.Stream
+    (default: current).
     """
     import torch
 
@@ -235,4 +238,8 @@ def row_operator(name: str, tensors: dict, *, stream=None, temperature_all: floa
         setattr(args.rows, field, describe(tensors.get(field)))
     args.rows.temperature_all = temperature_all
     s = (stream or torch.cuda.current_stream()).cuda_stream
-    check(getattr(load(), name)(ctypes.byref(args), ctypes.c_void_p(s)))
+    if name == "es_distill_loss" and tensors.get("teacher_status") is not None:
+        teacher_status = describe(tensors["teacher_status"])
+        check(load().es_distill_loss_status(ctypes.byref(args), ctypes.byref(teacher_status), ctypes.c_void_p(s)))
+    else:
+        check(getattr(load(), name)(ctypes.byref(args), ctypes.c_void_p(s)))

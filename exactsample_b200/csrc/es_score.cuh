@@ -93,6 +93,7 @@ struct LossParams {
   Grid2<const float> values;
   Grid2<const int64_t> ids;
   Column<const float> rest;
+  Column<const int32_t> teacher_status;
   int32_t k;
   Column<float> loss, logprobs, kl, entropy;
   Column<int32_t> status;
@@ -1311,7 +1312,11 @@ template <int DT, int OP, bool GRAD> struct LossRow {
           loaded = false;
         }
         if (GRAD) zero_grad();
-        if (rank == 0 && tid == 0) outputs(ES_OK, 0.f, 0.f, 0.f, 0.f);
+        if (rank == 0 && tid == 0) {
+          // (A teacher's row that failed has no entries either.)
+          const int status = OP == DISTILL && p.teacher_status.p ? p.teacher_status[row] : ES_OK;
+          outputs(status, 0.f, 0.f, 0.f, 0.f);
+        }
         continue;
       }
       uint32_t* const words = masked ? masks + (turn & 1) * (p.in.slice / 32) : nullptr;

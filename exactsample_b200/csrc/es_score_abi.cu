@@ -250,7 +250,7 @@ int policy_loss(const es_policy_args* a, cudaStream_t stream) {
   return run_loss(call, p, a->grad, POLICY, stream);
 }
 
-int distill_loss(const es_distill_args* a, cudaStream_t stream) {
+int distill_loss(const es_distill_args* a, const es_tensor* teacher_status, cudaStream_t stream) {
   Call call{a->in};
   int e = call.begin();
   if (e != ES_SUCCESS) return e;
@@ -260,10 +260,13 @@ int distill_loss(const es_distill_args* a, cudaStream_t stream) {
   if (e == ES_SUCCESS) e = call.grid(a->ids, ES_I64, k, "ids", call.inputs);
   if (e == ES_SUCCESS && present(a->rest)) e = call.column(a->rest, ES_F32, "rest", call.inputs);
   if (e == ES_SUCCESS && present(a->weights)) e = call.column(a->weights, ES_F32, "weights", call.inputs);
+  const bool of_teacher = teacher_status != nullptr && present(*teacher_status);
+  if (e == ES_SUCCESS && of_teacher) e = call.column(*teacher_status, ES_I32, "teacher_status", call.inputs);
   if (e == ES_SUCCESS) e = call.column(a->loss, ES_F32, "loss", call.outputs);
   if (e == ES_SUCCESS) e = call.column(a->status, ES_I32, "status", call.outputs);
   if (e != ES_SUCCESS) return e;
   LossParams p{};
+  if (of_teacher) p.teacher_status = col<const int32_t>(*teacher_status);
   p.values = grid2<const float>(a->values);
   p.ids = grid2<const int64_t>(a->ids);
   p.rest = col<const float>(a->rest);
@@ -311,7 +314,7 @@ int top_logits(const es_top_args* a, cudaStream_t stream) {
 }
 
 // No exception leaves a C entry point.
-template <class A> int guarded(const A* args, void* stream, int (*f)(const A*, cudaStream_t)) {
+template <class A, class F> int guarded(const A* args, void* stream, F f) {
   try {
     g_error.clear();
     if (args == nullptr) return fail(ES_ERR_ARGUMENT, "null arguments");
@@ -325,6 +328,9 @@ template <class A> int guarded(const A* args, void* stream, int (*f)(const A*, c
 extern "C" {
 int es_token_logprobs(const es_logprob_args* args, void* stream) { return guarded(args, stream, token_logprobs); }
 int es_policy_loss(const es_policy_args* args, void* stream) { return guarded(args, stream, policy_loss); }
-int es_distill_loss(const es_distill_args* args, void* stream) { return guarded(args, stream, distill_loss); }
+int es_distill_loss(const es_distill_args* args, void* stream) { return es_distill_loss_status(args, nullptr, stream); }
+int es_distill_loss_status(const es_distill_args* args, const es_tensor* teacher_status, void* stream) {
+  return guarded(args, stream, [=](const es_distill_args* a, cudaStream_t s) { return distill_loss(a, teacher_status, s); });
+}
 int es_top_logits(const es_top_args* args, void* stream) { return guarded(args, stream, top_logits); }
 }  // extern "C"

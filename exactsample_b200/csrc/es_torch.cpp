@@ -227,7 +227,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> policy_loss(
 std::tuple<Tensor, Tensor> distill_loss(const Tensor& logits, const Tensor& values, const Tensor& ids,
                                         const OptionalTensor& rest, const OptionalTensor& weights,
                                         const OptionalTensor& temperature, double temperature_all,
-                                        const OptionalTensor& mask, const OptionalTensor& grad) {
+                                        const OptionalTensor& mask, const OptionalTensor& grad,
+                                        const OptionalTensor& teacher_status) {
   const RowCall call(logits);
   auto [loss, status, _2, _3, _4] = call.columns(1);
   es_distill_args a{};
@@ -239,7 +240,8 @@ std::tuple<Tensor, Tensor> distill_loss(const Tensor& logits, const Tensor& valu
   a.loss = describe(loss);
   a.status = describe(status);
   a.grad = call.write(grad, "grad");
-  call.done(es_distill_loss(&a, call.stream.stream()));
+  const es_tensor failed = call.use(teacher_status, "teacher_status");
+  call.done(es_distill_loss_status(&a, &failed, call.stream.stream()));
   return {loss, status};
 }
 
@@ -331,26 +333,27 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
 struct DistillLoss : torch::autograd::Function<DistillLoss> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& values, const Tensor& ids,
                                const OptionalTensor& rest, const OptionalTensor& weights, const OptionalTensor& temperature,
-                               double temperature_all, const OptionalTensor& mask) {
+                               double temperature_all, const OptionalTensor& mask, const OptionalTensor& teacher_status) {
     ctx->save_for_backward({logits, values, ids, or_undefined(rest), or_undefined(weights), or_undefined(temperature),
                             or_undefined(mask)});
     ctx->saved_data["temperature"] = temperature_all;
     ctx->set_materialize_grads(false);
-    auto [loss, status] = distill_loss(logits, values, ids, rest, weights, temperature, temperature_all, mask, std::nullopt);
+    auto [loss, status] = distill_loss(logits, values, ids, rest, weights, temperature, temperature_all, mask, std::nullopt,
+                                       teacher_status);
     ctx->mark_non_differentiable({status});
     return {loss, status};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& out) {
-    if (!out[0].defined()) return variable_list(8);
+    if (!out[0].defined()) return variable_list(9);
     const variable_list saved = ctx->get_saved_variables();
     Tensor grad;
     {
       const at::NoGradGuard unrecorded;
       grad = at::empty_like(saved[0]);
       distill_loss(saved[0], saved[1], saved[2], or_none(saved[3]), weighted(saved[4], out[0]), or_none(saved[5]),
-                   ctx->saved_data["temperature"].toDouble(), or_none(saved[6]), grad);
+                   ctx->saved_data["temperature"].toDouble(), or_none(saved[6]), grad, std::nullopt);
     }
-    return logits_gradient(grad, 7);
+    return logits_gradient(grad, 8);
   }
 };
 
@@ -374,9 +377,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> policy_loss_tracked(
 std::tuple<Tensor, Tensor> distill_loss_tracked(const Tensor& logits, const Tensor& values, const Tensor& ids,
                                                 const OptionalTensor& rest, const OptionalTensor& weights,
                                                 const OptionalTensor& temperature, double temperature_all,
-                                                const OptionalTensor& mask) {
+                                                const OptionalTensor& mask, const OptionalTensor& teacher_status) {
   refuse_tangents(logits, values, rest, weights, temperature);
-  const variable_list out = DistillLoss::apply(logits, values, ids, rest, weights, temperature, temperature_all, mask);
+  const variable_list out = DistillLoss::apply(logits, values, ids, rest, weights, temperature, temperature_all, mask,
+                                               teacher_status);
   return {out[0], out[1]};
 }
 // ---- the operators as the dispatcher calls them, below autograd ----
@@ -413,7 +417,7 @@ TORCH_LIBRARY(exactsample, m) {
       "float kl_coef, float entropy_coef, Tensor(a!)? grad) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def(
       "distill_loss(Tensor logits, Tensor values, Tensor ids, Tensor? rest, Tensor? weights, Tensor? temperature, "
-      "float temperature_all, Tensor? mask, Tensor(a!)? grad) -> (Tensor, Tensor)");
+      "float temperature_all, Tensor? mask, Tensor(a!)? grad, Tensor? teacher_status=None) -> (Tensor, Tensor)");
   m.def(
       "token_logprobs_tracked(Tensor logits, Tensor tokens, Tensor? temperature, float temperature_all, Tensor? mask) "
       "-> (Tensor, Tensor, Tensor)", &token_logprobs_tracked);
@@ -423,7 +427,8 @@ TORCH_LIBRARY(exactsample, m) {
       "float kl_coef, float entropy_coef) -> (Tensor, Tensor, Tensor, Tensor, Tensor)", &policy_loss_tracked);
   m.def(
       "distill_loss_tracked(Tensor logits, Tensor values, Tensor ids, Tensor? rest, Tensor? weights, "
-      "Tensor? temperature, float temperature_all, Tensor? mask) -> (Tensor, Tensor)", &distill_loss_tracked);
+      "Tensor? temperature, float temperature_all, Tensor? mask, Tensor? teacher_status=None) -> (Tensor, Tensor)",
+      &distill_loss_tracked);
 }
 TORCH_LIBRARY_IMPL(exactsample, CUDA, m) {
   m.impl("verify_out", &verify_out);

@@ -164,8 +164,9 @@ def distill_loss(logits, teacher: TopLogits, *, weights=None, temperature=1.0, m
     same ``temperature``. With ``tail`` the teacher's remaining probability is
     held against the student's as one bucket; without it the teacher is
     renormalised over the tokens it kept. Entries with a negative id are
-    unused, and a row without used entries is padding. ``mask`` limits the
-    student. The loss is that of probabilities at ``temperature``: multiply it
+    unused, and a row without used entries is padding, unless the record's
+    ``status`` says that the teacher's row failed: then it has that status (its
+    loss is 0 and its gradient zeros as well). ``mask`` limits the student. The loss is that of probabilities at ``temperature``: multiply it
     (or ``weights``) by the temperature squared for gradients that keep their
     scale across temperatures.
     """
@@ -175,6 +176,6 @@ def distill_loss(logits, teacher: TopLogits, *, weights=None, temperature=1.0, m
     rest = teacher.rest if tail else None
     if _tracked(logits, grad, teacher.values, rest, weights, per_row):
         return DistillLoss(*_ops.distill_loss_tracked(logits, teacher.values, teacher.ids, rest, weights, per_row,
-                                                      everywhere, mask))
+                                                      everywhere, mask, teacher.status))
     return DistillLoss(*_ops.distill_loss(logits, teacher.values, teacher.ids, rest, weights, per_row,
-                                                  everywhere, mask, grad))
+                                          everywhere, mask, grad, teacher.status))

@@ -355,6 +355,10 @@ typedef struct es_distill_args {
   es_tensor grad;     /* optional out, the logits' type, [rows, vocab] */
 } es_distill_args;
 int es_distill_loss(const es_distill_args* args, void* stream);
+/* The same, against a record of which rows may have failed: teacher_status
+ * (i32 [rows]; null: as above) is the record's. A row without used entries,
+ * which is what a failed row's record is, then has the teacher's status. */
+int es_distill_loss_status(const es_distill_args* args, const es_tensor* teacher_status, void* stream);
 
 /* The message of the last error returned on this thread ("" after success). */
 const char* es_last_error(void);

@@ -283,3 +283,38 @@ def test_forward_derivatives_are_refused():
         weights = forward.make_dual(torch.ones(6, device="cuda"), torch.ones(6, device="cuda"))
         with pytest.raises(RuntimeError, match="forward"):
             scoring.policy_loss(logits, tokens, *columns[:2], weights=weights)
+
+
+def test_a_teacher_that_failed_is_not_padding():
+    """Rows whose record is empty because the teacher's row failed have the
+    teacher's status; padded rows are as they were."""
+    g, logits, tokens, columns, _ = step_inputs()
+    teacher_logits = logits * 0.8
+    teacher_logits[1, 5] = math.nan
+    teacher_logits[3] = -math.inf
+    teacher = scoring.top_logits(teacher_logits, 9)
+    assert teacher.status.cpu().tolist() == [0, 2, 0, 1, 0, 0]
+    teacher.ids[4] = -1  # padding
+    kept = torch.tensor([0, 2, 5])
+    for weights in (None, columns[2]):
+        grad = torch.full_like(logits, 5.0)
+        out = scoring.distill_loss(logits, teacher, weights=weights, grad=grad)
+        alone = scoring.distill_loss(logits, teacher, weights=weights)
+        leaf = logits.clone().requires_grad_()
+        tracked = scoring.distill_loss(leaf, teacher, weights=weights)
+        tracked.loss.sum().backward()
+        assert torch.equal(leaf.grad, grad)
+        for got in (out, alone, tracked):
+            assert got.status.cpu().tolist() == [0, 2, 0, 1, 0, 0]
+            assert bool((got.loss[[1, 3, 4]] == 0).all()) and bool((got.loss[kept.cuda()] != 0).all())
+        assert bool((grad[[1, 3, 4]] == 0).all()) and bool((grad[kept.cuda()] != 0).any(1).all())
+        # Without the record's statuses an empty row is padding.
+        bare = scoring.TopLogits(teacher.values, teacher.ids, teacher.rest)
+        again = scoring.distill_loss(logits, bare, weights=weights)
+        assert again.status.cpu().tolist() == [0] * 6 and torch.equal(again.loss, out.loss)
+    # A strided column of statuses, and one of the wrong type.
+    wide = torch.stack([teacher.status, teacher.status + 7], 1)
+    strided = scoring.TopLogits(teacher.values, teacher.ids, teacher.rest, wide[:, 0])
+    assert scoring.distill_loss(logits, strided).status.cpu().tolist() == [0, 2, 0, 1, 0, 0]
+    with pytest.raises(RuntimeError, match="teacher_status has wrong"):
+        scoring.distill_loss(logits, scoring.TopLogits(teacher.values, teacher.ids, teacher.rest, teacher.status.long()))

@@ -1,4 +1,7 @@
 """Refusals of the row operators without a GPU, beside those of test_scoring.py."""
+import ctypes
+
+import numpy as np
 import pytest
 import torch
 
@@ -46,3 +49,23 @@ def test_forward_derivatives_are_refused():
         for z in (x, x.clone().requires_grad_()):
             with pytest.raises(RuntimeError, match="no forward-mode derivative"):
                 scoring.policy_loss(z, tokens, column, column, weights=weights)
+
+
+def test_a_teachers_statuses_are_checked():
+    lib = capi.load()
+
+    def with_status(a, status):
+        code = lib.es_distill_loss_status(ctypes.byref(a), None if status is None else ctypes.byref(status), None)
+        return code, lib.es_last_error().decode()
+    a = arguments("es_distill_loss")
+    good = a._host.t((3,), np.int32, capi.ES_I32)
+    assert with_status(a, good)[0] == with_status(a, None)[0] == with_status(a, capi.Tensor())[0] == -7
+    assert with_status(a, a._host.t((3,), np.int64, capi.ES_I64)) == (-1, "teacher_status has wrong device, dtype or rank")
+    assert with_status(a, a._host.t((2,), np.int32, capi.ES_I32)) == (-1, "teacher_status must have one value per row")
+    between = capi.Tensor.from_buffer_copy(good)
+    between.data += 2
+    assert with_status(a, between) == (-3, "teacher_status must be aligned to its elements")
+    assert with_status(a, a.status) == (-4, "exactsample input/output aliasing is forbidden")
+    assert lib.es_distill_loss_status(None, None, None) == -1
+    empty = arguments("es_distill_loss", rows=0)
+    assert with_status(empty, empty._host.t((0,), np.int32, capi.ES_I32)) == (0, "")
