@@ -142,18 +142,26 @@ struct RowCall {
     r.temperature_all = temperature_all;
     return r;
   }
-  // The call's per-row outputs, `floats` of float32 and the statuses last, side
-  // by side in one allocation (each starts on 16 bytes).
+  // The call's per-row outputs: `floats` of float32 side by side in one
+  // allocation (each starts on 16 bytes), then the statuses in one of their own,
+  // since tensors of two types in one storage cannot be saved to one file.
+  // (Straight from the allocator: the host's part of a small call is 8.4 us, and
+  // was 8.2 with all of them in one at::empty.)
   std::array<Tensor, 5> columns(int floats) const {
     const int64_t rows = logits.size(0), width = (rows + 3) / 4 * 4;
-    const Tensor all = at::empty({width * (floats + 1)}, logits.options().dtype(at::kFloat));
+    const auto memory = [](int64_t words) {
+      return c10::Storage(c10::Storage::use_byte_size_t(), size_t(words) * 4, c10::GetAllocator(at::kCUDA), /*resizable=*/true);
+    };
+    const auto column = [rows](c10::Storage storage, int64_t offset, caffe2::TypeMeta type) {
+      Tensor t = at::detail::make_tensor<c10::TensorImpl>(std::move(storage), c10::DispatchKeySet(c10::DispatchKey::CUDA), type);
+      t.unsafeGetTensorImpl()->set_storage_offset(offset);
+      t.unsafeGetTensorImpl()->set_sizes_contiguous({rows});
+      return t;
+    };
+    const c10::Storage all = memory(width * floats);
     std::array<Tensor, 5> out;
-    for (int i = 0; i <= floats; ++i) {
-      const auto type = i < floats ? caffe2::TypeMeta::Make<float>() : caffe2::TypeMeta::Make<int32_t>();
-      out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), type);
-      out[i].unsafeGetTensorImpl()->set_storage_offset(width * i);
-      out[i].unsafeGetTensorImpl()->set_sizes_contiguous({rows});
-    }
+    for (int i = 0; i < floats; ++i) out[i] = column(all, width * i, caffe2::TypeMeta::Make<float>());
+    out[floats] = column(memory(rows), 0, caffe2::TypeMeta::Make<int32_t>());
     return out;
   }
   static void done(int result) { TORCH_CHECK(result == ES_SUCCESS, es_last_error()); }

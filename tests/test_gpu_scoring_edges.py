@@ -318,3 +318,15 @@ def test_a_teacher_that_failed_is_not_padding():
     assert scoring.distill_loss(logits, strided).status.cpu().tolist() == [0, 2, 0, 1, 0, 0]
     with pytest.raises(RuntimeError, match="teacher_status has wrong"):
         scoring.distill_loss(logits, scoring.TopLogits(teacher.values, teacher.ids, teacher.rest, teacher.status.long()))
+
+
+def test_results_are_saved_together(tmp_path):
+    """Log-probabilities and statuses of one call in one file."""
+    _, logits, tokens, columns, teacher = step_inputs()
+    outs = [scoring.token_logprobs(logits, tokens), scoring.policy_loss(logits, tokens, *columns[:2]),
+            scoring.distill_loss(logits, teacher), teacher]
+    for out in outs:
+        whole = {name: getattr(out, name) for name in out.__slots__}
+        torch.save(whole, tmp_path / "results.pt")
+        again = torch.load(tmp_path / "results.pt")
+        assert all(torch.equal(again[name], whole[name]) for name in whole)
