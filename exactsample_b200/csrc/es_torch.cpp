@@ -119,7 +119,9 @@ struct RowCall {
   }
   explicit RowCall(const Tensor& l)
       : logits(l), guard(device_of(l)), stream(c10::cuda::getCurrentCUDAStream(l.device().index())),
-        capturing(c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {}
+        // (The default stream is never captured.)
+        capturing(stream.stream() != nullptr &&
+                  c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {}
 
   es_tensor use(const Tensor& t, const char* name) const {
     TORCH_CHECK(t.device() == logits.device(), name, " has wrong device, dtype or rank");
@@ -145,8 +147,9 @@ struct RowCall {
   // The call's per-row outputs: `floats` of float32 side by side in one
   // allocation (each starts on 16 bytes), then the statuses in one of their own,
   // since tensors of two types in one storage cannot be saved to one file.
-  // (Straight from the allocator: the host's part of a small call is 8.4 us, and
-  // was 8.2 with all of them in one at::empty.)
+  // (Straight from the allocator: the host's part of a small call is 8.0 us, and
+  // was 8.2 with all of them in one at::empty; with a storage for each output a
+  // policy loss takes it 12 instead of 10.)
   std::array<Tensor, 5> columns(int floats) const {
     const int64_t rows = logits.size(0), width = (rows + 3) / 4 * 4;
     const auto memory = [](int64_t words) {
