@@ -256,6 +256,64 @@ std::tuple<Tensor, Tensor> distill_loss(const Tensor& logits, const Tensor& valu
   return {loss, status};
 }
 
+// ---- row operators on tensors without memory: what tracing asks for ----
+// The checks that the kind of the inputs decides; the results' shapes and types.
+struct Traced {
+  Tensor column, status;
+  explicit Traced(const Tensor& logits) {
+    TORCH_CHECK(logits.dim() == 2, "logits must be a 2D CUDA tensor");
+    const auto type = logits.scalar_type();
+    TORCH_CHECK(type == at::kFloat || type == at::kHalf || type == at::kBFloat16,
+                "row operators require float16/bfloat16/float32 logits");
+    column = at::empty_symint({logits.sym_size(0)}, logits.options().dtype(at::kFloat));
+    status = at::empty_symint({logits.sym_size(0)}, logits.options().dtype(at::kInt));
+  }
+  Tensor one() const { return at::empty_like(column); }
+};
+std::tuple<Tensor, Tensor, Tensor> token_logprobs_meta(const Tensor& logits, const Tensor&, const OptionalTensor&, double,
+                                                       const OptionalTensor&, const OptionalTensor&, const OptionalTensor&,
+                                                       const OptionalTensor&) {
+  const Traced t(logits);
+  return {t.one(), t.one(), t.status};
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor> top_logits_meta(const Tensor& logits, int64_t k, const OptionalTensor&, double,
+                                                           const OptionalTensor&) {
+  const Traced t(logits);
+  TORCH_CHECK(k >= 1 && k <= ES_MAX_TOP, "k must be in [1, 256]");
+  const std::array<c10::SymInt, 2> shape{logits.sym_size(0), k};
+  return {at::empty_symint(shape, t.column.options()), at::empty_symint(shape, t.column.options().dtype(at::kLong)), t.one(),
+          t.status};
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> policy_loss_meta(
+    const Tensor& logits, const Tensor&, const Tensor&, const Tensor&, const OptionalTensor&, const OptionalTensor&,
+    const OptionalTensor&, double, const OptionalTensor&, double, double, double, double, const OptionalTensor&) {
+  const Traced t(logits);
+  return {t.one(), t.one(), t.one(), t.one(), t.status};
+}
+std::tuple<Tensor, Tensor> distill_loss_meta(const Tensor& logits, const Tensor&, const Tensor&, const OptionalTensor&,
+                                             const OptionalTensor&, const OptionalTensor&, double, const OptionalTensor&,
+                                             const OptionalTensor&, const OptionalTensor&) {
+  const Traced t(logits);
+  return {t.one(), t.status};
+}
+
+// ---- the operators as the dispatcher has them ----
+constexpr char TOKEN_LOGPROBS[] = "exactsample::token_logprobs", TOP_LOGITS[] = "exactsample::top_logits",
+               POLICY_LOSS[] = "exactsample::policy_loss", DISTILL_LOSS[] = "exactsample::distill_loss";
+template <const char* NAME, class F> const c10::TypedOperatorHandle<F>& dispatched() {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(NAME, "").typed<F>();
+  return op;
+}
+// One of them from inside an autograd function: directly, or, for a call that
+// is being traced, so that the tracer sees it.
+template <const char* NAME, class R, class... A, class... B>
+R call_or_trace(R (*f)(A...), const Tensor& logits, B&&... args) {
+  const c10::DispatchKeySet traced{c10::DispatchKey::Python, c10::DispatchKey::Functionalize};
+  if (c10::impl::dispatch_mode_enabled() || logits.key_set().has_any(traced) || logits.is_meta())
+    return dispatched<NAME, R(A...)>().call(logits, std::forward<B>(args)...);
+  return f(logits, std::forward<B>(args)...);
+}
+
 // ---- row operators under autograd ----
 // Of forward-mode derivatives there are none, and a call that ran below
 // autograd would return its results with tangents of zero.
@@ -293,7 +351,8 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     ctx->saved_data["temperature"] = temperature_all;
     ctx->set_materialize_grads(false);
     auto [logprobs, entropy, status] =
-        token_logprobs(logits, tokens, temperature, temperature_all, mask, std::nullopt, std::nullopt, std::nullopt);
+        call_or_trace<TOKEN_LOGPROBS>(token_logprobs, logits, tokens, temperature, temperature_all, mask, std::nullopt,
+                                      std::nullopt, std::nullopt);
     ctx->mark_non_differentiable({status});
     return {logprobs, entropy, status};
   }
@@ -304,8 +363,9 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     {
       const at::NoGradGuard unrecorded;
       grad = at::empty_like(saved[0]);
-      token_logprobs(saved[0], saved[1], or_none(saved[2]), ctx->saved_data["temperature"].toDouble(), or_none(saved[3]),
-                     grad, or_none(out[0]), or_none(out[1]));
+      call_or_trace<TOKEN_LOGPROBS>(token_logprobs, saved[0], saved[1], or_none(saved[2]),
+                                    ctx->saved_data["temperature"].toDouble(), or_none(saved[3]), grad, or_none(out[0]),
+                                    or_none(out[1]));
     }
     return logits_gradient(grad, 4);
   }
@@ -321,8 +381,8 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     ctx->saved_data["numbers"] = std::vector<double>{temperature_all, clip_low, clip_high, kl_coef, entropy_coef};
     ctx->set_materialize_grads(false);
     auto [loss, logprobs, kl, entropy, status] =
-        policy_loss(logits, tokens, old_logprobs, advantages, ref_logprobs, weights, temperature, temperature_all, mask,
-                    clip_low, clip_high, kl_coef, entropy_coef, std::nullopt);
+        call_or_trace<POLICY_LOSS>(policy_loss, logits, tokens, old_logprobs, advantages, ref_logprobs, weights, temperature,
+                                   temperature_all, mask, clip_low, clip_high, kl_coef, entropy_coef, std::nullopt);
     ctx->mark_non_differentiable({logprobs, kl, entropy, status});
     return {loss, logprobs, kl, entropy, status};
   }
@@ -334,8 +394,9 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     {
       const at::NoGradGuard unrecorded;
       grad = at::empty_like(saved[0]);
-      policy_loss(saved[0], saved[1], saved[2], saved[3], or_none(saved[4]), weighted(saved[5], out[0]), or_none(saved[6]),
-                  numbers[0], or_none(saved[7]), numbers[1], numbers[2], numbers[3], numbers[4], grad);
+      call_or_trace<POLICY_LOSS>(policy_loss, saved[0], saved[1], saved[2], saved[3], or_none(saved[4]),
+                                 weighted(saved[5], out[0]), or_none(saved[6]), numbers[0], or_none(saved[7]), numbers[1],
+                                 numbers[2], numbers[3], numbers[4], grad);
     }
     return logits_gradient(grad, 12);
   }
@@ -349,8 +410,8 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
                             or_undefined(mask)});
     ctx->saved_data["temperature"] = temperature_all;
     ctx->set_materialize_grads(false);
-    auto [loss, status] = distill_loss(logits, values, ids, rest, weights, temperature, temperature_all, mask, std::nullopt,
-                                       teacher_status);
+    auto [loss, status] = call_or_trace<DISTILL_LOSS>(distill_loss, logits, values, ids, rest, weights, temperature,
+                                                      temperature_all, mask, std::nullopt, teacher_status);
     ctx->mark_non_differentiable({status});
     return {loss, status};
   }
@@ -361,8 +422,9 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
     {
       const at::NoGradGuard unrecorded;
       grad = at::empty_like(saved[0]);
-      distill_loss(saved[0], saved[1], saved[2], or_none(saved[3]), weighted(saved[4], out[0]), or_none(saved[5]),
-                   ctx->saved_data["temperature"].toDouble(), or_none(saved[6]), grad, std::nullopt);
+      call_or_trace<DISTILL_LOSS>(distill_loss, saved[0], saved[1], saved[2], or_none(saved[3]), weighted(saved[4], out[0]),
+                                  or_none(saved[5]), ctx->saved_data["temperature"].toDouble(), or_none(saved[6]), grad,
+                                  std::nullopt);
     }
     return logits_gradient(grad, 8);
   }
@@ -395,16 +457,12 @@ std::tuple<Tensor, Tensor> distill_loss_tracked(const Tensor& logits, const Tens
   return {out[0], out[1]};
 }
 // ---- the operators as the dispatcher calls them, below autograd ----
-constexpr char TOKEN_LOGPROBS[] = "exactsample::token_logprobs", TOP_LOGITS[] = "exactsample::top_logits",
-               POLICY_LOSS[] = "exactsample::policy_loss", DISTILL_LOSS[] = "exactsample::distill_loss";
-
 template <const char* NAME, class F> struct BelowAutograd;
 template <const char* NAME, class R, class... A> struct BelowAutograd<NAME, R(A...)> {
   static R call(c10::DispatchKeySet keys, A... args) {
     refuse_tangents(args...);
-    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(NAME, "").typed<R(A...)>();
     const at::AutoDispatchBelowADInplaceOrView below;
-    return op.redispatch(keys & c10::after_ADInplaceOrView_keyset, args...);
+    return dispatched<NAME, R(A...)>().redispatch(keys & c10::after_ADInplaceOrView_keyset, args...);
   }
 };
 }  // namespace
@@ -453,4 +511,10 @@ TORCH_LIBRARY_IMPL(exactsample, Autograd, m) {
   m.impl("top_logits", &BelowAutograd<TOP_LOGITS, decltype(top_logits)>::call);
   m.impl("policy_loss", &BelowAutograd<POLICY_LOSS, decltype(policy_loss)>::call);
   m.impl("distill_loss", &BelowAutograd<DISTILL_LOSS, decltype(distill_loss)>::call);
+}
+TORCH_LIBRARY_IMPL(exactsample, Meta, m) {
+  m.impl("token_logprobs", &token_logprobs_meta);
+  m.impl("top_logits", &top_logits_meta);
+  m.impl("policy_loss", &policy_loss_meta);
+  m.impl("distill_loss", &distill_loss_meta);
 }

@@ -27,7 +27,9 @@ autograd. Without it, on logits that require a gradient, the result is
 differentiable by the logits, once and in reverse mode (forward-mode
 derivatives are refused), and the backward pass reads them a second time.
 To capture a whole training step in a CUDA graph, ``grad=`` is the way that
-does not depend on what autograd's accumulation nodes were made on.
+does not depend on what autograd's accumulation nodes were made on. The calls
+can be traced (torch.compile, tensors without memory) once the library is
+loaded, which ``exactsample_b200.cuda.load_library`` or any call of one does.
 """
 from __future__ import annotations
 

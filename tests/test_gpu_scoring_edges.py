@@ -330,3 +330,33 @@ def test_results_are_saved_together(tmp_path):
         torch.save(whole, tmp_path / "results.pt")
         again = torch.load(tmp_path / "results.pt")
         assert all(torch.equal(again[name], whole[name]) for name in whole)
+
+
+# ---------------------------------------------------------------- tracing
+def test_compiled_training_step():
+    """Traced whole, forward and backward: the same results as in eager mode."""
+    _, logits, tokens, columns, teacher = step_inputs()
+
+    def losses(x):
+        out = scoring.token_logprobs(x, tokens, temperature=0.8)
+        policy = scoring.policy_loss(x, tokens, out.logprobs.detach(), columns[1], entropy_coef=0.1, temperature=0.8)
+        distill = scoring.distill_loss(x, teacher, weights=columns[2])
+        return out.logprobs.sum() + 0.1 * out.entropy.sum() + policy.loss.sum() + distill.loss.sum(), policy.status
+
+    def with_grad(x, grad):
+        top = scoring.top_logits(x, 7)
+        out = scoring.policy_loss(x, tokens, columns[0], columns[1], grad=grad)
+        return out.loss, out.status, top.values, top.ids, top.rest
+
+    leaf, other = logits.clone().requires_grad_(), logits.clone().requires_grad_()
+    want, status = losses(leaf)
+    want.backward()
+    got, other_status = torch.compile(losses, backend="aot_eager", fullgraph=True)(other)
+    got.backward()
+    assert torch.equal(status, other_status)
+    torch.testing.assert_close(got, want, rtol=1e-6, atol=0)  # (the sum of sums, in another order)
+    torch.testing.assert_close(other.grad, leaf.grad, rtol=1e-6, atol=1e-7)  # (three gradients added, likewise)
+    grads = [torch.full_like(logits, 5.0) for _ in range(2)]
+    eager = with_grad(logits, grads[0])
+    traced = torch.compile(with_grad, backend="aot_eager", fullgraph=True)(logits, grads[1])
+    assert all(torch.equal(a, b) for a, b in zip(eager, traced)) and torch.equal(*grads)

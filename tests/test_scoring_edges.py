@@ -69,3 +69,52 @@ def test_a_teachers_statuses_are_checked():
     assert lib.es_distill_loss_status(None, None, None) == -1
     empty = arguments("es_distill_loss", rows=0)
     assert with_status(empty, empty._host.t((0,), np.int32, capi.ES_I32)) == (0, "")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+def test_shapes_and_types_without_memory(dtype):
+    """What a tracer asks for: results of tensors without memory, forward and backward."""
+    rows, vocab, k = 3, 40, 4
+    x = torch.empty(rows, vocab, dtype=dtype, device="meta")
+    tokens = torch.empty(rows, dtype=torch.int64, device="meta")
+    column = torch.empty(rows, device="meta")
+    teacher = scoring.top_logits(x, k)
+    calls = [lambda z, **kw: scoring.token_logprobs(z, tokens, **kw),
+             lambda z, **kw: scoring.policy_loss(z, tokens, column, column, weights=column, **kw),
+             lambda z, **kw: scoring.distill_loss(z, teacher, weights=column, **kw)]
+    outs = [call_of(x) for call_of in calls] + [call_of(x, grad=torch.empty_like(x)) for call_of in calls]
+    for out in outs + [teacher]:
+        for name in out.__slots__:
+            kind = {"status": torch.int32, "ids": torch.int64}.get(name, torch.float32)
+            value = getattr(out, name)
+            assert value.dtype == kind and not value.requires_grad
+            assert value.shape == ((rows, k) if name in ("values", "ids") else (rows,))
+    for call_of in calls:
+        leaf = x.clone().requires_grad_()
+        out = call_of(leaf)
+        sum(getattr(out, name).sum() for name in out.__slots__ if getattr(out, name).requires_grad).backward()
+        assert leaf.grad.shape == x.shape and leaf.grad.dtype == dtype and not out.status.requires_grad
+    with pytest.raises(RuntimeError, match="float16/bfloat16/float32"):
+        scoring.token_logprobs(x.double(), tokens)
+    with pytest.raises(RuntimeError, match="k must be"):
+        scoring.top_logits(x, 257)
+
+
+def test_a_training_step_is_traced():
+    """Into one graph: each operator, and its gradient's call in the backward pass."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def step(x, tokens, column):
+        leaf = x.detach().requires_grad_()
+        loss = scoring.policy_loss(leaf, tokens, column, column).loss.sum()
+        loss = loss + scoring.token_logprobs(leaf, tokens).logprobs.sum()
+        loss = loss + scoring.distill_loss(leaf, scoring.top_logits(x, 5)).loss.sum()
+        return torch.autograd.grad(loss, leaf)
+    with FakeTensorMode():
+        inputs = (torch.empty(3, 8, device="meta"), torch.empty(3, dtype=torch.int64, device="meta"),
+                  torch.empty(3, device="meta"))
+        nodes = [str(node.target) for node in make_fx(step)(*inputs).graph.nodes]
+    counts = {name: sum(f"exactsample.{name}.default" == node for node in nodes)
+              for name in ("token_logprobs", "policy_loss", "distill_loss", "top_logits")}
+    assert counts == dict(token_logprobs=2, policy_loss=2, distill_loss=2, top_logits=1)
