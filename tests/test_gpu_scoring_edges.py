@@ -1,5 +1,7 @@
 """The row operators on the GPU where a factor leaves float32's range though
-the result does not."""
+the result does not, and in the calls around them: derivatives that they do not
+have, teachers that failed, saving, tracing, gradients handed on to a layer, and
+gradients that lie otherwise than the logits do."""
 import math
 
 import pytest
@@ -330,6 +332,94 @@ def test_results_are_saved_together(tmp_path):
         torch.save(whole, tmp_path / "results.pt")
         again = torch.load(tmp_path / "results.pt")
         assert all(torch.equal(again[name], whole[name]) for name in whole)
+
+
+def test_grad_through_a_layer():
+    """The call's gradient handed on to the layers before the logits: the same
+    as through autograd, into memory of its own and into the logits'."""
+    g = torch.Generator(device="cuda").manual_seed(22)
+    rows, vocab = 12, 900
+    hidden = torch.randn(rows, 32, device="cuda", generator=g)
+    weight = (torch.randn(vocab, 32, device="cuda", generator=g) * 0.2).requires_grad_()
+    tokens = torch.randint(vocab, (rows,), device="cuda", generator=g)
+    old, adv = torch.full((rows,), -7.0, device="cuda"), torch.randn(rows, device="cuda", generator=g)
+    scoring.policy_loss(hidden @ weight.t(), tokens, old, adv, entropy_coef=0.01).loss.sum().backward()
+    want, weight.grad = weight.grad, None
+    for over in (False, True):
+        logits = hidden @ weight.t()
+        flat = logits.detach()
+        grad = flat if over else torch.empty_like(flat)
+        scoring.policy_loss(flat, tokens, old, adv, entropy_coef=0.01, grad=grad)
+        logits.backward(grad)
+        assert torch.equal(weight.grad, want)
+        weight.grad = None
+    with pytest.raises(ValueError, match="grad= takes the gradient"):
+        logits = hidden @ weight.t()
+        scoring.policy_loss(logits, tokens, old, adv, grad=torch.empty_like(logits))
+
+
+# ---------------------------------------------------------------- many rows, other layouts
+def layout(rows, vocab, dtype, kind):
+    if kind == "plain":
+        return torch.full((rows, vocab), 3.0, dtype=dtype, device="cuda")
+    if kind == "even":   # rows on 16 bytes whatever the vocabulary
+        return torch.full((rows, (vocab + 7) // 8 * 8 + 8), 3.0, dtype=dtype, device="cuda")[:, :vocab]
+    if kind == "words":  # rows on 4 bytes and not on 16
+        return torch.full((rows, (vocab + 7) // 8 * 8 + 4), 3.0, dtype=dtype, device="cuda")[:, 2:2 + vocab]
+    if kind == "odd":
+        return torch.full((rows, vocab + 7 + vocab % 2), 3.0, dtype=dtype, device="cuda")[:, 3:3 + vocab]
+    return torch.full((rows, 2 * vocab), 3.0, dtype=dtype, device="cuda")[:, ::2]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
+@pytest.mark.parametrize("vocab", [1003, 1008, 40_001])
+@pytest.mark.parametrize("kind", ["even", "words", "odd", "gaps"])
+def test_rows_that_share_a_cluster_in_other_layouts(dtype, vocab, kind):
+    """Next rows copied while a gradient is written that starts elsewhere than
+    the logits do, or over the logits themselves; a temperature for each row."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    rows = 1500 if vocab < 2000 else 700
+    logits = layout(rows, vocab, dtype, kind)
+    logits.copy_(torch.randn(rows, vocab, device="cuda", generator=g) * 3)
+    logits[5::11, ::4] = -math.inf
+    tokens = torch.randint(vocab, (rows,), device="cuda", generator=g)
+    tokens[torch.rand(rows, device="cuda", generator=g) < 0.1] = -1
+    columns = [torch.randn(rows, device="cuda", generator=g) for _ in range(4)]
+    temperature = 0.5 + torch.rand(rows, device="cuda", generator=g, dtype=torch.float64)
+    temperature[7::50] = 0.0
+    ids = torch.stack([torch.randint(i * vocab // 9, (i + 1) * vocab // 9, (rows,), device="cuda", generator=g) for i in range(9)], 1)
+    ids[torch.rand(rows, device="cuda", generator=g) < 0.1] = -1
+    values = torch.randn(rows, 9, device="cuda", generator=g)
+
+    def call(which, x, at, grad):
+        c, t = [column[at] for column in columns], temperature[at]
+        if which == 0:
+            return scoring.token_logprobs(x, tokens[at], temperature=t, grad=grad, grad_logprobs=c[0], grad_entropy=c[1])
+        if which == 1:
+            return scoring.policy_loss(x, tokens[at], c[0], c[1], ref_logprobs=c[2], weights=c[3], kl_coef=0.1,
+                                       entropy_coef=0.02, temperature=t, grad=grad)
+        return scoring.distill_loss(x, scoring.TopLogits(values[at], ids[at], c[0]), weights=c[3], temperature=t, grad=grad)
+
+    whole = slice(0, rows)
+    for which in range(3):
+        want = layout(rows, vocab, dtype, "plain")
+        pieces = []
+        for first in range(0, rows, 40):  # batches whose rows have a cluster each
+            at = slice(first, first + 40)
+            pieces.append(call(which, logits[at].contiguous(), at, want[at]))
+        for grad_kind in ("plain", "even", "words", "odd", "gaps"):
+            grad = layout(rows, vocab, dtype, grad_kind)
+            out = call(which, logits, whole, grad)
+            assert torch.equal(grad, want), grad_kind
+            for name in out.__slots__:
+                assert torch.equal(getattr(out, name), torch.cat([getattr(o, name) for o in pieces])), name
+            if grad_kind != "plain":  # nothing beside the rows is written
+                assert int((grad._base == 3).sum()) - int((grad == 3).sum()) == grad._base.numel() - rows * vocab
+        over = layout(rows, vocab, dtype, kind)
+        over.copy_(logits)
+        call(which, over, whole, over)
+        assert torch.equal(over, want)
+        assert int((over._base == 3).sum()) - int((over == 3).sum()) == over._base.numel() - rows * vocab
 
 
 # ---------------------------------------------------------------- tracing
