@@ -732,9 +732,9 @@ __device__ __forceinline__ Record sum_slice(const Slice<DT>& slice, const uint32
       for (int i = c * N; i < slice.n; ++i) held |= Elem<DT>::get(slice[i]) == -INFINITY;
     acc_add<N, ENTROPY>(a, v, scale);
   }
-  const bool failed = tid < slice.chunks &&
-                      (blank || acc_failed<ENTROPY>(a) || scale < SMALL_SCALE || (RAISE && any && a.m <= NONE));
-  if (failed) {
+  // (A thread without chunks has nothing to fail on, and its warp's reference may overflow.)
+  const bool failed = blank || acc_failed<ENTROPY>(a) || scale < SMALL_SCALE || (RAISE && any && a.m <= NONE);
+  if (failed || tid >= slice.chunks) {
     a = acc_none();
 #pragma unroll 1
     for (c = tid; c < slice.chunks; c += THREADS) {
@@ -745,7 +745,7 @@ __device__ __forceinline__ Record sum_slice(const Slice<DT>& slice, const uint32
       acc_careful<N, ENTROPY>(a, v, max_of<N>(v), scale);
     }
   }
-  Record r = acc_exact<ENTROPY>(a, scale, failed);
+  Record r = acc_exact<ENTROPY>(a, scale, failed && tid < slice.chunks);
   if (HAS_MASK && !(seen_top < INFINITY)) r.flags |= BAD;
   if (held) r.flags |= HELD;
   return r;

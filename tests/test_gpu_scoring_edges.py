@@ -248,6 +248,45 @@ def test_entropy_gradients_beside_very_low_logits(dtype, far, incoming):
             assert bool((got[~live[r]] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
+@pytest.mark.parametrize("vocab", [2, 40, 129, 300, 600, 1001, 50_257])
+@pytest.mark.parametrize("masked", [False, True], ids=["open", "masked"])
+def test_logits_at_the_types_highest(dtype, vocab, masked):
+    """Rows whose exponents' reference is beyond float32, at sizes that leave
+    threads of a warp without tokens."""
+    highest = torch.finfo(dtype).max
+    x = torch.zeros(3, vocab, dtype=dtype)
+    x[0, 0] = highest
+    x[1] = highest
+    x[2, -1] = highest / 256
+    tokens = torch.tensor([0, vocab // 2, vocab - 1])
+    mask = ref.pack_mask(torch.ones(3, vocab, dtype=torch.bool)).cuda() if masked else None
+    teacher = scoring.TopLogits(torch.zeros(1, 1, device="cuda"), torch.zeros(1, 1, dtype=torch.int64, device="cuda"),
+                                torch.full((1,), 0.5, device="cuda"))
+    log_v = math.log(vocab)
+    for temperature in (1.0, 0.01):
+        grad = torch.full_like(x, 5.0, device="cuda")
+        ones = torch.ones(3, device="cuda")
+        out = scoring.token_logprobs(x.cuda(), tokens.cuda(), temperature=temperature, mask=mask, grad=grad,
+                                     grad_logprobs=ones, grad_entropy=ones)
+        assert out.status.cpu().tolist() == [0, 0, 0]
+        limit = sum_error(torch.zeros(vocab), vocab) + 2.0**-23 * log_v
+        for got, want in ((out.logprobs, [0, -log_v, 0]), (out.entropy, [0, log_v, 0])):
+            assert float((got.cpu().double() - torch.tensor(want).double()).abs().max()) <= 3 * limit
+        want = torch.full((vocab,), -1 / vocab, dtype=torch.float64)
+        want[vocab // 2] += 1
+        assert bool((grad[[0, 2]] == 0).all())
+        bound = (want.abs() * ref.HALF_STEP[dtype] + 6 * limit / vocab) * 1.01 + ref.SMALLEST[dtype]
+        bound[vocab // 2] += 6 * limit
+        assert bool(((grad[1].cpu().double() * temperature - want).abs() <= bound).all())
+        # Distillation against the row of equal logits: t and q of two classes.
+        got = scoring.distill_loss(x[1:2].cuda(), teacher, temperature=temperature, mask=None if mask is None else mask[1:2])
+        t = torch.softmax(torch.tensor([0.0, 0.5], dtype=torch.float64), 0)
+        loss = float((t * (t.log() - torch.tensor([1 / vocab, 1 - 1 / vocab]).double().log())).sum())
+        assert int(got.status[0]) == 0
+        assert abs(float(got.loss[0]) - loss) <= 3 * limit + 40 * 2.0**-24 * (1 + abs(loss))
+
+
 # ---------------------------------------------------------------- the calls
 def step_inputs(rows=6, vocab=700, seed=21):
     g = torch.Generator(device="cuda").manual_seed(seed)
