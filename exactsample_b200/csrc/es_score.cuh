@@ -210,14 +210,18 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 //
 // The fast forms take d = z scale - r in one instruction, with r = m scale
 // rounded to 32 bits; acc_exact afterwards makes s and u those of m itself.
-// Their m is not the maximum: 32-bit sums keep their digits wherever the
-// largest 2^d lies, so a warp's largest of its first tokens serves all of its
-// tokens, and no maximum is looked for after those (it took a third of the
-// pass). They leave some rows wrong, and acc_failed tells: sums of 2^60 and
-// more (a row's coefficient, 1 / s, is to stay a normal number), a -inf
-// beside an entropy (0 * -inf), an r that overflows, and an r so large that
-// its rounding moves the exponents. The careful form, which keeps the running
-// maximum, subtracts first and holds exponents at FAR, is right for those.
+// Their m is not the maximum, which took a third of the pass to look for, but
+// the largest of a warp's first tokens, and in the thread that has the row's
+// token that token's logit if it is larger. d's rounding grows with it, and the
+// entropy, log s - u / s, loses what log s and u / s have in common, so that m
+// should not lie far below where the mass is. A row whose token has most of it,
+// as most rows do, so has the maximum itself for m. (With the first tokens alone
+// a row whose peak was 22 nats above the others had an entropy of 7.6e-4 with an
+// error of 7e-6, and at 30 nats half of the log-probabilities were above 0.) The
+// fast forms leave some rows wrong, and acc_failed tells: sums of MOST and more,
+// a -inf beside an entropy (0 * -inf), an r that overflows, and an r so large
+// that its rounding moves the exponents. The careful form, which keeps the
+// running maximum, subtracts first and holds exponents at FAR, is right for those.
 struct Acc {
   float m, r;
   float2 s, u;
@@ -288,8 +292,9 @@ template <int N, bool ENTROPY> __device__ __forceinline__ void acc_add(Acc& a, c
     if (ENTROPY) a.u = fma2(e, d, a.u);
   }
 }
-// Raises the reference to `top` if that is 2^24 above it (masked rows, whose
+// Raises the reference to `top` if that is 2^16 above it (masked rows, whose
 // first tokens may all be masked).
+__device__ __forceinline__ float raise_limit(float m, float scale) { return __fadd_rn(m, __fdividef(16.f, scale)); }
 template <bool ENTROPY> __device__ __forceinline__ void acc_raise(Acc& a, float top, float scale, float& limit) {
   if (top > limit) {
     const float r = __fmul_rn(top, scale), d = __fsub_rn(a.r, r), f = a.m <= NONE ? 0.f : ex2(d);
@@ -297,7 +302,7 @@ template <bool ENTROPY> __device__ __forceinline__ void acc_raise(Acc& a, float 
     a.s = mul2(both(f), a.s);
     a.m = top;
     a.r = r;
-    limit = __fadd_rn(top, __fdividef(24.f, scale));
+    limit = raise_limit(top, scale);
   }
 }
 template <int N, bool ENTROPY>
@@ -317,10 +322,14 @@ __device__ __forceinline__ void acc_careful(Acc& a, const float2* v, float top, 
     if (ENTROPY) a.u = fma2(e, d, a.u);
   }
 }
+// The largest sum of a fast form. With an entropy a sum that large is 17 nats
+// above its reference, where log s and u / s are rounded by 1e-6; without one it
+// is only to keep a row's coefficient, 1 / s, a normal number.
+template <bool ENTROPY> constexpr float MOST = ENTROPY ? 0x1p24f : 0x1p60f;
 constexpr float LARGE_R = 65536.f;  // its rounding is 2^-8 at most, which acc_exact takes back
 template <bool ENTROPY> __device__ __forceinline__ bool acc_failed(const Acc& a) {
   const float s = a.s.x + a.s.y, u = a.u.x + a.u.y;
-  return !(fabsf(a.r) <= LARGE_R) || !(s < 0x1p60f) || (ENTROPY && !(fabsf(u) < 0x1p67f));
+  return !(fabsf(a.r) <= LARGE_R) || !(s < MOST<ENTROPY>) || (ENTROPY && !(fabsf(u) < 0x1p67f));
 }
 
 // What one rank knows of its slice: s and u against the maximum m.
@@ -639,7 +648,8 @@ template <int N> __device__ __forceinline__ float max_of(const float2* v) {
 
 // This thread's share of a slice as a Record: the fast form, or where that
 // fails the careful one. The slice has arrived up to `half`. `words`: a
-// MASKED_ROW's mask; its masked tokens are masked in the slice too. An
+// MASKED_ROW's mask; its masked tokens are masked in the slice too. `token`: the
+// row's, if it lies in the slice, or negative. An
 // OPEN_ROW's warps that see a -inf among their first tokens (rows that were
 // masked before) hold every -inf at MASKED instead; those that meet one later
 // take the careful form. (1,024 rows of 151,936 bf16 with a
@@ -647,7 +657,7 @@ template <int N> __device__ __forceinline__ float max_of(const float2* v) {
 // the careful form, 81 and 131 so, 74 and 127 without a -inf.)
 enum RowKind { OPEN_ROW, MASKED_ROW, HELD_ROW };
 template <int DT, bool ENTROPY, int KIND>
-__device__ __forceinline__ Record sum_slice(const Slice<DT>& slice, const uint32_t* words, float scale) {
+__device__ __forceinline__ Record sum_slice(const Slice<DT>& slice, const uint32_t* words, int token, float scale) {
   constexpr int N = Elem<DT>::N;
   constexpr bool HAS_MASK = KIND == MASKED_ROW, RAISE = KIND != OPEN_ROW;
   constexpr bool HOLD = RAISE && ENTROPY && DT == ES_F16;
@@ -690,11 +700,21 @@ __device__ __forceinline__ Record sum_slice(const Slice<DT>& slice, const uint32
         top = fmaxf(top, chunk_max<DT>(q, q));
         if (ENTROPY) lowest |= chunk_has_lowest<DT>(q);
       }
-    if (ENTROPY && __any_sync(0xffffffffu, lowest)) return sum_slice<DT, ENTROPY, ENTROPY ? HELD_ROW : OPEN_ROW>(slice, words, scale);
+    if (ENTROPY && __any_sync(0xffffffffu, lowest)) return sum_slice<DT, ENTROPY, ENTROPY ? HELD_ROW : OPEN_ROW>(slice, words, token, scale);
     top = warp_all(top, [](float x, float y) { return fmaxf(x, y); });
     blank = !(top > -INFINITY);
     a.m = blank ? 0.f : top;
     a.r = __fmul_rn(a.m, scale);
+  }
+  // The thread that has the row's token takes its logit for the reference.
+  if (ENTROPY && token >= 0 && token / N % THREADS == tid) {
+    if (token / N >= slice.half) slice.arrive_rest();
+    const float z = Elem<DT>::get(slice[token]);
+    if (z > a.m && (!HAS_MASK || mask_bits(words, token) & 1)) {
+      a.m = z;
+      a.r = __fmul_rn(z, scale);
+      if (RAISE) limit = raise_limit(z, scale);
+    }
   }
   // Four chunks a step, for independent loads and exponentials.
   int c = tid;
@@ -936,9 +956,10 @@ template <int DT, int OP, bool GRAD> struct LossRow {
   __device__ __forceinline__ void token_scalars(Shared& sh, float m, float s, float u, uint32_t flags, const Scale& scale,
                                                 const Inputs& in) {
     const float z = E::get(in.raw);
-    const Pair log_s = log_pair(s), lp = pair_sum(scaled_gap(z, m, scale), negated(log_s));
+    const Pair log_s = log_pair(s), below = scaled_gap(z, m, scale), lp = pair_sum(below, negated(log_s));
     const float inv_s = __frcp_rn(s), gap = u * inv_s * float(LN2);  // log(s) - h
-    const float h = value_of({log_s.hi, log_s.lo - gap});
+    // (Neither's rounding may take it past the end of its range.)
+    const float h = fmaxf(value_of({log_s.hi, log_s.lo - gap}), 0.f), logprob = fminf(value_of(lp), 0.f);
     const bool mass = z > -INFINITY && (in.mask >> (in.token & 31) & 1);
     // A NaN logit makes s NaN, +inf the maximum.
     bool bad = (flags & BAD) || !(s < INFINITY) || m == INFINITY || in.token >= p.in.vocab;
@@ -989,7 +1010,7 @@ template <int DT, int OP, bool GRAD> struct LossRow {
     else if (!mass) status = ES_DRAFT_ZERO_PROB;
     const bool ok = status == ES_OK;
     if (rank == 0)
-      outputs(status, ok ? loss : 0.f, ok ? value_of(lp) : -INFINITY, ok ? kl : 0.f, ok ? h : 0.f);
+      outputs(status, ok ? loss : 0.f, ok ? logprob : -INFINITY, ok ? kl : 0.f, ok ? h : 0.f);
     if (GRAD) {
       slope *= scale.hi;
       on_entropy *= scale.hi;
@@ -1000,7 +1021,8 @@ template <int DT, int OP, bool GRAD> struct LossRow {
       set_scalars(r, m, scale.log2, -(slope - on_entropy * gap) * inv_s, -on_entropy * float(LN2) * inv_s,
                   flags & CAREFUL || scale.log2 < SMALL_SCALE);
       r.held = flags & HELD;
-      r.token_grad = -slope * expm1f(value_of(lp)) - on_entropy * expf(value_of(lp)) * (value_of(lp) + h);
+      // log p + h without the log(s) that both have.
+      r.token_grad = -slope * expm1f(logprob) - on_entropy * expf(logprob) * ((below.hi - gap) + below.lo);
     }
   }
 
@@ -1103,7 +1125,8 @@ template <int DT, int OP, bool GRAD> struct LossRow {
     else if (lost) status = ES_DRAFT_ZERO_PROB;
     else if (!isfinite(loss)) status = ES_INVALID_INPUT;
     const bool ok = status == ES_OK;
-    if (rank == 0) outputs(status, ok ? in.w * loss : 0.f, 0.f, 0.f, 0.f);
+    // (A KL's rounding may not take it below 0 either.)
+    if (rank == 0) outputs(status, ok ? in.w * fmaxf(loss, 0.f) : 0.f, 0.f, 0.f, 0.f);
     if (GRAD) {
       RowScalars& r = sh.row;
       r.zero = !ok;
@@ -1366,8 +1389,10 @@ template <int DT, int OP, bool GRAD> struct LossRow {
         __syncthreads();
       }
 
-      Record rec = masked ? sum_slice<DT, ENTROPY, MASKED_ROW>(slice, words, scale.log2)
-                          : sum_slice<DT, ENTROPY, OPEN_ROW>(slice, nullptr, scale.log2);
+      const int64_t local = in.token - begin;
+      const int at = OP != DISTILL && local >= 0 && local < n ? int(local) : -1;
+      Record rec = masked ? sum_slice<DT, ENTROPY, MASKED_ROW>(slice, words, at, scale.log2)
+                          : sum_slice<DT, ENTROPY, OPEN_ROW>(slice, nullptr, at, scale.log2);
       // (The token's logit is looked at before this rank says that it has done
       // with the row's memory, which may be the gradient's.)
       if (OP != DISTILL && tid == 0) bad |= isnan(E::get(in.raw));
@@ -1400,8 +1425,6 @@ template <int DT, int OP, bool GRAD> struct LossRow {
           zero_grad();
           if (loaded) slice.load(p.in, row + stride, begin);
         } else {
-          const int64_t local = in.token - begin;
-          const int at = OP != DISTILL && local >= 0 && local < n ? int(local) : -1;
           write_form(slice, words, r, scale.log2, at, next);
           if (OP == DISTILL) __syncthreads();  // after the slice's zeros at these places
           if (OP == DISTILL)

@@ -287,6 +287,69 @@ def test_logits_at_the_types_highest(dtype, vocab, masked):
         assert abs(float(got.loss[0]) - loss) <= 3 * limit + 40 * 2.0**-24 * (1 + abs(loss))
 
 
+# ---------------------------------------------------------------- rows with one likely token
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
+@pytest.mark.parametrize("vocab", [700, 32_000, 151_936])
+@pytest.mark.parametrize("kind", ["open", "masked", "infinities"])
+@pytest.mark.parametrize("peak", [18, 24, 30, 40])
+def test_rows_whose_token_has_most_of_the_mass(dtype, vocab, kind, peak):
+    """The digits of small entropies and of log-probabilities near 0, wherever
+    in the row the token lies; none past the end of its range."""
+    g = torch.Generator(device="cuda").manual_seed(peak)
+    rows = 48
+    x = torch.randn(rows, vocab, device="cuda", generator=g) * 2
+    tokens = torch.randint(vocab, (rows,), device="cuda", generator=g)
+    tokens[:2] = torch.tensor([0, vocab - 1])
+    x.scatter_(1, tokens[:, None], peak + torch.rand(rows, 1, device="cuda", generator=g))
+    allowed = torch.ones(rows, vocab, dtype=torch.bool, device="cuda")
+    if kind != "open":
+        allowed = torch.rand(rows, vocab, device="cuda", generator=g) < 0.6
+        allowed.scatter_(1, tokens[:, None], True)
+    if kind == "infinities":
+        x.masked_fill_(~allowed, -math.inf)
+    x = x.to(dtype)
+    mask = ref.pack_mask(allowed.cpu()).cuda() if kind == "masked" else None
+    grads = [torch.empty_like(x) for _ in range(2)]
+    ones = torch.ones(rows, device="cuda")
+    out = scoring.token_logprobs(x, tokens, mask=mask, grad=grads[0], grad_entropy=ones)
+    step = scoring.policy_loss(x, tokens, out.logprobs, torch.zeros_like(ones), mask=mask, entropy_coef=-1.0, grad=grads[1])
+    assert torch.equal(step.logprobs, out.logprobs) and torch.equal(step.entropy, out.entropy)
+    logp = torch.log_softmax(x.double().masked_fill(~allowed, -math.inf), 1)
+    p = logp.exp()
+    plogp = torch.where(p > 0, p * logp, 0.0)
+    h, lp = -plogp.sum(1), logp.gather(1, tokens[:, None])[:, 0]
+    assert bool((out.logprobs <= 0).all()) and bool((out.entropy >= 0).all()) and not bool(out.status.any())
+    # The token's exponential is 1 exactly, and the sum is 1 + rest: it is
+    # rounded by each of the 26 joins of a row's partial sums and by a thread's
+    # 100 additions to 1 while those come to half a unit, all of it at most the
+    # rest itself and a few units where the rest is below one.
+    rest = -torch.expm1(lp)
+    lost = torch.minimum((26 + 100) * 2.0**-24 * torch.ones_like(rest), 4 * 2.0**-24 + 2 * rest)
+    relative = 2.0**-15  # of the others' sums: exponents of at most 60 nats (3 * 2^-24 each), 130 roundings
+    assert bool(((out.logprobs - lp).abs() <= lost + relative * lp.abs()).all())
+    assert bool(((out.entropy - h).abs() <= lost + relative * h).all())
+    # A gradient's factor log p + h is a quotient of sums at the token, and far
+    # from 0 at the others: each is right to its own digits. (The exponents'
+    # reference is rounded to 32 bits, by 2^-24 of the peak at most, and the
+    # token's exponent is what that takes away: the quotient's sum has that in
+    # it for as many as 130 additions, each rounded by 2^-24 of it, before it is
+    # taken back.)
+    want = -(plogp + p * h[:, None])
+    back = torch.zeros_like(want).scatter_(1, tokens[:, None], 130 * 2.0**-48 * (peak + 1))
+    for grad in grads:
+        limit = want.abs() * (2 * relative + ref.HALF_STEP[dtype] * 1.01) + ref.SMALLEST[dtype] * 2 + 2.0**-126 * 100 + back
+        assert bool(((grad.double() - want).abs() <= limit).all()), float(((grad.double() - want).abs() / limit).max())
+
+
+def test_a_student_like_its_teacher_has_no_negative_loss():
+    g = torch.Generator(device="cuda").manual_seed(17)
+    logits = torch.randn(400, 5000, device="cuda", generator=g) * 3
+    for k in (1, 20, 256):
+        for tail in (True, False):
+            out = scoring.distill_loss(logits, scoring.top_logits(logits, k), tail=tail)
+            assert bool((out.loss >= 0).all())
+
+
 # ---------------------------------------------------------------- the calls
 def step_inputs(rows=6, vocab=700, seed=21):
     g = torch.Generator(device="cuda").manual_seed(seed)
