@@ -153,7 +153,8 @@ struct RowCall {
   std::array<Tensor, 5> columns(int floats) const {
     const int64_t rows = logits.size(0), width = (rows + 3) / 4 * 4;
     const auto memory = [](int64_t words) {
-      return c10::Storage(c10::Storage::use_byte_size_t(), size_t(words) * 4, c10::GetAllocator(at::kCUDA), /*resizable=*/true);
+      return c10::Storage(c10::Storage::use_byte_size_t(), size_t(words) * 4, c10::cuda::CUDACachingAllocator::get(),
+                          /*resizable=*/true);
     };
     const auto column = [rows](c10::Storage storage, int64_t offset, caffe2::TypeMeta type) {
       Tensor t = at::detail::make_tensor<c10::TensorImpl>(std::move(storage), c10::DispatchKeySet(c10::DispatchKey::CUDA), type);
