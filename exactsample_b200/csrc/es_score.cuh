@@ -12,9 +12,11 @@
 //
 // Bounds: the HBM, then the exponentials (two a token, 16 a cycle and SM:
 // about 70 % of the time that 2-byte rows take at full HBM rate), then latency
-// between the passes. Measured on a B200, 4,096 rows of 151,936 bf16: the
-// policy step 453 us, 5.4 TB/s, 82 % of a copy's rate; without any
-// exponential the same loops take 408 us.
+// between the passes. Measured on B200s, 4,096 rows of 151,936 bf16: the
+// policy step takes 453 to 476 us in runs of 20, by the card (5.2 to 5.5 TB/s,
+// 80 to 84 % of a copy's rate), and 500 to 510 in runs of seconds, whose clocks
+// are lower (75 %). Without any exponential the same loops took 408 us where it
+// took 453.
 //
 // The split depends on the vocabulary and the type alone, and every thread
 // takes the same elements whatever the row's address, so a row's results are
@@ -253,7 +255,6 @@ template <int DT> __device__ __forceinline__ float chunk_max(const uint4& p, con
     return fmaxf(m.x, m.y);
   }
 }
-// The same, and NaN if there is one.
 // Whether a chunk holds a -inf.
 template <int DT> __device__ __forceinline__ bool chunk_has_lowest(const uint4& q) {
   if constexpr (DT == ES_F32) {
@@ -269,6 +270,7 @@ template <int DT> __device__ __forceinline__ bool chunk_has_lowest(const uint4& 
     return fminf(m.x, m.y) == -INFINITY;
   }
 }
+// The largest of a chunk, and NaN if there is one.
 template <int DT> __device__ __forceinline__ float chunk_max_nan(const uint4& q) {
   if constexpr (DT == ES_F32) {
     return max_nan(max_nan(__uint_as_float(q.x), __uint_as_float(q.y)), max_nan(__uint_as_float(q.z), __uint_as_float(q.w)));

@@ -18,8 +18,15 @@
 //      ones, and adds the entries past the k-th to the rest.
 // Entries are 64-bit words, the logit's order key above the complement of its
 // id, so that all are distinct and equal logits rank by the lowest id. Where a
-// rank lists more than its places on rank 0 (equal values, in the main), rank
-// 0 finds the exact threshold by a digit-by-digit count over the whole row.
+// rank lists more than its places on rank 0, rank 0 alone finds the exact
+// threshold by a digit-by-digit count over the whole row, 23 passes that load
+// single tokens. Two kinds of rows come to that: equal values in numbers, and
+// rows where one rank's slice has fewer tokens than it is asked for, since the
+// smallest of the ranks' bounds then lets every token through. Masks or -inf
+// that leave a part of the vocabulary empty make the second kind: 2,048 rows of
+// 151,936 bf16 take 58 ms where a mask allows ids below 3,000, 64 below 100,000,
+// 62 with -inf above 100,000 and 68 where all logits are equal, and 8 rows take
+// 6 to 7 ms, against 0.18 ms and 16 us for open rows.
 //
 // Bounds: the latency of the steps after the streaming, each of which waits
 // for the other ranks. Measured on a B200: the 64 largest of 2,048 rows of

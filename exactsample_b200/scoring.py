@@ -12,7 +12,9 @@
 They take the logits, packed masks and statuses of ``exactsample_b200.verify``
 and share its rules: every tensor is on the logits' device, bad values inside
 device tensors do not raise but show up as that row's status, and a row's
-results are the same bits in any batch. ``include/exactsample_b200.h`` states
+results are the same bits in any batch. Temperatures are one number, or one
+float64 per row, where ``verify`` has one per request, and are positive: there
+is no greedy 0, whose rows would be INVALID_INPUT. ``include/exactsample_b200.h`` states
 each operator's formulas and what its statuses mean.
 
 A call launches one kernel on the current stream. It allocates its per-row
@@ -131,7 +133,9 @@ def top_logits(logits, k: int, *, temperature=1.0, mask=None) -> TopLogits:
     ``values`` are the logits as they are; ``temperature`` is what ``rest`` is
     taken at. Log-probabilities follow as ``values / temperature - total`` with
     ``total = logaddexp(logsumexp(values / temperature), rest)``. Not recorded
-    for autograd: it is a teacher's or a server's pass.
+    for autograd: it is a teacher's or a server's pass. Rows that a mask, or
+    logits of -inf, leave without tokens over a long range of ids take a path
+    of milliseconds, as do rows of equal logits in numbers.
     """
     per_row, everywhere = _temperature(temperature)
     return TopLogits(*_ops.top_logits(logits, k, per_row, everywhere, mask))
@@ -144,7 +148,9 @@ def policy_loss(logits, tokens, old_logprobs, advantages, *, ref_logprobs=None, 
 
     ``tokens``, ``temperature`` and ``mask`` are ``token_logprobs``'s: with
     the temperature and masks the tokens were sampled under, the ratio is that
-    of the distributions they came from. ``old_logprobs``, ``advantages``,
+    of the distributions they came from, if those were not truncated by top-k,
+    top-p or min-p (probabilities here are over all allowed tokens).
+    ``old_logprobs``, ``advantages``,
     ``ref_logprobs`` and ``weights`` are float32 [rows]. The clip range of the
     ratio is [1 - clip_low, 1 + clip_high]. ``loss`` is differentiable by the
     logits; the other outputs are for monitoring.

@@ -252,14 +252,20 @@ int es_ipc_free(void* ptr);
  *
  * Statuses are per row and follow es_verify's: ES_INVALID_INPUT for a NaN or
  * +inf logit anywhere in the row (behind the mask too), for a temperature
- * that is not positive and finite (or beyond float32's range) and for any
- * other per-row input that is not finite or out of range, except weights and
- * incoming gradients, which multiply as they are; ES_NO_VALID_TOKEN
+ * that is not positive and finite (or beyond float32's range; 0 is not greedy
+ * here), for any other per-row input that is not finite or out of range,
+ * except weights and incoming gradients, which multiply as they are, and for a
+ * loss that is beyond float32's range before its weight; ES_NO_VALID_TOKEN
  * when no token is allowed or every allowed one is -inf; ES_DRAFT_ZERO_PROB
  * when a token that the operator needs has probability zero. A row whose
  * status is not ES_OK has log-probability -inf, loss, KL and entropy 0, and
  * a gradient of zeros. A log-probability below float32's range (the type's
  * lowest logit over a temperature below 1) is float32's lowest number.
+ *
+ * All arithmetic is float32's, of which a row's sum is off by 1e-6 at most or
+ * so, relatively: log-probabilities and entropies by as much beside their own
+ * rounding. No log-probability is above 0, and no entropy, KL or distillation
+ * loss below.
  *
  * Every tensor is aligned to its elements (ES_ERR_ALIGNMENT), with any strides
  * that are not negative. A gradient has the logits' type and shape. It may be
@@ -289,7 +295,9 @@ typedef struct es_logprob_args {
 int es_token_logprobs(const es_logprob_args* args, void* stream);
 
 /* The k largest logits of each row, in descending order and the lowest id
- * first among equal ones, and the rest's log-sum:
+ * first among equal ones, and the rest's log-sum (rows that a mask or -inf
+ * leaves without tokens over a long range of ids take milliseconds, and rows of
+ * equal logits do):
  *   rest = log(sum over the other tokens of exp(x[j])), -inf if there is none.
  * Entries beyond the row's allowed tokens have id -1 and value -inf. So does
  * every entry of a row whose status is not ES_OK; its rest is -inf. */
@@ -309,11 +317,10 @@ int es_top_logits(const es_top_args* args, void* stream);
  *          where it is beyond)
  *   loss = weights * (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
  *                     + kl_coef * kl - entropy_coef * H).
- * Where r A equals the clipped product the gradient goes through r. A row whose
- * loss, before its weight, or whose gradient by log p[token] is beyond
- * float32's range is ES_INVALID_INPUT; with kl_coef 0 the KL takes no part in
- * either. Negative tokens as in es_token_logprobs. With `grad`: the gradient of
- * the losses' sum. */
+ * Where r A equals the clipped product the gradient goes through r. A gradient by
+ * log p[token] beyond float32's range is ES_INVALID_INPUT as a loss is; with
+ * kl_coef 0 the KL takes no part in either. Negative tokens as in
+ * es_token_logprobs. With `grad`: the gradient of the losses' sum. */
 typedef struct es_policy_args {
   es_rows in;
   es_tensor tokens;        /* i64 [rows] */
